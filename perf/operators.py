@@ -317,6 +317,10 @@ def work(case):
 
 
 # ------------------------------------------------- the definition in 64 bits
+def _power(p):
+    return torch.ldexp(torch.ones_like(p), p.int())
+
+
 def _q64(x):
     """Quantised values by arithmetic alone: the block's power of two, then the nearest multiple of the step that
     three mantissa bits leave at the value's exponent (never below 2^-6), halves to even."""
@@ -324,9 +328,13 @@ def _q64(x):
     for k0 in range(0, x.shape[1], BLOCK):
         b = x[:, k0:k0 + BLOCK]
         amax = b.abs().amax(1, keepdim=True)
-        s = torch.exp2(torch.ceil(torch.log2((amax / 448.0).clamp(min=2.0 ** -110))))
+        r = (amax / 448.0).clamp(min=2.0 ** -110)
+        s = _power(torch.ceil(torch.log2(r)))
+        s = torch.where(s < r, 2 * s, torch.where(s >= 2 * r, s / 2, s))  # log2 rounds
         v = b / s
-        step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3.0)
+        a = v.abs().clamp(min=2.0 ** -6)
+        t = _power(torch.floor(torch.log2(a)))
+        step = torch.where(t > a, t / 2, torch.where(2 * t <= a, 2 * t, t)) / 8
         out[:, k0:k0 + BLOCK] = torch.round(v / step) * step * s
     return out
 
