@@ -11,6 +11,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
@@ -42,15 +43,18 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not _stale():
         return OUT
     BUILD_DIR.mkdir(exist_ok=True)
-    objs = []
-    for src in sources():
+
+    def compile_one(src: Path) -> str:
         obj = BUILD_DIR / (src.stem + ".o")
         cmd = [NVCC, *ARCH, *FLAGS, "-c", str(src), "-o", str(obj)]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
-        objs.append(str(obj))
+        return str(obj)
+
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        objs = list(pool.map(compile_one, sources()))
     tmp = OUT.with_suffix(".so.tmp")
     subprocess.run([NVCC, *ARCH, "-shared", "-o", str(tmp), *objs], check=True)
     os.replace(tmp, OUT)

@@ -1,0 +1,135 @@
+// Rows and weights to block-scaled e4m3 (the rule in fp8.cuh).
+//
+// Rows: bound by HBM (2 or 4 bytes in, 1 out).  16 lanes hold one block of
+// 128 values, 8 each (one 16-byte load of bf16), so the maximum is four
+// shuffles and a warp stores 256 consecutive bytes.  With slot_pos a row is
+// read once and written to each of its k expert-sorted places: the gather of
+// the bf16 path costs no pass of its own.
+#include "fp8.cuh"
+
+namespace {
+using namespace frank;
+
+template <class TX>
+__device__ __forceinline__ void load8(const TX* p, float (&v)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+template <class TX>
+__global__ void __launch_bounds__(256)
+quantize_rows_kernel(const TX* __restrict__ x, int64_t T, int64_t K, int nb, const int32_t* __restrict__ slot_pos,
+                     int k, uint8_t* __restrict__ q, float* __restrict__ q_scale) {
+  pdl_wait();
+  pdl_launch();
+  const int half = (threadIdx.x >> 4) & 1, l16 = threadIdx.x & 15;
+  const int pairs = (nb + 1) >> 1;
+  const int64_t warp = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), nwarps = (int64_t)gridDim.x * 8;
+  const int64_t R = slot_pos != nullptr ? T * k : T;
+  for (int64_t i = warp; i < T * pairs; i += nwarps) {
+    const int64_t t = i / pairs;
+    const int b = (int)(i % pairs) * 2 + half;
+    const int64_t c = (int64_t)b * kQB + l16 * 8;
+    float v[8] = {};
+    if (c < K) load8(x + t * K + c, v);
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
+#pragma unroll
+    for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const BlockScale s = block_scale(m);
+    uint2 u;
+    u.x = e4m3x4(v[0] * s.inv, v[1] * s.inv, v[2] * s.inv, v[3] * s.inv);
+    u.y = e4m3x4(v[4] * s.inv, v[5] * s.inv, v[6] * s.inv, v[7] * s.inv);
+    if (c < K) {
+      for (int j = 0; j < k; ++j) {
+        const int64_t r = slot_pos != nullptr ? (int64_t)slot_pos[j * T + t] : t;
+        *reinterpret_cast<uint2*>(q + r * K + c) = u;
+        if (l16 == 0) q_scale[b * R + r] = s.scale;
+      }
+    }
+  }
+}
+
+// [O, I, E] -> [E, O, I]: one block for each 128 x 128 block of (o, i) and all
+// experts.  The first pass finds each expert's maximum (values of one o are
+// contiguous over (i, e)), the second writes runs along i.  Done once.
+template <class TX>
+__global__ void __launch_bounds__(256)
+prepack_fp8_kernel(const TX* __restrict__ src, int64_t O, int64_t I, int64_t E, uint8_t* __restrict__ q,
+                   float* __restrict__ scale) {
+  extern __shared__ uint32_t amax[];  // [E], then the inverse scales
+  const int64_t o0 = (int64_t)blockIdx.y * kQB, i0 = (int64_t)blockIdx.x * kQB;
+  const int64_t on = min((int64_t)kQB, O - o0), in = min((int64_t)kQB, I - i0);
+  for (int64_t e = threadIdx.x; e < E; e += 256) amax[e] = 0;
+  __syncthreads();
+  for (int64_t o = 0; o < on; ++o) {
+    const TX* row = src + ((o0 + o) * I + i0) * E;
+    for (int64_t j = threadIdx.x; j < in * E; j += 256) atomicMax(&amax[j % E], abs_bits(load_as_f32(row, j)));
+  }
+  __syncthreads();
+  for (int64_t e = threadIdx.x; e < E; e += 256) {
+    const BlockScale s = block_scale(amax[e]);
+    scale[(e * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = s.scale;
+    amax[e] = __float_as_uint(s.inv);
+  }
+  __syncthreads();
+  for (int64_t o = 0; o < on; ++o) {
+    const TX* row = src + ((o0 + o) * I + i0) * E;
+    for (int64_t j = threadIdx.x; j < in * E; j += 256) {
+      const int64_t e = j / in, i = j % in;
+      const float v = load_as_f32(row, i * E + e) * __uint_as_float(amax[e]);
+      q[(e * O + o0 + o) * I + i0 + i] = (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+    }
+  }
+}
+
+}  // namespace
+
+namespace frank {
+
+int launch_quantize_rows(int x_dtype, const void* x, int64_t T, int64_t K, const int32_t* slot_pos, int64_t k,
+                         void* q, float* q_scale, cudaStream_t st) {
+  if (T == 0) return FRANK_OK;
+  const int nb = (int)q_blocks(K);
+  const int64_t warps = T * ((nb + 1) / 2), cap = (int64_t)num_sms() * 8;
+  const int64_t blocks = (warps + 7) / 8;
+  const dim3 grid((unsigned)(blocks < cap ? blocks : cap));
+  cudaError_t e;
+  if (x_dtype == FRANK_F32)
+    e = launch_chained(quantize_rows_kernel<float>, grid, dim3(256), 0, st, 1, (const float*)x, T, K, nb, slot_pos,
+                       (int)k, (uint8_t*)q, q_scale);
+  else
+    e = launch_chained(quantize_rows_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, 1, (const __nv_bfloat16*)x, T, K,
+                       nb, slot_pos, (int)k, (uint8_t*)q, q_scale);
+  FRANK_CUDA_TRY(e);
+  FRANK_LAUNCH_CHECK();
+  return FRANK_OK;
+}
+
+int launch_prepack_fp8(int in_dtype, const void* src, int64_t O, int64_t I, int64_t E, void* q, float* scale,
+                       cudaStream_t st) {
+  if (O == 0 || I == 0 || E == 0) return FRANK_OK;
+  const dim3 grid((unsigned)q_blocks(I), (unsigned)q_blocks(O));
+  if (in_dtype == FRANK_F32)
+    prepack_fp8_kernel<float><<<grid, 256, E * 4, st>>>((const float*)src, O, I, E, (uint8_t*)q, scale);
+  else
+    prepack_fp8_kernel<__nv_bfloat16><<<grid, 256, E * 4, st>>>((const __nv_bfloat16*)src, O, I, E, (uint8_t*)q,
+                                                                scale);
+  FRANK_LAUNCH_CHECK();
+  return FRANK_OK;
+}
+
+}  // namespace frank

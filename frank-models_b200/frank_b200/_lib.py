@@ -15,6 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libfrankmoe.so"
 
 F32 = 0
 BF16 = 1
+FP8_BLOCK = 128  # FRANK_FP8_BLOCK
 ROUTER_PACKED = 16  # wr_dtype of a router pack (frank_router_pack)
 
 OK = 0
@@ -30,7 +31,7 @@ _c_int = ctypes.c_int
 _c_vp = ctypes.c_void_p
 _c_size = ctypes.c_size_t
 
-# name -> (restype, argtypes); mirrors include/frank_moe.h one to one.
+# name -> (restype, argtypes); mirrors include/frank_moe.h and include/frank_fp8.h one to one.
 SIGNATURES = {
     "frank_last_error": (ctypes.c_char_p, []),
     "frank_abi_version": (_c_int, []),
@@ -75,6 +76,23 @@ SIGNATURES = {
     "frank_selftest_bounded_wait": (_c_int, [_c_i64, _c_vp, _c_vp]),
     "frank_profile_stages": (_c_int, [_c_int]),
     "frank_profile_read": (_c_int, [_c_vp, _c_int, _c_vp]),
+    "frank_quantize_fp8": (_c_int, [_c_int, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp]),
+    "frank_rms_norm_fp8": (_c_int, [_c_int, _c_vp, _c_vp, _c_i64, _c_i64, ctypes.c_float, _c_vp, _c_vp, _c_vp,
+                                    _c_vp]),
+    "frank_prepack_experts_fp8": (_c_int, [_c_int, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp]),
+    "frank_fp8_matmul": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_vp,
+                                  _c_vp]),
+    "frank_fp8_moe_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
+    "frank_fp8_moe_experts": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64,
+                                       _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_size, _c_vp]),
+    "frank_fp8_moe_block": (_c_int, [_c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64,
+                                     _c_i64, _c_i64, _c_i64, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_size,
+                                     _c_vp]),
+    "frank_fp8_moe_sublayer": (_c_int, [_c_int, _c_vp, _c_vp, ctypes.c_float, _c_int, _c_vp, _c_vp, _c_vp, _c_vp,
+                                        _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_vp,
+                                        _c_vp, _c_i64, ctypes.c_float, _c_vp, _c_vp, _c_vp, _c_vp, _c_size, _c_vp]),
+    "frank_post_norm_residual": (_c_int, [_c_int, _c_vp, _c_int, _c_vp, _c_vp, ctypes.c_float, _c_vp, _c_i64,
+                                          ctypes.c_float, _c_vp, _c_vp, _c_int, _c_vp, _c_i64, _c_i64, _c_vp]),
 }
 
 _lib = None

@@ -25,7 +25,7 @@ from typing import Mapping
 import numpy as np
 import torch
 
-from . import ops
+from . import fp8, ops
 
 _SUFFIXES = ("ffn_gate_inp.weight", "ffn_up_exps.weight", "ffn_gate_exps.weight", "ffn_down_exps.weight")
 
@@ -92,6 +92,21 @@ def pack_reference_experts(w_oie, dtype: torch.dtype, device, chunk_bytes: int =
     return ops.PackedExperts(packed)
 
 
+def quantize_reference_experts(w_oie, device, chunk_bytes: int = 256 << 20) -> fp8.Fp8Experts:
+    """[O, I, E] reference-layout expert tensor (numpy or torch, any device)
+    -> Fp8Experts on ``device``, uploading and quantising whole blocks of 128
+    rows, about ``chunk_bytes`` of fp32 at a time."""
+    O, I, E = _shape(w_oie)
+    q = torch.empty((E, O, I), dtype=torch.float8_e4m3fn, device=device)
+    scale = torch.empty((E, -(-O // fp8.BLOCK), -(-I // fp8.BLOCK)), dtype=torch.float32, device=device)
+    rows = max(1, chunk_bytes // max(1, fp8.BLOCK * I * E * 4)) * fp8.BLOCK
+    for o0 in range(0, O, rows):
+        part = fp8.Fp8Experts.from_reference(_to_device(w_oie[o0:o0 + rows], device))
+        q[:, o0:o0 + rows].copy_(part.q)
+        scale[:, o0 // fp8.BLOCK:o0 // fp8.BLOCK + part.scale.shape[1]].copy_(part.scale)
+    return fp8.Fp8Experts(q, scale)
+
+
 class MoELayer:
     """One layer's MoE FFN: the packed block and (when present) the
     sub-layer's rms_norm weight."""
@@ -116,14 +131,18 @@ def moe_layer_from_params(params: Mapping[str, object], layer_idx: int, n_expert
                           chunk_bytes: int = 256 << 20) -> MoELayer:
     """Build layer ``layer_idx``'s MoE FFN from a name -> array mapping
     (numpy or torch; the reference's fp32 tensors).  Expert weights are packed
-    to ``dtype`` (bf16: tensor-core path; fp32: FFMA path); the router and
-    the norm weight stay fp32."""
+    to ``dtype`` (bf16: tensor-core path; fp32: FFMA path; float8_e4m3fn: the
+    8-bit path, tokens in bf16); the router and the norm weight stay fp32."""
     shapes = moe_param_shapes(params, layer_idx)
     if not (1 <= n_expert_used <= shapes.n_expert):
         raise ValueError(f"n_expert_used={n_expert_used} outside [1, {shapes.n_expert}]")
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     n = param_names(layer_idx)
     wr = _to_device(params[n["router"]], dev)
+    if dtype == torch.float8_e4m3fn:
+        wu, wg, wd = (quantize_reference_experts(params[n[key]], dev, chunk_bytes) for key in ("up", "gate", "down"))
+        block = fp8.Fp8MoEFFNBlock(wr, wu, wg, wd, shapes.n_expert, n_expert_used, normalize_weights)
+        return MoELayer(block, _to_device(params[n["norm"]], dev) if shapes.has_norm else None)
     wu, wg, wd = (pack_reference_experts(params[n[key]], dtype, dev, chunk_bytes) for key in ("up", "gate", "down"))
     block = ops.MoEFFNBlock(wr, wu, wg, wd, shapes.n_expert, n_expert_used, normalize_weights, dtype=dtype)
     norm = _to_device(params[n["norm"]], dev) if shapes.has_norm else None
