@@ -1,104 +1,601 @@
-// Grouped product of block-scaled e4m3 rows and weights.
+// Grouped product of block-scaled e4m3 rows and weights on the 5th-generation
+// tensor cores (tcgen05 + TMEM), fed by TMA.
 //
 //   y[r, n] = sum_b a_scale[b, r] * w_scale[e, n/128, b] * sum_{k in b} a[r, k] * w[e, n, k]
 //
-// A block of 128 threads owns 16 rows of one expert and 128 columns, one column
-// for each thread: the columns of one scale block, and with SWIGLU the values
-// that share a scale of h.
+// The scales differ from block to block along K, so the tensor core sums one
+// block of 128 (four tcgen05.mma.kind::f8f6f4 of K = 32) into TMEM and the
+// epilogue warps multiply that partial tile by the two scales and add it to
+// fp32 accumulators in registers, while the tensor core fills the other of two
+// TMEM buffers.  Per K block and SM the tensor core needs 512 cycles for
+// 128 x 256 x 128, the eight epilogue warps read 128 KB of TMEM and issue 128
+// packed FMAs each: both overlap, the tensor core stays the bound of large
+// groups.  Small groups are bound by the weights from HBM.
+//
+// Structure (persistent, 384 threads, one CTA per SM):
+//   warp 0      TMA producer: A 128 x 128 bytes and B 256 x 128 bytes a stage (SWIZZLE_128B)
+//   warp 1      TMEM allocator and MMA issuer
+//   warps 4..11 epilogue: two warps for each TMEM lane quadrant, each half of the columns;
+//               128 accumulators a thread, so they take registers from the first four warps
+// CG = 2: two CTAs on two SMs share a tile of 256 rows (cta_group::2); each
+// loads its 128 rows of A and half of B, 32 KB instead of 48 KB a K block.
+// Every wait is bounded (about 2 s); on expiry the CTA records FRANK_ETIMEOUT in
+// the device error word and unwinds, freeing its TMEM.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "fp8.cuh"
+#include "mbarrier.cuh"
 
 namespace {
 using namespace frank;
+using namespace frank_mbar;
 
-constexpr int kRows = 16;
-constexpr int kLd = kQB + 4;
+constexpr int BM = 128, BN = 256, BK = kQB;  // rows of one CTA, columns, bytes along K
+constexpr int kThreads = 384, kEpiWarps = 8;
+// registers a thread: 128 x 64 + 256 x 216 = 63,488 of the 384 x 168 = 64,512 at launch
+constexpr int kRegsLaunch = 168, kRegsFew = 64, kRegsEpilogue = 216;
+static_assert(128 * kRegsFew + 256 * kRegsEpilogue <= kThreads * kRegsLaunch);
+constexpr uint32_t kTileBytes = 128 * BK;  // 16 KiB: 128 rows of A or of B
+constexpr uint32_t kEpiBytes = kEpiWarps * 2048;
+constexpr uint32_t kTmemCols = 512;
+
+template <int CG>
+struct Shape {
+  static constexpr int kStages = CG == 1 ? 4 : 6;
+  static constexpr uint32_t kStageBytes = CG == 1 ? 3 * kTileBytes : 2 * kTileBytes;
+  static constexpr int kRows = CG * BM;  // rows of a tile
+  // kind::f8f6f4: D fp32 [4,6)=1, A and B e4m3 [7,10)=[10,13)=0, N>>3 at [17,23), M>>4 at [24,29)
+  static constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+  static constexpr size_t smem(int64_t E) {
+    return 1024 + kStages * kStageBytes + kEpiBytes + 2048 + 8 * (2 * kStages + 8) + 16 + 4 * (E + 1) + 64;
+  }
+};
+
+struct Maps {
+  CUtensorMap a[4];  // boxes of 128, 64, 32 and 16 rows
+  CUtensorMap w, w2;
+};
 
 struct Params {
-  const uint8_t* a;
   const float* a_scale;
-  const uint8_t* w[2];
-  const float* w_scale[2];
+  const float* w_scale;
+  const float* w2_scale;
   const int32_t* offsets;
-  int E;
-  int64_t rows, N, K;
+  int E, rows, n_tiles, N, nk, nb_n;
+  int band;  // row tiles whose rows of A stay in L2 while the CTAs sweep the columns
   const float* wrow;
   int out_dtype;
   void* out;
   float* h_scale;
+  int32_t* err;
 };
 
+// Bounded wait without a call: the epilogue waits with 128 live accumulators.
+__device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, volatile int* abort, int32_t* err) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 255u) {
+      if (*abort) return false;
+      const uint64_t now = global_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > 2000000000ull) {
+        *abort = 1;
+        atomicExch(err, FRANK_ETIMEOUT);
+        return false;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------ PTX glue --
+template <int CG>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+        "%4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// K-major operand, 128-byte swizzle: rows of 128 bytes, groups of 8 rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <int CG>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+  constexpr uint32_t idesc = Shape<CG>::kIdesc;
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Arrives when the MMAs issued so far are done: here, or at this offset in both CTAs of the pair.
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// acc[0..31] += v[0..31] * s, two lanes of the pair of floats at a time
+__device__ __forceinline__ void scale_add(float* acc, const uint32_t (&v)[32], float s) {
+  uint64_t s2;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(s));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    uint64_t a, b;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(acc[2 * i]), "f"(acc[2 * i + 1]));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "r"(v[2 * i]), "r"(v[2 * i + 1]));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(b), "l"(s2));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[2 * i]), "=f"(acc[2 * i + 1]) : "l"(a));
+  }
+}
+
+// ---------------------------------------------------------------- tiles --
+struct Tile {
+  int e, m0, m_end, n;
+};
+
+// First row of group e; offsets outside [0, rows] cannot lead out of the buffers.
+__device__ __forceinline__ int group_at(const Params& p, int e) {
+  return p.offsets != nullptr ? min(max(p.offsets[e], 0), p.rows) : (e == 0 ? 0 : p.rows);
+}
+
+__device__ __forceinline__ Tile tile_at(int t, const int* prefix, const Params& p, int rows) {
+  int lo = 0, hi = p.E;  // prefix[lo] <= t < prefix[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= t) lo = mid; else hi = mid;
+  }
+  const int r0 = group_at(p, lo), r1 = group_at(p, lo + 1);
+  const int mt = (r1 - r0 + rows - 1) / rows;
+  const int local = t - prefix[lo];
+  const int band = local / (p.band * p.n_tiles);
+  const int gm = min(p.band, mt - band * p.band);
+  const int in = local - band * p.band * p.n_tiles;
+  return Tile{lo, r0 + (band * p.band + in % gm) * rows, r1, in / gm};
+}
+
+// Rows of a warp's tile to global memory through 2 KB of shared memory: 32
+// rows of 64 bytes, chunk c of row r at c ^ (r / 2 % 4), so that the row-wise
+// writes and the reads of 8 rows x 64 bytes are both free of bank conflicts.
+__device__ __forceinline__ void put_rows(uint4* stage, const uint4 (&v)[4], char* out, int64_t ld_bytes, int row0,
+                                         int row_end, int col_bytes, int end_bytes) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 4; ++c) stage[lane * 4 + (c ^ ((lane >> 1) & 3))] = v[c];
+  __syncwarp();
+  const int c = lane & 3, at = col_bytes + c * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    const uint4 u = stage[r * 4 + (c ^ ((r >> 1) & 3))];
+    if (row0 + r < row_end && at < end_bytes) *reinterpret_cast<uint4*>(out + (row0 + r) * ld_bytes + at) = u;
+  }
+}
+
+// --------------------------------------------------------------- kernel --
 template <int MODE>
-__global__ void __launch_bounds__(128) fp8_gemm_simple_kernel(const Params p) {
-  constexpr int NW = MODE == FP8_SWIGLU ? 2 : 1;
-  __shared__ float as[kRows][kQB];
-  __shared__ uint8_t ws[NW][kQB][kLd];
-  __shared__ uint32_t amax[kRows];
+__device__ __forceinline__ bool tile_out(const Params& p, const Tile& tl, int row0, int half, float* acc,
+                                         uint4* stage, uint32_t* amax, int quad, uint32_t parity, uint32_t row_bar,
+                                         volatile int* abort_flag) {
+  const int lane = threadIdx.x & 31, row = row0 + lane;
+  if constexpr (MODE == FP8_SWIGLU) {
+    // acc[0..63]: gate, acc[64..127]: up, columns half * 64 + 0..63 of this block of F
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+      acc[i] *= silu_ref(acc[64 + i]);
+      m = max(m, abs_bits(acc[i]));
+    }
+    // the row's other 64 columns are in the other warp of this quadrant
+    uint32_t* mine = amax + parity * 256 + quad * 32 + lane;
+    mine[half * 128] = m;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(row_bar);
+    if (!wait_inline(row_bar, parity, abort_flag, p.err)) return false;
+    m = max(m, mine[(half ^ 1) * 128]);
+    const BlockScale s = block_scale(m);
+    uint4 v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float* a = acc + c * 16 + j * 4;
+        w[j] = e4m3x4(a[0] * s.inv, a[1] * s.inv, a[2] * s.inv, a[3] * s.inv);
+      }
+      v[c] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    put_rows(stage, v, static_cast<char*>(p.out), p.N, row0, tl.m_end, tl.n * 128 + half * 64, p.N);
+    if (half == 0 && row < tl.m_end) p.h_scale[(int64_t)tl.n * p.rows + row] = s.scale;
+  } else {
+    float s = 1.f;
+    if (MODE == FP8_SCALE && row < tl.m_end) s = p.wrow[row];
+    const int col = tl.n * BN + half * 128;
+    if (p.out_dtype == FRANK_F32) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float* a = acc + c * 16 + j * 4;
+          v[j] = make_uint4(__float_as_uint(a[0] * s), __float_as_uint(a[1] * s), __float_as_uint(a[2] * s),
+                            __float_as_uint(a[3] * s));
+        }
+        put_rows(stage, v, static_cast<char*>(p.out), (int64_t)p.N * 4, row0, tl.m_end, (col + c * 16) * 4, p.N * 4);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float* a = acc + c * 32 + j * 8;
+          v[j] = make_uint4(pack_bf16x2(a[0] * s, a[1] * s), pack_bf16x2(a[2] * s, a[3] * s),
+                            pack_bf16x2(a[4] * s, a[5] * s), pack_bf16x2(a[6] * s, a[7] * s));
+        }
+        put_rows(stage, v, static_cast<char*>(p.out), (int64_t)p.N * 2, row0, tl.m_end, (col + c * 32) * 2, p.N * 2);
+      }
+    }
+  }
+  return true;
+}
+
+template <int MODE, int CG>
+__device__ __forceinline__ void fp8_gemm_body(const Maps& maps, const Params& p) {
+  using S = Shape<CG>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* epi = smem + S::kStages * S::kStageBytes;
+  uint32_t* amax = reinterpret_cast<uint32_t*>(epi + kEpiBytes);  // [2 parities][2 halves][128 rows]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(epi + kEpiBytes + 2048);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::kStages + 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* prefix = reinterpret_cast<int*>(tmem_slot + 4);  // [E + 1]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t rank = 0;
+  if constexpr (CG == 2) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  const uint32_t bar0 = smem_u32(bars);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (S::kStages + s); };
+  auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * S::kStages + a); };
+  auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * S::kStages + 2 + a); };
+  auto row_bar = [&](int quad) { return bar0 + 8u * (2 * S::kStages + 4 + quad); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), kEpiWarps * CG);
+    }
+    for (int q = 0; q < 4; ++q) mbar_init(row_bar(q), 2);  // the two warps of a quadrant
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    if constexpr (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(kTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(kTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+  }
   pdl_wait();
   pdl_launch();
-  int e = 0;
-  int64_t r0 = 0, r1 = 0, tile = blockIdx.x;
-  for (; e < p.E; ++e) {
-    r0 = p.offsets != nullptr ? p.offsets[e] : 0;
-    r1 = p.offsets != nullptr ? p.offsets[e + 1] : p.rows;
-    const int64_t tiles = (r1 - r0 + kRows - 1) / kRows;
-    if (tile < tiles) break;
-    tile -= tiles;
-  }
-  if (e == p.E) return;
-  r0 += tile * kRows;
-  const int nr = (int)min((int64_t)kRows, r1 - r0);
-  const int64_t n0 = (int64_t)blockIdx.y * kQB, n = n0 + threadIdx.x;
-  const int nb = (int)((p.K + kQB - 1) / kQB);
-  float acc[NW][kRows] = {};
-  for (int b = 0; b < nb; ++b) {
-    const int64_t k0 = (int64_t)b * kQB;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kRows * kQB; i += 128) {
-      const int r = i / kQB, c = i % kQB;
-      as[r][c] = r < nr && k0 + c < p.K ? e4m3_to_f32(p.a[(r0 + r) * p.K + k0 + c]) : 0.f;
-    }
-    for (int m = 0; m < NW; ++m)
-      for (int i = threadIdx.x; i < kQB * kQB; i += 128) {
-        const int r = i / kQB, c = i % kQB;
-        ws[m][r][c] = n0 + r < p.N && k0 + c < p.K ? p.w[m][((int64_t)e * p.N + n0 + r) * p.K + k0 + c] : 0;
-      }
-    __syncthreads();
-    for (int m = 0; m < NW; ++m) {
-      float part[kRows] = {};
-      for (int c = 0; c < kQB; ++c) {
-        const float w = e4m3_to_f32(ws[m][threadIdx.x][c]);
+  if (warp == 0) {  // prefix[e] = tiles of the experts before e
+    int carry = 0;
+    for (int base = 0; base < p.E; base += 32) {
+      const int e = base + lane;
+      const int v =
+          e < p.E ? (max(group_at(p, e + 1) - group_at(p, e), 0) + S::kRows - 1) / S::kRows * p.n_tiles : 0;
+      int incl = v;
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) part[r] = fmaf(as[r][c], w, part[r]);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
       }
-      const float sw = p.w_scale[m][((int64_t)e * gridDim.y + blockIdx.y) * nb + b];
-      for (int r = 0; r < kRows; ++r)
-        if (r < nr) acc[m][r] = fmaf(part[r], p.a_scale[b * p.rows + r0 + r] * sw, acc[m][r]);
+      if (e < p.E) prefix[e] = carry + incl - v;
+      carry += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) prefix[p.E] = carry;
+  }
+  fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // the peer's barriers are initialised before any remote use
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int total = prefix[p.E];
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
+    if (warp == 0 && lane == 0) {
+      // ---------------------------------------------- TMA producer --
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = first; t < total && ok; t += step) {
+        const Tile tl = tile_at(t, prefix, p, S::kRows);
+        // a small group needs few rows of A: boxes of 128, 64, 32 or 16 rows
+        int box = 0;
+        if (CG == 1)
+          while (box < 3 && tl.m_end - tl.m0 <= (64 >> box)) ++box;
+        const uint32_t a_bytes = CG == 1 ? kTileBytes >> box : kTileBytes;
+        for (int kb = 0; kb < p.nk; ++kb, ++it) {
+          const int s = it % S::kStages;
+          if (!wait_inline(empty_bar(s), ((it / S::kStages) & 1u) ^ 1u, abort_flag, p.err)) {
+            ok = false;
+            break;
+          }
+          const uint32_t st = smem_u32(smem + s * S::kStageBytes);
+          if constexpr (CG == 1) {
+            mbar_expect_tx(full_bar(s), a_bytes + 2 * kTileBytes);
+            load_2d<1>(st, &maps.a[box], kb * BK, tl.m0, full_bar(s));
+            if constexpr (MODE == FP8_SWIGLU) {
+              load_3d<1>(st + kTileBytes, &maps.w, kb * BK, tl.n * 128, tl.e, full_bar(s));
+              load_3d<1>(st + 2 * kTileBytes, &maps.w2, kb * BK, tl.n * 128, tl.e, full_bar(s));
+            } else {
+              load_3d<1>(st + kTileBytes, &maps.w, kb * BK, tl.n * BN, tl.e, full_bar(s));
+              load_3d<1>(st + 2 * kTileBytes, &maps.w, kb * BK, tl.n * BN + 128, tl.e, full_bar(s));
+            }
+          } else {
+            if (rank == 0) mbar_expect_tx(full_bar(s), 2 * S::kStageBytes);
+            const uint32_t fb = mapa(full_bar(s), 0);
+            load_2d<2>(st, &maps.a[0], kb * BK, tl.m0 + (int)rank * BM, fb);
+            if constexpr (MODE == FP8_SWIGLU)
+              load_3d<2>(st + kTileBytes, rank == 0 ? &maps.w : &maps.w2, kb * BK, tl.n * 128, tl.e, fb);
+            else
+              load_3d<2>(st + kTileBytes, &maps.w, kb * BK, tl.n * BN + (int)rank * 128, tl.e, fb);
+          }
+        }
+      }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      // ----------------------------------------------- MMA issuer --
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = first; t < total && ok; t += step) {
+        for (int kb = 0; kb < p.nk; ++kb, ++it) {
+          const int s = it % S::kStages;
+          const uint32_t a = it & 1u;
+          if (!wait_inline(tempty_bar(a), ((it >> 1) & 1u) ^ 1u, abort_flag, p.err) ||
+              !wait_inline(full_bar(s), (it / S::kStages) & 1u, abort_flag, p.err)) {
+            ok = false;
+            break;
+          }
+          fence_after();
+          const uint32_t st = smem_u32(smem + s * S::kStageBytes);
+          const uint64_t ad = smem_desc(st), bd = smem_desc(st + kTileBytes);
+#pragma unroll
+          for (int j = 0; j < BK / 32; ++j)  // 32 bytes along K inside the swizzled row
+            mma<CG>(tmem + a * BN, ad + (uint64_t)(2 * j), bd + (uint64_t)(2 * j), j != 0);
+          commit<CG>(empty_bar(s));
+          commit<CG>(tfull_bar(a));
+        }
+      }
+    }
+  } else {
+    // -------------------------------------------------- epilogue --
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
+    const int quad = warp & 3, half = (warp - 4) >> 2;
+    uint4* stage = reinterpret_cast<uint4*>(epi + (warp - 4) * 2048);
+    // columns of this warp: SWIGLU 64 of gate and the same 64 of up, else 128 in a row
+    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+    const uint32_t col0 = MODE == FP8_SWIGLU ? half * 64 : half * 128;
+    const uint32_t col1 = MODE == FP8_SWIGLU ? 128 + half * 64 : half * 128 + 64;
+    uint32_t it = 0, tiles = 0;  // K blocks; tiles with rows of this warp
+    bool ok = true;
+    for (int t = first; t < total && ok; t += step) {
+      const Tile tl = tile_at(t, prefix, p, S::kRows);
+      const int row0 = tl.m0 + (int)rank * BM + quad * 32;
+      const bool work = row0 < tl.m_end;
+      const float* sa = p.a_scale + min(row0 + lane, p.rows - 1);
+      const int nb = MODE == FP8_SWIGLU ? tl.n : min(2 * tl.n + half, p.nb_n - 1);
+      const float* sw = p.w_scale + ((int64_t)tl.e * p.nb_n + nb) * p.nk;
+      const float* sw2 = p.w2_scale + ((int64_t)tl.e * p.nb_n + nb) * p.nk;
+      float acc[128];
+#pragma unroll
+      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      // scales of the next two K blocks: they come from L2 while the tensor core works
+      float a0 = 0.f, a1 = 0.f, w0 = 0.f, w1 = 0.f, u0 = 0.f, u1 = 0.f;
+      if (work) {
+        a0 = __ldg(sa), w0 = __ldg(sw);
+        if (MODE == FP8_SWIGLU) u0 = __ldg(sw2);
+        if (p.nk > 1) {
+          a1 = __ldg(sa + p.rows), w1 = __ldg(sw + 1);
+          if (MODE == FP8_SWIGLU) u1 = __ldg(sw2 + 1);
+        }
+      }
+#pragma unroll 1
+      for (int kb = 0; kb < p.nk; ++kb, ++it) {
+        const uint32_t a = it & 1u;
+        const float s0 = a0 * w0, s1 = MODE == FP8_SWIGLU ? a0 * u0 : s0;
+        a0 = a1, w0 = w1, u0 = u1;
+        if (work && kb + 2 < p.nk) {
+          a1 = __ldg(sa + (int64_t)(kb + 2) * p.rows), w1 = __ldg(sw + kb + 2);
+          if (MODE == FP8_SWIGLU) u1 = __ldg(sw2 + kb + 2);
+        }
+        if (!wait_inline(tfull_bar(a), (it >> 1) & 1u, abort_flag, p.err)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+        if (work) {
+          const uint32_t ta = tmem + a * BN + lane_base;
+          uint32_t v[32];
+          tmem_ld32(ta + col0, v);
+          tmem_wait();
+          scale_add(acc, v, s0);
+          tmem_ld32(ta + col0 + 32, v);
+          tmem_wait();
+          scale_add(acc + 32, v, s0);
+          tmem_ld32(ta + col1, v);
+          tmem_wait();
+          scale_add(acc + 64, v, s1);
+          tmem_ld32(ta + col1 + 32, v);
+          tmem_wait();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 1) mbar_arrive(tempty_bar(a));
+            else
+              asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa(tempty_bar(a), 0))
+                           : "memory");
+          }
+          scale_add(acc + 96, v, s1);
+        } else {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 1) mbar_arrive(tempty_bar(a));
+            else
+              asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa(tempty_bar(a), 0))
+                           : "memory");
+          }
+        }
+      }
+      if (ok && work)
+        ok = tile_out<MODE>(p, tl, row0, half, acc, stage, amax, quad, tiles++ & 1u, row_bar(quad), abort_flag);
     }
   }
-  if (MODE == FP8_SWIGLU) {
-    if (threadIdx.x < kRows) amax[threadIdx.x] = 0;
-    __syncthreads();
-    for (int r = 0; r < nr; ++r) {
-      acc[0][r] = n < p.N ? acc[0][r] * silu_ref(acc[NW - 1][r]) : 0.f;
-      atomicMax(&amax[r], abs_bits(acc[0][r]));
-    }
-    __syncthreads();
-    for (int r = 0; r < nr; ++r) {
-      const BlockScale s = block_scale(amax[r]);
-      if (n < p.N)
-        static_cast<uint8_t*>(p.out)[(r0 + r) * p.N + n] =
-            (uint8_t)__nv_cvt_float_to_fp8(acc[0][r] * s.inv, __NV_SATFINITE, __NV_E4M3);
-      if (threadIdx.x == 0) p.h_scale[blockIdx.y * p.rows + r0 + r] = s.scale;
-    }
-  } else if (n < p.N) {
-    for (int r = 0; r < nr; ++r) {
-      const float v = MODE == FP8_SCALE ? acc[0][r] * p.wrow[r0 + r] : acc[0][r];
-      if (p.out_dtype == FRANK_F32)
-        static_cast<float*>(p.out)[(r0 + r) * p.N + n] = v;
-      else
-        static_cast<__nv_bfloat16*>(p.out)[(r0 + r) * p.N + n] = __float2bfloat16_rn(v);
-    }
+
+  fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // the leader's MMAs read the peer's shared memory until here
+  if (warp == 1) {
+    fence_after();
+    if constexpr (CG == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  fp8_gemm_body<MODE, 1>(maps, p);
+}
+
+template <int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+fp8_gemm_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  fp8_gemm_body<MODE, 2>(maps, p);
+}
+
+// ------------------------------------------------------------ host side --
+// Map of bytes [E, R, K] (E = 1: two dimensions), box 128 bytes x box_rows, 128-byte swizzle.
+int make_map(CUtensorMap* m, const void* base, int64_t E, int64_t R, int64_t K, uint32_t box_rows, bool three) {
+  static PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }();
+  if (!enc) {
+    frank::set_error("cuTensorMapEncodeTiled unavailable");
+    return FRANK_ECUDA;
+  }
+  const cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)R, (cuuint64_t)E};
+  const cuuint64_t strides[2] = {(cuuint64_t)K, (cuuint64_t)(R * K)};
+  const cuuint32_t box[3] = {BK, box_rows, 1}, estr[3] = {1, 1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, three ? 3 : 2, const_cast<void*>(base), dims, strides, box,
+                         estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    frank::set_error("cuTensorMapEncodeTiled([%lld, %lld, %lld] bytes) failed: %d", (long long)E, (long long)R,
+                     (long long)K, (int)r);
+    return FRANK_ECUDA;
+  }
+  return FRANK_OK;
+}
+
+template <typename Kern>
+int launch(Kern kern, size_t smem, unsigned grid, const Maps& maps, const Params& p, cudaStream_t st) {
+  FRANK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  FRANK_CUDA_TRY(frank::launch_chained(kern, dim3(grid), dim3(kThreads), smem, st, 1, maps, p));
+  FRANK_LAUNCH_CHECK();
+  return FRANK_OK;
 }
 
 }  // namespace
@@ -107,30 +604,46 @@ namespace frank {
 
 int launch_fp8_gemm(const Fp8Gemm& g, cudaStream_t st) {
   if (g.rows == 0) return FRANK_OK;
+  Maps maps;
+  for (int i = 0; i < 4; ++i) FRANK_TRY(make_map(&maps.a[i], g.a, 1, g.rows, g.K, 128u >> i, false));
+  FRANK_TRY(make_map(&maps.w, g.w, g.E, g.N, g.K, 128, true));
+  maps.w2 = maps.w;
+  if (g.mode == FP8_SWIGLU) FRANK_TRY(make_map(&maps.w2, g.w2, g.E, g.N, g.K, 128, true));
   Params p;
-  p.a = (const uint8_t*)g.a;
   p.a_scale = g.a_scale;
-  p.w[0] = (const uint8_t*)g.w;
-  p.w[1] = (const uint8_t*)g.w2;
-  p.w_scale[0] = g.w_scale;
-  p.w_scale[1] = g.w2_scale;
+  p.w_scale = g.w_scale;
+  p.w2_scale = g.mode == FP8_SWIGLU ? g.w2_scale : g.w_scale;
   p.offsets = g.offsets;
   p.E = (int)g.E;
-  p.rows = g.rows;
-  p.N = g.N;
-  p.K = g.K;
+  p.rows = (int)g.rows;
+  p.n_tiles = (int)(g.mode == FP8_SWIGLU ? q_blocks(g.N) : (g.N + BN - 1) / BN);
+  p.N = (int)g.N;
+  p.nk = (int)q_blocks(g.K);
+  p.nb_n = (int)q_blocks(g.N);
   p.wrow = g.wrow;
   p.out_dtype = g.out_dtype;
   p.out = g.out;
   p.h_scale = g.h_scale;
-  const dim3 grid((unsigned)((g.rows + kRows - 1) / kRows + g.E), (unsigned)q_blocks(g.N));
-  cudaError_t e;
-  if (g.mode == FP8_SWIGLU) e = launch_chained(fp8_gemm_simple_kernel<FP8_SWIGLU>, grid, dim3(128), 0, st, 1, p);
-  else if (g.mode == FP8_SCALE) e = launch_chained(fp8_gemm_simple_kernel<FP8_SCALE>, grid, dim3(128), 0, st, 1, p);
-  else e = launch_chained(fp8_gemm_simple_kernel<FP8_PLAIN>, grid, dim3(128), 0, st, 1, p);
-  FRANK_CUDA_TRY(e);
-  FRANK_LAUNCH_CHECK();
-  return FRANK_OK;
+  p.err = device_error_word();
+  // A pair of CTAs wastes up to 255 rows of a tile: for groups of 1024 rows on average.
+  const bool pair = g.rows >= 1024 * g.E && num_sms() >= 2;
+  const int64_t rows = pair ? 2 * BM : BM;
+  // rows of A that the CTAs share through L2 while they sweep the columns: 64 MB
+  int64_t band = (64ll << 20) / g.K / rows;
+  p.band = (int)(band < 1 ? 1 : (band * rows > 8192 ? 8192 / rows : band));
+  const unsigned grid = (unsigned)(pair ? num_sms() & ~1 : num_sms());
+  const size_t smem = pair ? Shape<2>::smem(g.E) : Shape<1>::smem(g.E);
+  switch (g.mode) {
+    case FP8_SWIGLU:
+      return pair ? launch(fp8_gemm_pair_kernel<FP8_SWIGLU>, smem, grid, maps, p, st)
+                  : launch(fp8_gemm_kernel<FP8_SWIGLU>, smem, grid, maps, p, st);
+    case FP8_SCALE:
+      return pair ? launch(fp8_gemm_pair_kernel<FP8_SCALE>, smem, grid, maps, p, st)
+                  : launch(fp8_gemm_kernel<FP8_SCALE>, smem, grid, maps, p, st);
+    default:
+      return pair ? launch(fp8_gemm_pair_kernel<FP8_PLAIN>, smem, grid, maps, p, st)
+                  : launch(fp8_gemm_kernel<FP8_PLAIN>, smem, grid, maps, p, st);
+  }
 }
 
 }  // namespace frank
