@@ -8,17 +8,23 @@
 // epilogue warps multiply that partial tile by the two scales and add it to
 // fp32 accumulators in registers, while the tensor core fills the other of two
 // TMEM buffers.  Per K block and SM the tensor core needs 512 cycles for
-// 128 x 256 x 128, the eight epilogue warps read 128 KB of TMEM and issue 128
-// packed FMAs each: both overlap, the tensor core stays the bound of large
-// groups.  Small groups are bound by the weights from HBM.
+// 128 x 256 x 128, the eight epilogue warps read 128 KB of TMEM and issue 64
+// packed FMAs each, at the same time.  Small groups are bound by the weights from HBM.
 //
 // Structure (persistent, 384 threads, one CTA per SM):
-//   warp 0      TMA producer: A 128 x 128 bytes and B 256 x 128 bytes a stage (SWIZZLE_128B)
+//   warp 0      TMA producer: A 128 x 128 bytes and B 256 x 128 bytes a stage (SWIZZLE_128B), four stages
 //   warp 1      TMEM allocator and MMA issuer
 //   warps 4..11 epilogue: two warps for each TMEM lane quadrant, each half of the columns;
 //               128 accumulators a thread, so they take registers from the first four warps
-// CG = 2: two CTAs on two SMs share a tile of 256 rows (cta_group::2); each
-// loads its 128 rows of A and half of B, 32 KB instead of 48 KB a K block.
+// Tiles are (expert, m, n) with m fastest inside a band of rows that stays in L2.
+//
+// Measured, 8192 x 14336 x 4096: 482 us, 2.0 PFLOP/s; without the epilogue's loads
+// and FMAs the same pipeline takes 396 us, and 364 us without the loads of A as
+// well: the copies from L2 (48 KB a K block, 11 TB/s over all SMs) and the hand-over of
+// the two TMEM buffers bound it together.  Slower: pairs of CTAs (cta_group::2, 256 x
+// 256 tiles, a third less from L2, but a longer hand-over: 501 us), sixteen
+// epilogue warps (724 us), halves of 128 columns with barriers of their own (581 us),
+// TMEM loads one chunk ahead of the FMAs (533 us).
 // Every wait is bounded (about 2 s); on expiry the CTA records FRANK_ETIMEOUT in
 // the device error word and unwinds, freeing its TMEM.
 #include <cuda.h>
@@ -33,24 +39,19 @@ using namespace frank_mbar;
 
 constexpr int BM = 128, BN = 256, BK = kQB;  // rows of one CTA, columns, bytes along K
 constexpr int kThreads = 384, kEpiWarps = 8;
-// registers a thread: 128 x 64 + 256 x 216 = 63,488 of the 384 x 168 = 64,512 at launch
-constexpr int kRegsLaunch = 168, kRegsFew = 64, kRegsEpilogue = 216;
-static_assert(128 * kRegsFew + 256 * kRegsEpilogue <= kThreads * kRegsLaunch);
+// registers a thread: 128 x 40 + 256 x 224 = 62,464 of the 384 x 168 = 64,512 at launch
+constexpr int kRegsLaunch = 168, kRegsFew = 40, kRegsEpilogue = 224;
+static_assert(128 * kRegsFew + 32 * kEpiWarps * kRegsEpilogue <= kThreads * kRegsLaunch, "setmaxnreg would wait");
 constexpr uint32_t kTileBytes = 128 * BK;  // 16 KiB: 128 rows of A or of B
 constexpr uint32_t kEpiBytes = kEpiWarps * 2048;
 constexpr uint32_t kTmemCols = 512;
-
-template <int CG>
-struct Shape {
-  static constexpr int kStages = CG == 1 ? 4 : 6;
-  static constexpr uint32_t kStageBytes = CG == 1 ? 3 * kTileBytes : 2 * kTileBytes;
-  static constexpr int kRows = CG * BM;  // rows of a tile
-  // kind::f8f6f4: D fp32 [4,6)=1, A and B e4m3 [7,10)=[10,13)=0, N>>3 at [17,23), M>>4 at [24,29)
-  static constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-  static constexpr size_t smem(int64_t E) {
-    return 1024 + kStages * kStageBytes + kEpiBytes + 2048 + 8 * (2 * kStages + 8) + 16 + 4 * (E + 1) + 64;
-  }
-};
+constexpr int kStages = 4;
+constexpr uint32_t kStageBytes = 3 * kTileBytes;
+// kind::f8f6f4: D fp32 [4,6)=1, A and B e4m3 [7,10)=[10,13)=0, N>>3 at [17,23), M>>4 at [24,29)
+constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+size_t smem_bytes(int64_t E) {
+  return 1024 + kStages * kStageBytes + kEpiBytes + 2048 + 8 * (2 * kStages + 8) + 16 + 4 * (E + 1) + 64;
+}
 
 struct Maps {
   CUtensorMap a[4];  // boxes of 128, 64, 32 and 16 rows
@@ -91,36 +92,20 @@ __device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, volat
 }
 
 // ------------------------------------------------------------ PTX glue --
-template <int CG>
 __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  if constexpr (CG == 1)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-        "%3}], [%4];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
 }
 
-template <int CG>
 __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  if constexpr (CG == 1)
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-        "[%5];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-        "%4}], [%5];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-        : "memory");
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -132,45 +117,18 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr) {
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-template <int CG>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
-  constexpr uint32_t idesc = Shape<CG>::kIdesc;
-  if constexpr (CG == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(kIdesc), "r"(accumulate)
+      : "memory");
 }
 
-// Arrives when the MMAs issued so far are done: here, or at this offset in both CTAs of the pair.
-template <int CG>
+// Arrives when the MMAs issued so far are done.
 __device__ __forceinline__ void commit(uint32_t bar) {
-  if constexpr (CG == 1)
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-  else
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"((uint16_t)3)
-        : "memory");
-}
-
-__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -209,19 +167,19 @@ __device__ __forceinline__ int group_at(const Params& p, int e) {
   return p.offsets != nullptr ? min(max(p.offsets[e], 0), p.rows) : (e == 0 ? 0 : p.rows);
 }
 
-__device__ __forceinline__ Tile tile_at(int t, const int* prefix, const Params& p, int rows) {
+__device__ __forceinline__ Tile tile_at(int t, const int* prefix, const Params& p) {
   int lo = 0, hi = p.E;  // prefix[lo] <= t < prefix[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (prefix[mid] <= t) lo = mid; else hi = mid;
   }
   const int r0 = group_at(p, lo), r1 = group_at(p, lo + 1);
-  const int mt = (r1 - r0 + rows - 1) / rows;
+  const int mt = (r1 - r0 + BM - 1) / BM;
   const int local = t - prefix[lo];
   const int band = local / (p.band * p.n_tiles);
   const int gm = min(p.band, mt - band * p.band);
   const int in = local - band * p.band * p.n_tiles;
-  return Tile{lo, r0 + (band * p.band + in % gm) * rows, r1, in / gm};
+  return Tile{lo, r0 + (band * p.band + in % gm) * BM, r1, in / gm};
 }
 
 // Rows of a warp's tile to global memory through 2 KB of shared memory: 32
@@ -311,37 +269,34 @@ __device__ __forceinline__ bool tile_out(const Params& p, const Tile& tl, int ro
   return true;
 }
 
-template <int MODE, int CG>
-__device__ __forceinline__ void fp8_gemm_body(const Maps& maps, const Params& p) {
-  using S = Shape<CG>;
+template <int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* epi = smem + S::kStages * S::kStageBytes;
+  uint8_t* epi = smem + kStages * kStageBytes;
   uint32_t* amax = reinterpret_cast<uint32_t*>(epi + kEpiBytes);  // [2 parities][2 halves][128 rows]
   uint64_t* bars = reinterpret_cast<uint64_t*>(epi + kEpiBytes + 2048);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::kStages + 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* prefix = reinterpret_cast<int*>(tmem_slot + 4);  // [E + 1]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint32_t rank = 0;
-  if constexpr (CG == 2) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  const int first = blockIdx.x / CG, step = gridDim.x / CG;
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (S::kStages + s); };
-  auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * S::kStages + a); };
-  auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * S::kStages + 2 + a); };
-  auto row_bar = [&](int quad) { return bar0 + 8u * (2 * S::kStages + 4 + quad); };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (kStages + s); };
+  auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * kStages + a); };
+  auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kStages + 2 + a); };
+  auto row_bar = [&](int quad) { return bar0 + 8u * (2 * kStages + 4 + quad); };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), kEpiWarps * CG);
+      mbar_init(tempty_bar(a), kEpiWarps);
     }
     for (int q = 0; q < 4; ++q) mbar_init(row_bar(q), 2);  // the two warps of a quadrant
     *abort_flag = 0;
@@ -349,17 +304,10 @@ __device__ __forceinline__ void fp8_gemm_body(const Maps& maps, const Params& p)
     fence_proxy_async_smem();
   }
   if (warp == 1) {
-    if constexpr (CG == 1) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                   "r"(kTmemCols)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                   "r"(kTmemCols)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    }
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
   pdl_launch();
@@ -368,7 +316,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Maps& maps, const Params& p)
     for (int base = 0; base < p.E; base += 32) {
       const int e = base + lane;
       const int v =
-          e < p.E ? (max(group_at(p, e + 1) - group_at(p, e), 0) + S::kRows - 1) / S::kRows * p.n_tiles : 0;
+          e < p.E ? (max(group_at(p, e + 1) - group_at(p, e), 0) + BM - 1) / BM * p.n_tiles : 0;
       int incl = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -382,7 +330,6 @@ __device__ __forceinline__ void fp8_gemm_body(const Maps& maps, const Params& p)
   }
   fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();  // the peer's barriers are initialised before any remote use
   fence_after();
   const uint32_t tmem = *tmem_slot;
   const int total = prefix[p.E];
@@ -393,62 +340,51 @@ __device__ __forceinline__ void fp8_gemm_body(const Maps& maps, const Params& p)
       // ---------------------------------------------- TMA producer --
       uint32_t it = 0;
       bool ok = true;
-      for (int t = first; t < total && ok; t += step) {
-        const Tile tl = tile_at(t, prefix, p, S::kRows);
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        const Tile tl = tile_at(t, prefix, p);
         // a small group needs few rows of A: boxes of 128, 64, 32 or 16 rows
         int box = 0;
-        if (CG == 1)
-          while (box < 3 && tl.m_end - tl.m0 <= (64 >> box)) ++box;
-        const uint32_t a_bytes = CG == 1 ? kTileBytes >> box : kTileBytes;
+        while (box < 3 && tl.m_end - tl.m0 <= (64 >> box)) ++box;
+        const uint32_t a_bytes = kTileBytes >> box;
         for (int kb = 0; kb < p.nk; ++kb, ++it) {
-          const int s = it % S::kStages;
-          if (!wait_inline(empty_bar(s), ((it / S::kStages) & 1u) ^ 1u, abort_flag, p.err)) {
+          const int s = it % kStages;
+          if (!wait_inline(empty_bar(s), ((it / kStages) & 1u) ^ 1u, abort_flag, p.err)) {
             ok = false;
             break;
           }
-          const uint32_t st = smem_u32(smem + s * S::kStageBytes);
-          if constexpr (CG == 1) {
-            mbar_expect_tx(full_bar(s), a_bytes + 2 * kTileBytes);
-            load_2d<1>(st, &maps.a[box], kb * BK, tl.m0, full_bar(s));
-            if constexpr (MODE == FP8_SWIGLU) {
-              load_3d<1>(st + kTileBytes, &maps.w, kb * BK, tl.n * 128, tl.e, full_bar(s));
-              load_3d<1>(st + 2 * kTileBytes, &maps.w2, kb * BK, tl.n * 128, tl.e, full_bar(s));
-            } else {
-              load_3d<1>(st + kTileBytes, &maps.w, kb * BK, tl.n * BN, tl.e, full_bar(s));
-              load_3d<1>(st + 2 * kTileBytes, &maps.w, kb * BK, tl.n * BN + 128, tl.e, full_bar(s));
-            }
+          const uint32_t st = smem_u32(smem + s * kStageBytes);
+          mbar_expect_tx(full_bar(s), a_bytes + 2 * kTileBytes);
+          load_2d(st, &maps.a[box], kb * BK, tl.m0, full_bar(s));
+          if constexpr (MODE == FP8_SWIGLU) {
+            load_3d(st + kTileBytes, &maps.w, kb * BK, tl.n * 128, tl.e, full_bar(s));
+            load_3d(st + 2 * kTileBytes, &maps.w2, kb * BK, tl.n * 128, tl.e, full_bar(s));
           } else {
-            if (rank == 0) mbar_expect_tx(full_bar(s), 2 * S::kStageBytes);
-            const uint32_t fb = mapa(full_bar(s), 0);
-            load_2d<2>(st, &maps.a[0], kb * BK, tl.m0 + (int)rank * BM, fb);
-            if constexpr (MODE == FP8_SWIGLU)
-              load_3d<2>(st + kTileBytes, rank == 0 ? &maps.w : &maps.w2, kb * BK, tl.n * 128, tl.e, fb);
-            else
-              load_3d<2>(st + kTileBytes, &maps.w, kb * BK, tl.n * BN + (int)rank * 128, tl.e, fb);
+            load_3d(st + kTileBytes, &maps.w, kb * BK, tl.n * BN, tl.e, full_bar(s));
+            load_3d(st + 2 * kTileBytes, &maps.w, kb * BK, tl.n * BN + 128, tl.e, full_bar(s));
           }
         }
       }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && lane == 0) {
       // ----------------------------------------------- MMA issuer --
       uint32_t it = 0;
       bool ok = true;
-      for (int t = first; t < total && ok; t += step) {
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
         for (int kb = 0; kb < p.nk; ++kb, ++it) {
-          const int s = it % S::kStages;
+          const int s = it % kStages;
           const uint32_t a = it & 1u;
           if (!wait_inline(tempty_bar(a), ((it >> 1) & 1u) ^ 1u, abort_flag, p.err) ||
-              !wait_inline(full_bar(s), (it / S::kStages) & 1u, abort_flag, p.err)) {
+              !wait_inline(full_bar(s), (it / kStages) & 1u, abort_flag, p.err)) {
             ok = false;
             break;
           }
           fence_after();
-          const uint32_t st = smem_u32(smem + s * S::kStageBytes);
+          const uint32_t st = smem_u32(smem + s * kStageBytes);
           const uint64_t ad = smem_desc(st), bd = smem_desc(st + kTileBytes);
 #pragma unroll
           for (int j = 0; j < BK / 32; ++j)  // 32 bytes along K inside the swizzled row
-            mma<CG>(tmem + a * BN, ad + (uint64_t)(2 * j), bd + (uint64_t)(2 * j), j != 0);
-          commit<CG>(empty_bar(s));
-          commit<CG>(tfull_bar(a));
+            mma(tmem + a * BN, ad + (uint64_t)(2 * j), bd + (uint64_t)(2 * j), j != 0);
+          commit(empty_bar(s));
+          commit(tfull_bar(a));
         }
       }
     }
@@ -463,73 +399,54 @@ __device__ __forceinline__ void fp8_gemm_body(const Maps& maps, const Params& p)
     const uint32_t col1 = MODE == FP8_SWIGLU ? 128 + half * 64 : half * 128 + 64;
     uint32_t it = 0, tiles = 0;  // K blocks; tiles with rows of this warp
     bool ok = true;
-    for (int t = first; t < total && ok; t += step) {
-      const Tile tl = tile_at(t, prefix, p, S::kRows);
-      const int row0 = tl.m0 + (int)rank * BM + quad * 32;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      const Tile tl = tile_at(t, prefix, p);
+      const int row0 = tl.m0 + quad * 32;
       const bool work = row0 < tl.m_end;
-      const float* sa = p.a_scale + min(row0 + lane, p.rows - 1);
-      const int nb = MODE == FP8_SWIGLU ? tl.n : min(2 * tl.n + half, p.nb_n - 1);
-      const float* sw = p.w_scale + ((int64_t)tl.e * p.nb_n + nb) * p.nk;
-      const float* sw2 = p.w2_scale + ((int64_t)tl.e * p.nb_n + nb) * p.nk;
+      // where the next scales are: blocks of 128 bytes in 180 GB fit 32 bits
+      uint32_t ia = (uint32_t)min(row0 + lane, p.rows - 1);
+      uint32_t iw = (uint32_t)((tl.e * p.nb_n + (MODE == FP8_SWIGLU ? tl.n : min(2 * tl.n + half, p.nb_n - 1))) * p.nk);
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.f;
       // scales of the next two K blocks: they come from L2 while the tensor core works
       float a0 = 0.f, a1 = 0.f, w0 = 0.f, w1 = 0.f, u0 = 0.f, u1 = 0.f;
-      if (work) {
-        a0 = __ldg(sa), w0 = __ldg(sw);
-        if (MODE == FP8_SWIGLU) u0 = __ldg(sw2);
-        if (p.nk > 1) {
-          a1 = __ldg(sa + p.rows), w1 = __ldg(sw + 1);
-          if (MODE == FP8_SWIGLU) u1 = __ldg(sw2 + 1);
-        }
-      }
+      auto next_scales = [&](float& fa, float& fw, float& fu) {
+        fa = __ldg(p.a_scale + ia), fw = __ldg(p.w_scale + iw);
+        if (MODE == FP8_SWIGLU) fu = __ldg(p.w2_scale + iw);
+        ia += (uint32_t)p.rows, ++iw;
+      };
+      if (work) next_scales(a0, w0, u0);
+      if (work && p.nk > 1) next_scales(a1, w1, u1);
 #pragma unroll 1
       for (int kb = 0; kb < p.nk; ++kb, ++it) {
         const uint32_t a = it & 1u;
         const float s0 = a0 * w0, s1 = MODE == FP8_SWIGLU ? a0 * u0 : s0;
         a0 = a1, w0 = w1, u0 = u1;
-        if (work && kb + 2 < p.nk) {
-          a1 = __ldg(sa + (int64_t)(kb + 2) * p.rows), w1 = __ldg(sw + kb + 2);
-          if (MODE == FP8_SWIGLU) u1 = __ldg(sw2 + kb + 2);
-        }
+        if (work && kb + 2 < p.nk) next_scales(a1, w1, u1);
         if (!wait_inline(tfull_bar(a), (it >> 1) & 1u, abort_flag, p.err)) {
           ok = false;
           break;
         }
         fence_after();
+        uint32_t v0[32], v1[32];
         if (work) {
           const uint32_t ta = tmem + a * BN + lane_base;
-          uint32_t v[32];
-          tmem_ld32(ta + col0, v);
+          tmem_ld32(ta + col0, v0);
+          tmem_ld32(ta + col0 + 32, v1);
           tmem_wait();
-          scale_add(acc, v, s0);
-          tmem_ld32(ta + col0 + 32, v);
+          scale_add(acc, v0, s0);
+          tmem_ld32(ta + col1, v0);
+          scale_add(acc + 32, v1, s0);
+          tmem_ld32(ta + col1 + 32, v1);
           tmem_wait();
-          scale_add(acc + 32, v, s0);
-          tmem_ld32(ta + col1, v);
-          tmem_wait();
-          scale_add(acc + 64, v, s1);
-          tmem_ld32(ta + col1 + 32, v);
-          tmem_wait();
-          fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (CG == 1) mbar_arrive(tempty_bar(a));
-            else
-              asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa(tempty_bar(a), 0))
-                           : "memory");
-          }
-          scale_add(acc + 96, v, s1);
-        } else {
-          fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (CG == 1) mbar_arrive(tempty_bar(a));
-            else
-              asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa(tempty_bar(a), 0))
-                           : "memory");
-          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty_bar(a));
+        if (work) {
+          scale_add(acc + 64, v0, s1);
+          scale_add(acc + 96, v1, s1);
         }
       }
       if (ok && work)
@@ -539,26 +456,10 @@ __device__ __forceinline__ void fp8_gemm_body(const Maps& maps, const Params& p)
 
   fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();  // the leader's MMAs read the peer's shared memory until here
   if (warp == 1) {
     fence_after();
-    if constexpr (CG == 1)
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
-    else
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
-}
-
-template <int MODE>
-__global__ void __launch_bounds__(kThreads, 1)
-fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
-  fp8_gemm_body<MODE, 1>(maps, p);
-}
-
-template <int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-fp8_gemm_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
-  fp8_gemm_body<MODE, 2>(maps, p);
 }
 
 // ------------------------------------------------------------ host side --
@@ -590,10 +491,13 @@ int make_map(CUtensorMap* m, const void* base, int64_t E, int64_t R, int64_t K, 
   return FRANK_OK;
 }
 
-template <typename Kern>
-int launch(Kern kern, size_t smem, unsigned grid, const Maps& maps, const Params& p, cudaStream_t st) {
-  FRANK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  FRANK_CUDA_TRY(frank::launch_chained(kern, dim3(grid), dim3(kThreads), smem, st, 1, maps, p));
+template <int MODE>
+int launch(const Maps& maps, const Params& p, cudaStream_t st) {
+  const size_t smem = smem_bytes(p.E);
+  FRANK_CUDA_TRY(
+      cudaFuncSetAttribute(fp8_gemm_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  FRANK_CUDA_TRY(
+      frank::launch_chained(fp8_gemm_kernel<MODE>, dim3(frank::num_sms()), dim3(kThreads), smem, st, 1, maps, p));
   FRANK_LAUNCH_CHECK();
   return FRANK_OK;
 }
@@ -625,24 +529,13 @@ int launch_fp8_gemm(const Fp8Gemm& g, cudaStream_t st) {
   p.out = g.out;
   p.h_scale = g.h_scale;
   p.err = device_error_word();
-  // A pair of CTAs wastes up to 255 rows of a tile: for groups of 1024 rows on average.
-  const bool pair = g.rows >= 1024 * g.E && num_sms() >= 2;
-  const int64_t rows = pair ? 2 * BM : BM;
   // rows of A that the CTAs share through L2 while they sweep the columns: 64 MB
-  int64_t band = (64ll << 20) / g.K / rows;
-  p.band = (int)(band < 1 ? 1 : (band * rows > 8192 ? 8192 / rows : band));
-  const unsigned grid = (unsigned)(pair ? num_sms() & ~1 : num_sms());
-  const size_t smem = pair ? Shape<2>::smem(g.E) : Shape<1>::smem(g.E);
+  const int64_t band = (64ll << 20) / g.K / BM;
+  p.band = (int)(band < 1 ? 1 : (band > 64 ? 64 : band));
   switch (g.mode) {
-    case FP8_SWIGLU:
-      return pair ? launch(fp8_gemm_pair_kernel<FP8_SWIGLU>, smem, grid, maps, p, st)
-                  : launch(fp8_gemm_kernel<FP8_SWIGLU>, smem, grid, maps, p, st);
-    case FP8_SCALE:
-      return pair ? launch(fp8_gemm_pair_kernel<FP8_SCALE>, smem, grid, maps, p, st)
-                  : launch(fp8_gemm_kernel<FP8_SCALE>, smem, grid, maps, p, st);
-    default:
-      return pair ? launch(fp8_gemm_pair_kernel<FP8_PLAIN>, smem, grid, maps, p, st)
-                  : launch(fp8_gemm_kernel<FP8_PLAIN>, smem, grid, maps, p, st);
+    case FP8_SWIGLU: return launch<FP8_SWIGLU>(maps, p, st);
+    case FP8_SCALE: return launch<FP8_SCALE>(maps, p, st);
+    default: return launch<FP8_PLAIN>(maps, p, st);
   }
 }
 
