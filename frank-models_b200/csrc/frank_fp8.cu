@@ -3,6 +3,7 @@
 #include <initializer_list>
 
 #include "fp8.cuh"
+#include "fp8_few.cuh"
 
 namespace frank {
 
@@ -97,10 +98,41 @@ static int check_moe(const char* what, int64_t T, int64_t E, int64_t k, int64_t 
   return FRANK_OK;
 }
 
+// A few tokens: the weights bound the call, and few_fp8.cu reads them once.
+static bool few_tokens(int64_t T, int64_t k) { return T <= 64 && k * T <= kFewMaxSlots; }
+
+static FewArgs few_args(const Fp8Weights& W, int64_t T, int64_t E, int64_t k, int64_t H, int64_t F, const float* w,
+                        const int32_t* ids, const Fp8MoeWs& L) {
+  FewArgs a;
+  a.w_up = static_cast<const uint8_t*>(W.up);
+  a.w_gate = static_cast<const uint8_t*>(W.gate);
+  a.w_down = static_cast<const uint8_t*>(W.down);
+  a.s_up = W.s_up;
+  a.s_gate = W.s_gate;
+  a.s_down = W.s_down;
+  a.xq = L.xq;
+  a.xs = L.xs;
+  a.hq = L.hq;
+  a.hs = L.hs;
+  a.d = L.d;
+  a.w = w;
+  a.ids = ids;
+  a.T = (int)T;
+  a.E = (int)E;
+  a.k = (int)k;
+  a.H = (int)H;
+  a.F = (int)F;
+  return a;
+}
+
 // Routed rows through the experts: L.d[r] = w * down(q(h)) for the expert-sorted rows r.
 static int run_experts(const void* x, const float* w, const int32_t* ids, const Fp8Weights& W, int64_t T, int64_t E,
                        int64_t k, int64_t H, int64_t F, int32_t* err, const Fp8MoeWs& L, cudaStream_t st) {
   const int64_t n = k * T;
+  if (few_tokens(T, k)) {
+    FRANK_TRY(launch_quantize_rows(FRANK_BF16, x, T, H, nullptr, 1, L.xq, L.xs, st));
+    return launch_few_experts(few_args(W, T, E, k, H, F, w, ids, L), err, st);
+  }
   FRANK_TRY(launch_permute(ids, n, E, L.sorted_slots, L.offsets, L.slot_pos, err, L.perm, L.perm_bytes, st, w,
                            L.wsorted));
   FRANK_TRY(launch_quantize_rows(FRANK_BF16, x, T, H, L.slot_pos, k, L.xq, L.xs, st));
@@ -140,7 +172,7 @@ static int run_experts(const void* x, const float* w, const int32_t* ids, const 
 static NormRows combine_of(const Fp8MoeWs& L, int64_t T, int64_t k, int64_t H, int out_dtype, void* out) {
   NormRows a;
   a.d = L.d;
-  a.slot_pos = L.slot_pos;
+  a.slot_pos = few_tokens(T, k) ? nullptr : L.slot_pos;
   a.k = (int)k;
   a.T = T;
   a.H = H;
@@ -149,8 +181,10 @@ static NormRows combine_of(const Fp8MoeWs& L, int64_t T, int64_t k, int64_t H, i
   return a;
 }
 
-static int route(const void* x, int wr_dtype, const void* wr, int64_t T, int64_t E, int64_t k, int64_t H,
-                 int normalize, float* w, int32_t* ids, const Fp8MoeWs& L, cudaStream_t st) {
+// The block up to L.d: x [T, H] bf16, or with norm_w the residual it is normalised from.
+static int route_and_run(int x_dtype, const void* x, const float* norm_w, float eps, int wr_dtype, const void* wr,
+                         const Fp8Weights& W, int64_t T, int64_t E, int64_t k, int64_t H, int64_t F, int normalize,
+                         float* w, int32_t* ids, const Fp8MoeWs& L, cudaStream_t st) {
   const __nv_bfloat16* wr3 = nullptr;
   if (wr_dtype == FRANK_ROUTER_PACKED) {
     wr3 = reinterpret_cast<const __nv_bfloat16*>(static_cast<const char*>(wr) + router_pack_offset(E, H));
@@ -158,7 +192,40 @@ static int route(const void* x, int wr_dtype, const void* wr, int64_t T, int64_t
   }
   FRANK_TRY(check_float_dtype(wr_dtype, "fp8_moe router"));
   FRANK_CHECK_ARG(wr != nullptr, "fp8_moe router: null pointer");
-  return launch_router_topk(FRANK_BF16, x, wr_dtype, wr, T, H, E, k, normalize, w, ids, L.logits, st, wr3);
+  if (few_tokens(T, k)) {
+    FewRoute r;
+    r.x = x;
+    r.x_dtype = x_dtype;
+    r.norm_w = norm_w;
+    r.eps = eps;
+    r.wr = wr;
+    r.wr_dtype = wr_dtype;
+    r.T = (int)T;
+    r.H = (int)H;
+    r.E = (int)E;
+    r.k = (int)k;
+    r.normalize = normalize;
+    r.xq = L.xq;
+    r.xs = L.xs;
+    r.w = w;
+    r.ids = ids;
+    FRANK_TRY(launch_few_route(r, st));
+    return launch_few_experts(few_args(W, T, E, k, H, F, w, ids, L), nullptr, st);
+  }
+  if (norm_w != nullptr) {
+    NormRows pre;
+    pre.y_dtype = x_dtype;
+    pre.y = x;
+    pre.eps = eps;
+    pre.next_w = norm_w;
+    pre.next = L.xn;
+    pre.T = T;
+    pre.H = H;
+    FRANK_TRY(launch_norm_rows(pre, st));
+    x = L.xn;
+  }
+  FRANK_TRY(launch_router_topk(FRANK_BF16, x, wr_dtype, wr, T, H, E, k, normalize, w, ids, L.logits, st, wr3));
+  return run_experts(x, w, ids, W, T, E, k, H, F, nullptr, L, st);
 }
 
 static int check_gate(const char* what, const float* gate, int64_t gate_rows, int64_t T) {
@@ -278,8 +345,7 @@ int frank_fp8_moe_block(const void* x, int wr_dtype, const void* wr, const void*
   fp8_moe_layout(T, H, F, E, k, workspace, ws_bytes, &L);
   float* w = route_w ? route_w : L.w;
   int32_t* ids = route_ids ? route_ids : L.ids;
-  FRANK_TRY(route(x, wr_dtype, wr, T, E, k, H, normalize, w, ids, L, st));
-  FRANK_TRY(run_experts(x, w, ids, W, T, E, k, H, F, nullptr, L, st));
+  FRANK_TRY(route_and_run(FRANK_BF16, x, nullptr, 0.f, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
   return launch_norm_rows(combine_of(L, T, k, H, y_dtype, y), st);
 }
 
@@ -301,17 +367,8 @@ int frank_fp8_moe_sublayer(int res_dtype, const void* residual, const float* nor
   fp8_moe_layout(T, H, F, E, k, workspace, ws_bytes, &L);
   float* w = route_w ? route_w : L.w;
   int32_t* ids = route_ids ? route_ids : L.ids;
-  NormRows pre;
-  pre.y_dtype = res_dtype;
-  pre.y = residual;
-  pre.eps = eps;
-  pre.next_w = norm_w;
-  pre.next = L.xn;
-  pre.T = T;
-  pre.H = H;
-  FRANK_TRY(launch_norm_rows(pre, st));
-  FRANK_TRY(route(L.xn, wr_dtype, wr, T, E, k, H, normalize, w, ids, L, st));
-  FRANK_TRY(run_experts(L.xn, w, ids, W, T, E, k, H, F, nullptr, L, st));
+  FRANK_TRY(
+      route_and_run(res_dtype, residual, norm_w, eps, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
   NormRows a = combine_of(L, T, k, H, res_dtype, out);
   a.post_w = post_w;
   a.eps = eps;
