@@ -1,28 +1,33 @@
 // The 8-bit MoE layer for a few tokens, bound by the expert weights in HBM:
 // three launches chained by programmatic dependent launch (and the combine in
-// norm.cu), without a permutation, a gather or atomics.
+// norm.cu), without a permutation or a gather, each weight read once.
 //
 //   few_route   [norm,] quantisation, router, softmax and top-k: clusters of 8
 //               CTAs take 8 tokens, each CTA an eighth of H.  The sums of squares and
 //               the partial logits are exchanged through distributed shared memory
 //               and added in CTA order.
-//   few_up      h = gate * silu(up), quantised: clusters of 4 CTAs take one expert and
-//               128 columns of F, each CTA 32 of them; a block of h shares one scale, so
-//               the maxima go round the cluster.
-//   few_down    d[slot] = route weight * down(h[slot])
+//   few_up      h = gate * silu(up) for items of 8 columns of F of one expert; the
+//               last of the 16 items of a quantisation block quantises it
+//   few_down    d[slot] = route weight * down(h[slot]) for items of 16 rows of one expert
 //
-// The weights are read once, straight into the registers of the warps that use
-// them, 16 bytes a lane and four K blocks (8 KB a warp) at a time: with two CTAs an SM
-// 128 KB are under way, what 6.5 TB/s need at 3 us.  A warp multiplies 16 weight rows (8 of
-// gate and the same 8 of up, or 16 of down) with 8 tokens by mma.m16n8k16 in
-// fp16, into which e4m3 converts exactly, with fp32 sums; one K block is summed and
-// then scaled.  Lane t of a quad holds K elements 16 t .. 16 t + 15 of a row: the
-// MMA's K index is permuted alike for weights and tokens, which leaves the sum.
+// few_up and few_down are persistent, 8 warps an SM.  A warp takes an item by itself: its
+// weight rows come by TMA, 8 KB (16 rows x 512 values) a stage, three stages a warp,
+// so 192 KB an SM are under way and no warp waits for another one.  A warp
+// multiplies 16 weight rows (8 of gate and the same 8 of up, or 16 of down) with 8
+// tokens by mma.m16n8k16 in fp16, into which e4m3 converts exactly, with fp32
+// sums; one K block is summed and then scaled.  Lane t of a quad holds K elements
+// 16 t .. 16 t + 15 of a row: the MMA's K index is permuted alike for weights and
+// tokens, which leaves the sum.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "fp8.cuh"
 #include "fp8_few.cuh"
+#include "mbarrier.cuh"
 
 namespace {
 using namespace frank;
+using namespace frank_mbar;
 
 // ------------------------------------------------------------ cluster --
 __device__ __forceinline__ uint32_t cta_rank() {
@@ -67,11 +72,21 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
   constexpr int kWarps = kRouteThreads / 32;
   const uint32_t rank = cta_rank();
   const int t0 = blockIdx.x / kRouteCtas * kRouteTok, nt = min(kRouteTok, a.T - t0);
+  if (a.wr != nullptr) {  // the router's slice does not wait for the stream's last kernel
+    const int64_t esz = a.wr_dtype == FRANK_F32 ? 4 : 2;
+    const int h0 = (int)rank * ((a.H + kQB * kRouteCtas - 1) / (kQB * kRouteCtas)) * kQB;
+    const int h1 = min(h0 + (a.H + kQB * kRouteCtas - 1) / (kQB * kRouteCtas) * kQB, a.H);
+    const int lines = (int)(((h1 - h0) * esz + 127) / 128);
+    for (int i = threadIdx.x; i < a.E * lines; i += kRouteThreads)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(a.wr) +
+                                                    ((int64_t)(i / lines) * a.H + h0) * esz + i % lines * 128));
+  }
   const int nb = (a.H + kQB - 1) / kQB, sb = (nb + kRouteCtas - 1) / kRouteCtas;  // blocks of a row, of a slice
   const int slice = sb * kQB, h0 = (int)rank * slice;
   pdl_wait();
   pdl_launch();
   cluster_arrive();  // every CTA has started before its memory is written
+  for (int i = blockIdx.x * kRouteThreads + threadIdx.x; i < a.n_count; i += gridDim.x * kRouteThreads) a.count[i] = 0;
   // one (token, block) a warp: a vector of 4 for each lane
   for (int i = warp; i < kRouteTok * sb; i += kWarps) {
     const int t = i / sb, b = i % sb, h = h0 + b * kQB + lane * 4;
@@ -121,6 +136,7 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
       if (lane == 0) a.xs[(int64_t)(h / kQB) * a.T + t0 + t] = s.scale;
     }
   }
+  if (a.wr == nullptr) return;  // the routing is given
   __syncthreads();
   // partial logits of this slice: four experts a warp, 8 tokens each
   for (int e0 = warp * 4; e0 < a.E; e0 += kWarps * 4) {
@@ -225,7 +241,6 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
 }
 
 // ------------------------------------------------------------- products --
-// 16 weight rows times 8 tokens of one K block, one 64-byte half at a time.
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -243,262 +258,280 @@ __device__ __forceinline__ void to_half(const uint4& v, uint32_t (&h)[8]) {
   }
 }
 
-// Weights are read once by one SM: past L1, first to leave L2.
-__device__ __forceinline__ uint4 load_weights(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+constexpr int kWarps = 8, kFewThreads = 32 * kWarps;
+constexpr int kChunkK = 512, kChunkB = kChunkK / kQB;      // values and blocks along K of a stage
+constexpr int kRows = 16, kStages = 3;
+constexpr int kStageBytes = kRows * kChunkK;
+constexpr int kMaxGroups = 8;  // of 8 tokens: an expert has at most 64
+
+struct FewMaps {
+  CUtensorMap a, b;  // few_up: gate and up; few_down: down
+};
+
+// The routing as every CTA sees it: the experts that have tokens, ascending, and their slots.
+struct Table {
+  int nact;
+  int expert[kFewMaxE];
+  int start[kFewMaxE + 1];
+  int slots[kFewMaxSlots];
+};
+
+__device__ __forceinline__ void build_table(const FewArgs& a, Table& tb, int* sid, int* sums) {
+  const int n = a.k * a.T, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int s = tid; s < n; s += kFewThreads) sid[s] = min(max(a.ids[s], 0), a.E - 1);
+  __syncthreads();
+  // thread e counts expert e
+  int c = 0;
+  for (int s = 0; s < n; ++s) c += sid[s] == tid;
+  int v = c | (c != 0) << 16;  // slots and experts before this one
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) sums[warp] = v;
+  __syncthreads();
+  int before = v - (c | (c != 0) << 16), total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sums[w];
+    total += sums[w];
+  }
+  if (c != 0) {
+    int at = before & 0xffff;
+    tb.expert[before >> 16] = tid;
+    tb.start[before >> 16] = at;
+    for (int s = 0; s < n; ++s)
+      if (sid[s] == tid) tb.slots[at++] = s;
+  }
+  if (tid == 0) tb.nact = total >> 16, tb.start[total >> 16] = n;
+  __syncthreads();
 }
 
-constexpr int kGroups = kFewGroups;    // groups of 8 tokens taken at once
-constexpr int kFewThreads = 256;
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int k8, int row, int e, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(map), "r"(k8), "r"(row), "r"(e), "r"(bar)
+      : "memory");
+}
 
-// acc[g][0..3] += (rows r0 and r1, this lane's two tokens of group g) over K blocks [b0, b1).
-//   r0, r1      this lane's two weight rows (row g of the MMA and row g + 8)
-//   s0, s1      their scales, one a K block
-//   tok[g]      this lane's token row of group g for the product (lane / 4), or -1
-//   col[g][2]   the rows of its two accumulator columns (2 (lane % 4) and the next), or -1
-template <int G>
-__device__ __forceinline__ void product(float (&acc)[G][4], const uint8_t* r0, const uint8_t* r1, const float* s0,
-                                        const float* s1, const uint8_t* x, const float* x_scale, int64_t ld_scale,
-                                        const int (&tok)[G], const int (&col)[G][2], int K, int b0, int b1) {
-  constexpr int kBatch = G == 1 ? 4 : 2;  // K blocks under way a warp
-  const int k_lane = (threadIdx.x & 3) * 16;
-#pragma unroll 1
-  for (int b = b0; b < b1; b += kBatch) {
-    uint4 w0[kBatch][2], w1[kBatch][2];
+// One stage: acc[g] += 16 rows x the tokens of group g over the blocks [b0, b0 + 4) of K.
+// tok / col: this lane's token row of the product and the rows of its two accumulator columns, or -1.
+template <int G, int ROWS>
+__device__ __forceinline__ void stage_product(float (&acc)[kMaxGroups][4], const uint8_t* st, const uint8_t* x,
+                                              const float* x_scale, int64_t ld_scale, const float* s0,
+                                              const float* s1, const int* tok, const int (*col)[2], int K, int b0,
+                                              int nb, uint32_t bar, uint32_t parity, bool& ok, volatile int* abort,
+                                              int32_t* err) {
+  const int lane = threadIdx.x & 31, row = lane >> 2, k_lane = (lane & 3) * 16;
+  // up to 16 tokens: everything but the weights is loaded before they are waited for
+  constexpr bool kAhead = G <= 2;
+  uint4 v[kAhead ? G : 1][kChunkB][2];
+  float xs[kAhead ? G : 1][kChunkB][2], f0[kChunkB], f1[kChunkB];
+  auto tokens = [&](int g, int i, uint4 (&q)[2], float (&sc)[2]) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i)
+    for (int h = 0; h < 2; ++h) {
+      const int k = (b0 + i) * kQB + h * 64 + k_lane;
+      q[h] = make_uint4(0u, 0u, 0u, 0u);
+      if (tok[g] >= 0 && k < K) q[h] = *reinterpret_cast<const uint4*>(x + (int64_t)tok[g] * K + k);
+      sc[h] = b0 + i < nb && col[g][h] >= 0 ? x_scale[(b0 + i) * ld_scale + col[g][h]] : 0.f;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kChunkB; ++i) {
+    const bool in = b0 + i < nb;
+    f0[i] = in ? __ldg(s0 + b0 + i) : 0.f;
+    f1[i] = in ? __ldg(s1 + b0 + i) : 0.f;
+    if (kAhead) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) tokens(g, i, v[g][i], xs[g][i]);
+    }
+  }
+  if (!mbar_wait_inline(bar, parity, abort, err)) ok = false;
+#pragma unroll
+  for (int i = 0; i < kChunkB; ++i) {
+    if (b0 + i < nb) {
+      uint32_t a0[2][8], a1[2][8] = {};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = (b + i) * kQB + h * 64 + k_lane;
-        w0[i][h] = w1[i][h] = make_uint4(0u, 0u, 0u, 0u);
-        if (b + i < b1 && k < K) {
-          w0[i][h] = load_weights(r0 + k);
-          w1[i][h] = load_weights(r1 + k);
-        }
+        const uint8_t* p = st + row * kChunkK + i * kQB + h * 64 + k_lane;
+        to_half(*reinterpret_cast<const uint4*>(p), a0[h]);
+        if (ROWS == 16) to_half(*reinterpret_cast<const uint4*>(p + 8 * kChunkK), a1[h]);
       }
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (b + i < b1) {
-        float part[G][4] = {};
+      for (int g = 0; g < G; ++g) {
+        float part[4] = {};
+        uint4 q[2];
+        float sc[2];
+        if (!kAhead) tokens(g, i, q, sc);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int k = (b + i) * kQB + h * 64 + k_lane;
-          uint32_t a0[8], a1[8];
-          to_half(w0[i][h], a0);
-          to_half(w1[i][h], a1);
+          uint32_t t[8];
+          to_half(kAhead ? v[kAhead ? g : 0][i][h] : q[h], t);
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (tok[g] >= 0 && k < K) v = *reinterpret_cast<const uint4*>(x + (int64_t)tok[g] * K + k);
-            uint32_t t[8];
-            to_half(v, t);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              mma_16816(part[g], a0[2 * j], a1[2 * j], a0[2 * j + 1], a1[2 * j + 1], t[2 * j], t[2 * j + 1]);
-          }
+          for (int j = 0; j < 4; ++j)
+            mma_16816(part, a0[h][2 * j], a1[h][2 * j], a0[h][2 * j + 1], a1[h][2 * j + 1], t[2 * j], t[2 * j + 1]);
         }
-        const float f0 = __ldg(s0 + b + i), f1 = __ldg(s1 + b + i);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const float* xs = x_scale + (int64_t)(b + i) * ld_scale;
-          const float c0 = col[g][0] >= 0 ? xs[col[g][0]] : 0.f, c1 = col[g][1] >= 0 ? xs[col[g][1]] : 0.f;
-          acc[g][0] = fmaf(part[g][0], c0 * f0, acc[g][0]);
-          acc[g][1] = fmaf(part[g][1], c1 * f0, acc[g][1]);
-          acc[g][2] = fmaf(part[g][2], c0 * f1, acc[g][2]);
-          acc[g][3] = fmaf(part[g][3], c1 * f1, acc[g][3]);
-        }
+        const float x0 = kAhead ? xs[kAhead ? g : 0][i][0] : sc[0], x1 = kAhead ? xs[kAhead ? g : 0][i][1] : sc[1];
+        acc[g][0] = fmaf(part[0], x0 * f0[i], acc[g][0]);
+        acc[g][1] = fmaf(part[1], x1 * f0[i], acc[g][1]);
+        acc[g][2] = fmaf(part[2], x0 * f1[i], acc[g][2]);
+        acc[g][3] = fmaf(part[3], x1 * f1[i], acc[g][3]);
       }
     }
   }
 }
 
-// Expert id of a slot, inside [0, E) whatever the caller gave.
-__device__ __forceinline__ int expert_of(const int32_t* ids, int s, int E) { return min(max(ids[s], 0), E - 1); }
+// The stream of one warp's stages: item after item, chunk after chunk along K.  Lane 0
+// issues the loads, three stages ahead; the warp that read a stage refills it.
+//   UP: 8 rows of map a over 8 rows of map b; else ROWS rows of map a
+template <bool UP, int ROWS>
+struct Stream {
+  const FewMaps* maps;
+  const Table* tb;
+  uint8_t* smem;      // this warp's stages
+  uint32_t bar;       // this warp's barriers
+  int items, per;     // items in all, items an expert
+  int chunks;         // chunks of an item
+  int next, chunk, step;
+  uint32_t issued;
 
-// This unit's expert and its slots, ascending, in shared memory.  With no more slots than
-// experts a unit is a slot and works if it is the first one of its expert;
-// otherwise a unit is an expert.  Returns the number of slots, 0: nothing to do.
-__device__ __forceinline__ int unit_slots(const FewArgs& a, int unit, int* slots, int* expert) {
-  __shared__ int count;
-  const int n = a.k * a.T, lane = threadIdx.x & 31;
-  if (threadIdx.x < 32) {
-    const int e = n <= a.E ? expert_of(a.ids, unit, a.E) : unit;
-    int c = 0;
-    for (int base = 0; base < n; base += 32) {
-      const int s = base + lane;
-      const bool mine = s < n && expert_of(a.ids, s, a.E) == e;
-      const uint32_t m = __ballot_sync(0xffffffffu, mine);
-      if (mine) slots[c + __popc(m & ((1u << lane) - 1u))] = s;
-      c += __popc(m);
-    }
-    __syncwarp();
-    if (n <= a.E && slots[0] != unit) c = 0;
-    if (lane == 0) count = c, *expert = e;
+  __device__ __forceinline__ void issue() {
+    if (next >= items) return;
+    const uint32_t s = issued % kStages, dst = smem_u32(smem + s * kStageBytes), b = bar + 8 * s;
+    const int e = tb->expert[next / per], i = next % per, k8 = chunk * (kChunkK / 8);
+    mbar_expect_tx(b, (UP ? 16 : ROWS) * kChunkK);
+    load_box(dst, &maps->a, k8, i * (UP ? 8 : ROWS), e, b);
+    if (UP) load_box(dst + 8 * kChunkK, &maps->b, k8, i * 8, e, b);
+    ++issued;
+    if (++chunk == chunks) chunk = 0, next += step;
   }
-  __syncthreads();
-  return count;
-}
+};
 
-template <int G>
-__device__ __forceinline__ void lane_tokens(const int* slots, int c0, int c, int mod, int (&tok)[G], int (&col)[G][2]) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const int i = c0 + g * 8 + (lane >> 2), j = c0 + g * 8 + (lane & 3) * 2;
-    tok[g] = i < c ? slots[i] % mod : -1;
-    col[g][0] = j < c ? slots[j] % mod : -1;
-    col[g][1] = j + 1 < c ? slots[j + 1] % mod : -1;
-  }
-}
-
-// -------------------------------------------------------------- gate/up --
-constexpr int kUpCtas = 4, kUpItems = 4;  // a CTA: 4 items of 8 columns of F, two warps each along K
-
-template <int G>
-__device__ __forceinline__ void up_chunk(const FewArgs& a, int e, const int* slots, int c0, int c, int fb,
-                                         uint32_t rank, float (*red)[kGroups][4][32], uint32_t (*amax)[kFewChunk],
-                                         uint32_t (*peers)[kFewChunk]) {
+template <bool UP, int ROWS>
+__global__ void __launch_bounds__(kFewThreads, 1)
+few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ FewArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  __shared__ Table tb;
+  __shared__ int sid[kFewMaxSlots], sums[kWarps];
+  __shared__ uint64_t bars[kWarps * kStages];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int item = warp >> 1, split = warp & 1;
-  const int nbh = (a.H + kQB - 1) / kQB, nbf = (a.F + kQB - 1) / kQB;
-  const int f = fb * kQB + (int)rank * 32 + item * 8 + (lane >> 2);
-  const int64_t row = (int64_t)e * a.F + min(f, a.F - 1);
-  int tok[G], col[G][2];
-  lane_tokens<G>(slots, c0, c, a.T, tok, col);
-  float acc[G][4] = {};
-  const int half = (nbh + 1) / 2;
-  const int64_t so = ((int64_t)e * nbf + fb) * nbh;
-  product<G>(acc, a.w_gate + row * a.H, a.w_up + row * a.H, a.s_gate + so, a.s_up + so, a.xq, a.xs, a.T, tok, col,
-             a.H, split * half, split ? nbh : half);
-  // the second half of K, then h of 8 columns x this lane's two tokens a group
-  if (split) {
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) red[item][g][i][lane] = acc[g][i];
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kWarps * kStages; ++i) mbar_init(smem_u32(&bars[i]), 1);
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async_smem();
   }
-  __syncthreads();
-  float h[G][2];
-  if (!split) {
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[g][i] += red[item][g][i][lane];
-      uint32_t m[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        h[g][i] = f < a.F ? acc[g][i] * silu_ref(acc[g][2 + i]) : 0.f;
-        m[i] = abs_bits(h[g][i]);
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
-        if (lane < 4) amax[item][g * 8 + lane * 2 + i] = m[i];
-      }
-    }
-  }
-  __syncthreads();
-  if (c0 == 0) cluster_wait();
-  if (threadIdx.x < G * 8 * kUpCtas) {
-    const int t = threadIdx.x % (G * 8), to = threadIdx.x / (G * 8);
-    uint32_t m = 0;
-    for (int i = 0; i < kUpItems; ++i) m = max(m, amax[i][t]);
-    st_peer(peer_addr(&peers[rank][t], (uint32_t)to), m);
-  }
-  cluster_sync();
-  if (!split) {
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int t = g * 8 + (lane & 3) * 2 + i;
-        if (c0 + t < c) {
-          const BlockScale s = block_scale(max(max(peers[0][t], peers[1][t]), max(peers[2][t], peers[3][t])));
-          const int slot = slots[c0 + t];
-          if (f < a.F) {
-            const float v = h[g][i] * s.inv;
-            a.hq[(int64_t)slot * a.F + f] = (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
-          }
-          if (rank == 0 && item == 0 && lane < 4) a.hs[(int64_t)fb * a.k * a.T + slot] = s.scale;
-        }
-      }
-  }
-  cluster_sync();  // the maxima are read before the next chunk's arrive
-}
-
-__global__ void __launch_bounds__(kFewThreads, 2) few_up_kernel(const FewArgs a) {
-  __shared__ int slots[kFewMaxSlots];
-  __shared__ int expert;
-  __shared__ float red[kUpItems][kGroups][4][32];
-  __shared__ uint32_t amax[kUpItems][kFewChunk], peers[kUpCtas][kFewChunk];
-  const uint32_t rank = cta_rank();
-  const int nbf = (a.F + kQB - 1) / kQB;
-  const int cluster = blockIdx.x / kUpCtas, unit = cluster / nbf, fb = cluster % nbf;
   pdl_wait();
   pdl_launch();
-  const int c = unit_slots(a, unit, slots, &expert);
-  if (c == 0) return;  // the whole cluster
-  cluster_arrive();    // every CTA has started before its memory is written
-  for (int c0 = 0; c0 < c; c0 += kFewChunk) {
-    if (c - c0 <= 8) up_chunk<1>(a, expert, slots, c0, c, fb, rank, red, amax, peers);
-    else up_chunk<kGroups>(a, expert, slots, c0, c, fb, rank, red, amax, peers);
-  }
-}
+  build_table(a, tb, sid, sums);  // and the barriers are initialised
 
-// ----------------------------------------------------------------- down --
-// A CTA takes 128 / SPLIT rows of one expert's down matrix, SPLIT warps along K for each 16 rows.
-template <int G, int SPLIT>
-__device__ __forceinline__ void down_chunk(const FewArgs& a, int e, const int* slots, int c0, int c, int rb,
-                                           float (*red)[kGroups][4][32]) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int item = warp / SPLIT, split = warp % SPLIT;
-  const int nbh = (a.H + kQB - 1) / kQB, nbf = (a.F + kQB - 1) / kQB;
-  const int h = rb * (128 / SPLIT) + item * 16 + (lane >> 2);  // and h + 8
-  const int64_t base = (int64_t)e * a.H;
-  int tok[G], col[G][2];
-  lane_tokens<G>(slots, c0, c, 0x7fffffff, tok, col);
-  float acc[G][4] = {};
-  const int per = (nbf + SPLIT - 1) / SPLIT;
-  const float* sw = a.s_down + ((int64_t)e * nbh + min(h, a.H - 1) / kQB) * nbf;
-  product<G>(acc, a.w_down + (base + min(h, a.H - 1)) * a.F, a.w_down + (base + min(h + 8, a.H - 1)) * a.F, sw, sw,
-             a.hq, a.hs, (int64_t)a.k * a.T, tok, col, a.F, min(split * per, nbf), min((split + 1) * per, nbf));
-  if (split) {
+  const int n = a.k * a.T, K = UP ? a.H : a.F, N = UP ? a.F : a.H;
+  const int nb = (K + kQB - 1) / kQB, nbn = (N + kQB - 1) / kQB;
+  Stream<UP, ROWS> sm;
+  sm.maps = &maps;
+  sm.tb = &tb;
+  sm.smem = smem + warp * kStages * kStageBytes;
+  sm.bar = smem_u32(&bars[warp * kStages]);
+  sm.per = (N + (UP ? 8 : ROWS) - 1) / (UP ? 8 : ROWS);
+  sm.items = tb.nact * sm.per;
+  sm.chunks = (nb + kChunkB - 1) / kChunkB;
+  sm.step = gridDim.x * kWarps;
+  sm.next = blockIdx.x + gridDim.x * warp;  // neighbouring items on different SMs
+  sm.chunk = 0;
+  sm.issued = 0;
+  const int first = sm.next;
+  if (lane == 0)
+    for (int s = 0; s < kStages; ++s) sm.issue();
+  uint32_t it = 0;
+  bool ok = true;
+  for (int item = first; item < sm.items && ok; item += sm.step) {
+    const int ai = item / sm.per, i = item % sm.per, e = tb.expert[ai];
+    const int c0 = tb.start[ai], c = tb.start[ai + 1] - c0;
+    int tok[kMaxGroups], col[kMaxGroups][2];
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) red[warp][g][i][lane] = acc[g][i];
-  }
-  __syncthreads();
-  if (!split) {
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int s = 1; s < SPLIT; ++s) acc[g][i] += red[warp + s][g][i][lane];
-        const int slot = col[g][i & 1], r = h + (i >> 1) * 8;
-        if (slot >= 0 && r < a.H) a.d[(int64_t)slot * a.H + r] = acc[g][i] * a.w[slot];
+    for (int g = 0; g < kMaxGroups; ++g) {
+      const int t = g * 8 + (lane >> 2), u = g * 8 + (lane & 3) * 2;
+      tok[g] = t < c ? tb.slots[c0 + t] : -1;
+      col[g][0] = u < c ? tb.slots[c0 + u] : -1;
+      col[g][1] = u + 1 < c ? tb.slots[c0 + u + 1] : -1;
+      if (UP) {  // slots of one token share its row
+        if (tok[g] >= 0) tok[g] %= a.T;
+        if (col[g][0] >= 0) col[g][0] %= a.T;
+        if (col[g][1] >= 0) col[g][1] %= a.T;
       }
     }
+    const int64_t so = ((int64_t)e * nbn + i * (UP ? 8 : ROWS) / kQB) * nb;
+    const float* s0 = (UP ? a.s_gate : a.s_down) + so;
+    const float* s1 = (UP ? a.s_up : a.s_down) + so;
+    const uint8_t* x = UP ? a.xq : a.hq;
+    const float* x_scale = UP ? a.xs : a.hs;
+    const int64_t ld = UP ? a.T : n;
+    float acc[kMaxGroups][4] = {};
+    for (int ch = 0; ch < sm.chunks && ok; ++ch, ++it) {
+      const uint32_t s = it % kStages, parity = (it / kStages) & 1u;
+      const uint8_t* st = sm.smem + s * kStageBytes;
+#define FRANK_STAGE(G)                                                                                             \
+  stage_product<G, UP ? 16 : ROWS>(acc, st, x, x_scale, ld, s0, s1, tok, col, K, ch * kChunkB, nb, sm.bar + 8 * s, \
+                                   parity, ok, abort_flag, a.err)
+      if (c <= 8) FRANK_STAGE(1);
+      else if (c <= 16) FRANK_STAGE(2);
+      else if (c <= 32) FRANK_STAGE(4);
+      else FRANK_STAGE(8);
+#undef FRANK_STAGE
+      __syncwarp();
+      if (lane == 0 && ok) sm.issue();
+    }
+    if (!ok) break;
+    if constexpr (UP) {
+      // h of 8 columns: row lane / 4, this lane's two tokens of each group
+      const int f = i * 8 + (lane >> 2), fb = i * 8 / kQB;
+#pragma unroll
+      for (int g = 0; g < kMaxGroups; ++g)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int t = g * 8 + (lane & 3) * 2 + j;
+          if (t < c && f < a.F) a.h[(int64_t)tb.slots[c0 + t] * a.F + f] = acc[g][j] * silu_ref(acc[g][2 + j]);
+        }
+      __threadfence();
+      __syncwarp();
+      int old = 0;
+      if (lane == 0) old = atomicAdd(a.count + (int64_t)e * nbn + fb, 1);
+      old = __shfl_sync(0xffffffffu, old, 0);
+      if (old == min(kQB / 8, sm.per - fb * (kQB / 8)) - 1) {
+        // the block's last item: its 128 values of every slot, four a lane
+        __threadfence();
+        const int fq = fb * kQB + lane * 4;
+#pragma unroll 4
+        for (int t = 0; t < c; ++t) {
+          const int slot = tb.slots[c0 + t];
+          float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (fq < a.F) q = __ldcg(reinterpret_cast<const float4*>(a.h + (int64_t)slot * a.F + fq));
+          const BlockScale sc = block_scale(__reduce_max_sync(
+              0xffffffffu, max(max(abs_bits(q.x), abs_bits(q.y)), max(abs_bits(q.z), abs_bits(q.w)))));
+          if (fq < a.F)
+            *reinterpret_cast<uint32_t*>(a.hq + (int64_t)slot * a.F + fq) =
+                e4m3x4(q.x * sc.inv, q.y * sc.inv, q.z * sc.inv, q.w * sc.inv);
+          if (lane == 0) a.hs[(int64_t)fb * n + slot] = sc.scale;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < kMaxGroups; ++g)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int slot = col[g][j & 1], r = i * ROWS + (lane >> 2) + (j >> 1) * 8;
+          if (slot >= 0 && (j < 2 || ROWS == 16) && r < a.H) a.d[(int64_t)slot * a.H + r] = acc[g][j] * a.w[slot];
+        }
+    }
   }
-  __syncthreads();
-}
-
-template <int SPLIT>
-__global__ void __launch_bounds__(kFewThreads, 2) few_down_kernel(const FewArgs a) {
-  __shared__ int slots[kFewMaxSlots];
-  __shared__ int expert;
-  __shared__ float red[kFewThreads / 32][kGroups][4][32];
-  const int nrb = (a.H + 128 / SPLIT - 1) / (128 / SPLIT);
-  const int unit = blockIdx.x / nrb, rb = blockIdx.x % nrb;
-  pdl_wait();
-  pdl_launch();
-  const int c = unit_slots(a, unit, slots, &expert);
-  for (int c0 = 0; c0 < c; c0 += kFewChunk) {
-    if (c - c0 <= 8) down_chunk<1, SPLIT>(a, expert, slots, c0, c, rb, red);
-    else down_chunk<kGroups, SPLIT>(a, expert, slots, c0, c, rb, red);
+  if (!ok) {  // no copy may land after this CTA is gone; these waits are bounded too
+    abort_word = 0;
+    for (uint32_t s = it; s < __shfl_sync(0xffffffffu, sm.issued, 0); ++s)
+      mbar_wait(sm.bar + 8 * (s % kStages), (s / kStages) & 1u, abort_flag, a.err);
   }
 }
 
@@ -525,26 +558,61 @@ int launch_few_route(const FewRoute& a, cudaStream_t st) {
   return FRANK_OK;
 }
 
-int launch_few_experts(const FewArgs& a, int32_t* err, cudaStream_t st) {
-  const int n = a.k * a.T, units = n <= a.E ? n : a.E;
-  if (err != nullptr) {
-    FRANK_CUDA_TRY(launch_chained(few_check_ids_kernel, dim3(1), dim3(256), 0, st, 1, a.ids, n, a.E, err));
-    FRANK_LAUNCH_CHECK();
+// Map of e4m3 [E, N, K] as 8-byte elements, box 512 bytes x rows.
+static int few_map(CUtensorMap* m, const void* base, int64_t E, int64_t N, int64_t K, uint32_t rows) {
+  static PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }();
+  if (!enc) {
+    set_error("cuTensorMapEncodeTiled unavailable");
+    return FRANK_ECUDA;
   }
-  const unsigned nbf = (unsigned)q_blocks(a.F);
+  const cuuint64_t dims[3] = {(cuuint64_t)K / 8, (cuuint64_t)N, (cuuint64_t)E};
+  const cuuint64_t strides[2] = {(cuuint64_t)K, (cuuint64_t)(N * K)};
+  const cuuint32_t box[3] = {kChunkK / 8, rows, 1}, estr[3] = {1, 1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_INT64, 3, const_cast<void*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled([%lld, %lld, %lld] bytes) failed: %d", (long long)E, (long long)N, (long long)K,
+              (int)r);
+    return FRANK_ECUDA;
+  }
+  return FRANK_OK;
+}
+
+template <bool UP, int ROWS>
+static int launch_few_product(const FewMaps& maps, const FewArgs& a, cudaStream_t st) {
+  const size_t smem = 128 + (size_t)kWarps * kStages * kStageBytes;
   FRANK_CUDA_TRY(
-      launch_chained(few_up_kernel, dim3(units * nbf * kUpCtas), dim3(kFewThreads), 0, st, kUpCtas, a));
-  FRANK_LAUNCH_CHECK();
-  // long rows are split over all eight warps, so that a CTA's loads cover them sooner
-  if (nbf >= 32) {
-    FRANK_CUDA_TRY(
-        launch_chained(few_down_kernel<8>, dim3(units * (unsigned)((a.H + 15) / 16)), dim3(kFewThreads), 0, st, 1, a));
-  } else {
-    FRANK_CUDA_TRY(
-        launch_chained(few_down_kernel<2>, dim3(units * (unsigned)((a.H + 63) / 64)), dim3(kFewThreads), 0, st, 1, a));
-  }
+      cudaFuncSetAttribute(few_product_kernel<UP, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  FRANK_CUDA_TRY(
+      launch_chained(few_product_kernel<UP, ROWS>, dim3(num_sms()), dim3(kFewThreads), smem, st, 1, maps, a));
   FRANK_LAUNCH_CHECK();
   return FRANK_OK;
+}
+
+int launch_few_experts(const FewArgs& args, int32_t* err, cudaStream_t st) {
+  FewArgs a = args;
+  a.err = device_error_word();
+  if (err != nullptr) {
+    FRANK_CUDA_TRY(launch_chained(few_check_ids_kernel, dim3(1), dim3(256), 0, st, 1, a.ids, a.k * a.T, a.E, err));
+    FRANK_LAUNCH_CHECK();
+  }
+  FewMaps up, down;
+  FRANK_TRY(few_map(&up.a, a.w_gate, a.E, a.F, a.H, 8));
+  FRANK_TRY(few_map(&up.b, a.w_up, a.E, a.F, a.H, 8));
+  FRANK_TRY((launch_few_product<true, 16>(up, a, st)));
+  // An item of 16 rows of 4096 values or more holds an SM's last warp too long: 8 rows then.
+  const bool wide = a.F < 4096;
+  FRANK_TRY(few_map(&down.a, a.w_down, a.E, a.H, a.F, wide ? 16 : 8));
+  down.b = down.a;
+  return wide ? launch_few_product<false, 16>(down, a, st) : launch_few_product<false, 8>(down, a, st);
 }
 
 }  // namespace frank

@@ -32,6 +32,11 @@ struct Fp8Weights {
   const float *s_up, *s_gate, *s_down;
 };
 
+// A few tokens: the weights bound the call, and few_fp8.cu reads them once.
+static bool few_tokens(int64_t T, int64_t k, int64_t E, int64_t F) {
+  return T <= kFewMaxT && k * T <= kFewMaxSlots && E * q_blocks(F) <= kFewMaxCounts;
+}
+
 // Workspace of one call; the same for a block, its experts and its sub-layer
 // (which adds the normalised tokens).
 struct Fp8MoeWs {
@@ -47,6 +52,8 @@ struct Fp8MoeWs {
   uint8_t* hq;            // [n, F]
   float* hs;              // [F/128, n]
   float* d;               // [n, H]
+  int32_t* count;         // [E, F/128] and h [n, F], for a few tokens
+  float* h;
   float* logits;
   void* perm;
   size_t perm_bytes;
@@ -69,6 +76,9 @@ static size_t fp8_moe_layout(int64_t T, int64_t H, int64_t F, int64_t E, int64_t
   l.hq = c.take<uint8_t>(n * F);
   l.hs = c.take<float>(n * q_blocks(F));
   l.d = c.take<float>(n * H);
+  const bool few = few_tokens(T, k, E, F);
+  l.count = c.take<int32_t>(few ? E * q_blocks(F) : 0);
+  l.h = c.take<float>(few ? n * F : 0);
   l.logits = c.take<float>(router_scratch_bytes(FRANK_BF16, T, H, E) / sizeof(float) + 1);
   l.perm_bytes = permute_workspace_size(n, E);
   l.perm = c.take<char>(l.perm_bytes);
@@ -98,9 +108,6 @@ static int check_moe(const char* what, int64_t T, int64_t E, int64_t k, int64_t 
   return FRANK_OK;
 }
 
-// A few tokens: the weights bound the call, and few_fp8.cu reads them once.
-static bool few_tokens(int64_t T, int64_t k) { return T <= 64 && k * T <= kFewMaxSlots; }
-
 static FewArgs few_args(const Fp8Weights& W, int64_t T, int64_t E, int64_t k, int64_t H, int64_t F, const float* w,
                         const int32_t* ids, const Fp8MoeWs& L) {
   FewArgs a;
@@ -112,6 +119,8 @@ static FewArgs few_args(const Fp8Weights& W, int64_t T, int64_t E, int64_t k, in
   a.s_down = W.s_down;
   a.xq = L.xq;
   a.xs = L.xs;
+  a.count = L.count;
+  a.h = L.h;
   a.hq = L.hq;
   a.hs = L.hs;
   a.d = L.d;
@@ -125,12 +134,37 @@ static FewArgs few_args(const Fp8Weights& W, int64_t T, int64_t E, int64_t k, in
   return a;
 }
 
+static FewRoute few_route(int x_dtype, const void* x, const float* norm_w, float eps, int wr_dtype, const void* wr,
+                          int64_t T, int64_t E, int64_t k, int64_t H, int64_t F, int normalize, float* w, int32_t* ids,
+                          const Fp8MoeWs& L) {
+  FewRoute r;
+  r.x = x;
+  r.x_dtype = x_dtype;
+  r.norm_w = norm_w;
+  r.eps = eps;
+  r.wr = wr;
+  r.wr_dtype = wr_dtype;
+  r.T = (int)T;
+  r.H = (int)H;
+  r.E = (int)E;
+  r.k = (int)k;
+  r.normalize = normalize;
+  r.xq = L.xq;
+  r.xs = L.xs;
+  r.w = w;
+  r.ids = ids;
+  r.count = L.count;
+  r.n_count = (int)(E * q_blocks(F));
+  return r;
+}
+
 // Routed rows through the experts: L.d[r] = w * down(q(h)) for the expert-sorted rows r.
 static int run_experts(const void* x, const float* w, const int32_t* ids, const Fp8Weights& W, int64_t T, int64_t E,
                        int64_t k, int64_t H, int64_t F, int32_t* err, const Fp8MoeWs& L, cudaStream_t st) {
   const int64_t n = k * T;
-  if (few_tokens(T, k)) {
-    FRANK_TRY(launch_quantize_rows(FRANK_BF16, x, T, H, nullptr, 1, L.xq, L.xs, st));
+  if (few_tokens(T, k, E, F)) {
+    FRANK_TRY(launch_few_route(few_route(FRANK_BF16, x, nullptr, 0.f, FRANK_F32, nullptr, T, E, k, H, F, 0, nullptr,
+                                         nullptr, L), st));
     return launch_few_experts(few_args(W, T, E, k, H, F, w, ids, L), err, st);
   }
   FRANK_TRY(launch_permute(ids, n, E, L.sorted_slots, L.offsets, L.slot_pos, err, L.perm, L.perm_bytes, st, w,
@@ -169,10 +203,11 @@ static int run_experts(const void* x, const float* w, const int32_t* ids, const 
   return launch_fp8_gemm(d, st);
 }
 
-static NormRows combine_of(const Fp8MoeWs& L, int64_t T, int64_t k, int64_t H, int out_dtype, void* out) {
+static NormRows combine_of(const Fp8MoeWs& L, int64_t T, int64_t E, int64_t k, int64_t H, int64_t F, int out_dtype,
+                           void* out) {
   NormRows a;
   a.d = L.d;
-  a.slot_pos = few_tokens(T, k) ? nullptr : L.slot_pos;
+  a.slot_pos = few_tokens(T, k, E, F) ? nullptr : L.slot_pos;
   a.k = (int)k;
   a.T = T;
   a.H = H;
@@ -192,24 +227,9 @@ static int route_and_run(int x_dtype, const void* x, const float* norm_w, float 
   }
   FRANK_TRY(check_float_dtype(wr_dtype, "fp8_moe router"));
   FRANK_CHECK_ARG(wr != nullptr, "fp8_moe router: null pointer");
-  if (few_tokens(T, k)) {
-    FewRoute r;
-    r.x = x;
-    r.x_dtype = x_dtype;
-    r.norm_w = norm_w;
-    r.eps = eps;
-    r.wr = wr;
-    r.wr_dtype = wr_dtype;
-    r.T = (int)T;
-    r.H = (int)H;
-    r.E = (int)E;
-    r.k = (int)k;
-    r.normalize = normalize;
-    r.xq = L.xq;
-    r.xs = L.xs;
-    r.w = w;
-    r.ids = ids;
-    FRANK_TRY(launch_few_route(r, st));
+  if (few_tokens(T, k, E, F)) {
+    FRANK_TRY(launch_few_route(
+        few_route(x_dtype, x, norm_w, eps, wr_dtype, wr, T, E, k, H, F, normalize, w, ids, L), st));
     return launch_few_experts(few_args(W, T, E, k, H, F, w, ids, L), nullptr, st);
   }
   if (norm_w != nullptr) {
@@ -327,7 +347,7 @@ int frank_fp8_moe_experts(const void* x, const float* route_w, const int32_t* ro
   Fp8MoeWs L;
   fp8_moe_layout(T, H, F, E, k, workspace, ws_bytes, &L);
   FRANK_TRY(run_experts(x, route_w, route_ids, W, T, E, k, H, F, err_flag, L, st));
-  return launch_norm_rows(combine_of(L, T, k, H, y_dtype, y), st);
+  return launch_norm_rows(combine_of(L, T, E, k, H, F, y_dtype, y), st);
 }
 
 int frank_fp8_moe_block(const void* x, int wr_dtype, const void* wr, const void* w_up, const float* s_up,
@@ -346,7 +366,7 @@ int frank_fp8_moe_block(const void* x, int wr_dtype, const void* wr, const void*
   float* w = route_w ? route_w : L.w;
   int32_t* ids = route_ids ? route_ids : L.ids;
   FRANK_TRY(route_and_run(FRANK_BF16, x, nullptr, 0.f, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
-  return launch_norm_rows(combine_of(L, T, k, H, y_dtype, y), st);
+  return launch_norm_rows(combine_of(L, T, E, k, H, F, y_dtype, y), st);
 }
 
 int frank_fp8_moe_sublayer(int res_dtype, const void* residual, const float* norm_w, float eps, int wr_dtype,
@@ -369,7 +389,7 @@ int frank_fp8_moe_sublayer(int res_dtype, const void* residual, const float* nor
   int32_t* ids = route_ids ? route_ids : L.ids;
   FRANK_TRY(
       route_and_run(res_dtype, residual, norm_w, eps, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
-  NormRows a = combine_of(L, T, k, H, res_dtype, out);
+  NormRows a = combine_of(L, T, E, k, H, F, res_dtype, out);
   a.post_w = post_w;
   a.eps = eps;
   a.gate = gate;

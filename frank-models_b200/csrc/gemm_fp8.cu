@@ -72,25 +72,6 @@ struct Params {
   int32_t* err;
 };
 
-// Bounded wait without a call: the epilogue waits with 128 live accumulators.
-__device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, volatile int* abort, int32_t* err) {
-  uint64_t t0 = 0;
-  for (uint32_t i = 0;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 255u) == 255u) {
-      if (*abort) return false;
-      const uint64_t now = global_ns();
-      if (t0 == 0) {
-        t0 = now;
-      } else if (now - t0 > 2000000000ull) {
-        *abort = 1;
-        atomicExch(err, FRANK_ETIMEOUT);
-        return false;
-      }
-    }
-  }
-}
-
 // ------------------------------------------------------------ PTX glue --
 __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
@@ -220,7 +201,7 @@ __device__ __forceinline__ bool tile_out(const Params& p, const Tile& tl, int ro
     mine[half * 128] = m;
     __syncwarp();
     if (lane == 0) mbar_arrive(row_bar);
-    if (!wait_inline(row_bar, parity, abort_flag, p.err)) return false;
+    if (!mbar_wait_inline(row_bar, parity, abort_flag, p.err)) return false;
     m = max(m, mine[(half ^ 1) * 128]);
     const BlockScale s = block_scale(m);
     uint4 v[4];
@@ -348,7 +329,7 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
         const uint32_t a_bytes = kTileBytes >> box;
         for (int kb = 0; kb < p.nk; ++kb, ++it) {
           const int s = it % kStages;
-          if (!wait_inline(empty_bar(s), ((it / kStages) & 1u) ^ 1u, abort_flag, p.err)) {
+          if (!mbar_wait_inline(empty_bar(s), ((it / kStages) & 1u) ^ 1u, abort_flag, p.err)) {
             ok = false;
             break;
           }
@@ -372,8 +353,8 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
         for (int kb = 0; kb < p.nk; ++kb, ++it) {
           const int s = it % kStages;
           const uint32_t a = it & 1u;
-          if (!wait_inline(tempty_bar(a), ((it >> 1) & 1u) ^ 1u, abort_flag, p.err) ||
-              !wait_inline(full_bar(s), (it / kStages) & 1u, abort_flag, p.err)) {
+          if (!mbar_wait_inline(tempty_bar(a), ((it >> 1) & 1u) ^ 1u, abort_flag, p.err) ||
+              !mbar_wait_inline(full_bar(s), (it / kStages) & 1u, abort_flag, p.err)) {
             ok = false;
             break;
           }
@@ -424,7 +405,7 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
         const float s0 = a0 * w0, s1 = MODE == FP8_SWIGLU ? a0 * u0 : s0;
         a0 = a1, w0 = w1, u0 = u1;
         if (work && kb + 2 < p.nk) next_scales(a1, w1, u1);
-        if (!wait_inline(tfull_bar(a), (it >> 1) & 1u, abort_flag, p.err)) {
+        if (!mbar_wait_inline(tfull_bar(a), (it >> 1) & 1u, abort_flag, p.err)) {
           ok = false;
           break;
         }

@@ -62,6 +62,25 @@ __device__ __noinline__ inline bool mbar_wait(uint32_t bar, uint32_t parity, vol
   }
 }
 
+// mbar_wait without a call, for code that waits with many live registers.
+__device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, volatile int* abort, int32_t* err,
+                                                 uint64_t limit_ns = 2000000000ull) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 255u) {
+      if (*abort) return false;
+      const uint64_t now = global_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > limit_ns) {
+        *abort = 1;
+        atomicExch(err, FRANK_ETIMEOUT);
+        return false;
+      }
+    }
+  }
+}
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
