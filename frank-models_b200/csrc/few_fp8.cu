@@ -14,10 +14,9 @@
 // weight rows come by TMA, 8 KB (16 rows x 512 values) a stage, three stages a warp,
 // so 192 KB an SM are under way and no warp waits for another one.  A warp
 // multiplies 16 weight rows (8 of gate and the same 8 of up, or 16 of down) with 8
-// tokens by mma.m16n8k16 in fp16, into which e4m3 converts exactly, with fp32
-// sums; one K block is summed and then scaled.  Lane t of a quad holds K elements
-// 16 t .. 16 t + 15 of a row: the MMA's K index is permuted alike for weights and
-// tokens, which leaves the sum.
+// tokens by mma.m16n8k32 (e4m3, fp32 sums); one K block is summed and then
+// scaled.  Lane t of a quad holds K elements 16 t .. 16 t + 15 of a row: the MMA's
+// K index is permuted alike for weights and tokens, which leaves the sum.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -241,28 +240,19 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
 }
 
 // ------------------------------------------------------------- products --
-__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+__device__ __forceinline__ void mma_16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void to_half(const uint4& v, uint32_t (&h)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    h[2 * i] = e4m3x2_to_half2(w[i] & 0xffffu);
-    h[2 * i + 1] = e4m3x2_to_half2(w[i] >> 16);
-  }
 }
 
 constexpr int kWarps = 8, kFewThreads = 32 * kWarps;
 constexpr int kChunkK = 512, kChunkB = kChunkK / kQB;      // values and blocks along K of a stage
 constexpr int kRows = 16, kStages = 3;
 constexpr int kStageBytes = kRows * kChunkK;
-constexpr int kMaxGroups = 8;  // of 8 tokens: an expert has at most 64
+static_assert(kFewMaxT <= 64, "an expert has at most 8 groups of 8 tokens");
 
 struct FewMaps {
   CUtensorMap a, b;  // few_up: gate and up; few_down: down
@@ -274,6 +264,7 @@ struct Table {
   int expert[kFewMaxE];
   int start[kFewMaxE + 1];
   int slots[kFewMaxSlots];
+  int tokens[kFewMaxSlots];  // of the slots
 };
 
 __device__ __forceinline__ void build_table(const FewArgs& a, Table& tb, int* sid, int* sums) {
@@ -301,7 +292,7 @@ __device__ __forceinline__ void build_table(const FewArgs& a, Table& tb, int* si
     tb.expert[before >> 16] = tid;
     tb.start[before >> 16] = at;
     for (int s = 0; s < n; ++s)
-      if (sid[s] == tid) tb.slots[at++] = s;
+      if (sid[s] == tid) tb.slots[at] = s, tb.tokens[at++] = s % a.T;
   }
   if (tid == 0) tb.nact = total >> 16, tb.start[total >> 16] = n;
   __syncthreads();
@@ -313,73 +304,6 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
           dst),
       "l"(map), "r"(k8), "r"(row), "r"(e), "r"(bar)
       : "memory");
-}
-
-// One stage: acc[g] += 16 rows x the tokens of group g over the blocks [b0, b0 + 4) of K.
-// tok / col: this lane's token row of the product and the rows of its two accumulator columns, or -1.
-template <int G, int ROWS>
-__device__ __forceinline__ void stage_product(float (&acc)[kMaxGroups][4], const uint8_t* st, const uint8_t* x,
-                                              const float* x_scale, int64_t ld_scale, const float* s0,
-                                              const float* s1, const int* tok, const int (*col)[2], int K, int b0,
-                                              int nb, uint32_t bar, uint32_t parity, bool& ok, volatile int* abort,
-                                              int32_t* err) {
-  const int lane = threadIdx.x & 31, row = lane >> 2, k_lane = (lane & 3) * 16;
-  // up to 16 tokens: everything but the weights is loaded before they are waited for
-  constexpr bool kAhead = G <= 2;
-  uint4 v[kAhead ? G : 1][kChunkB][2];
-  float xs[kAhead ? G : 1][kChunkB][2], f0[kChunkB], f1[kChunkB];
-  auto tokens = [&](int g, int i, uint4 (&q)[2], float (&sc)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = (b0 + i) * kQB + h * 64 + k_lane;
-      q[h] = make_uint4(0u, 0u, 0u, 0u);
-      if (tok[g] >= 0 && k < K) q[h] = *reinterpret_cast<const uint4*>(x + (int64_t)tok[g] * K + k);
-      sc[h] = b0 + i < nb && col[g][h] >= 0 ? x_scale[(b0 + i) * ld_scale + col[g][h]] : 0.f;
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kChunkB; ++i) {
-    const bool in = b0 + i < nb;
-    f0[i] = in ? __ldg(s0 + b0 + i) : 0.f;
-    f1[i] = in ? __ldg(s1 + b0 + i) : 0.f;
-    if (kAhead) {
-#pragma unroll
-      for (int g = 0; g < G; ++g) tokens(g, i, v[g][i], xs[g][i]);
-    }
-  }
-  if (!mbar_wait_inline(bar, parity, abort, err)) ok = false;
-#pragma unroll
-  for (int i = 0; i < kChunkB; ++i) {
-    if (b0 + i < nb) {
-      uint32_t a0[2][8], a1[2][8] = {};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* p = st + row * kChunkK + i * kQB + h * 64 + k_lane;
-        to_half(*reinterpret_cast<const uint4*>(p), a0[h]);
-        if (ROWS == 16) to_half(*reinterpret_cast<const uint4*>(p + 8 * kChunkK), a1[h]);
-      }
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        float part[4] = {};
-        uint4 q[2];
-        float sc[2];
-        if (!kAhead) tokens(g, i, q, sc);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t t[8];
-          to_half(kAhead ? v[kAhead ? g : 0][i][h] : q[h], t);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_16816(part, a0[h][2 * j], a1[h][2 * j], a0[h][2 * j + 1], a1[h][2 * j + 1], t[2 * j], t[2 * j + 1]);
-        }
-        const float x0 = kAhead ? xs[kAhead ? g : 0][i][0] : sc[0], x1 = kAhead ? xs[kAhead ? g : 0][i][1] : sc[1];
-        acc[g][0] = fmaf(part[0], x0 * f0[i], acc[g][0]);
-        acc[g][1] = fmaf(part[1], x1 * f0[i], acc[g][1]);
-        acc[g][2] = fmaf(part[2], x0 * f1[i], acc[g][2]);
-        acc[g][3] = fmaf(part[3], x1 * f1[i], acc[g][3]);
-      }
-    }
-  }
 }
 
 // The stream of one warp's stages: item after item, chunk after chunk along K.  Lane 0
@@ -408,6 +332,167 @@ struct Stream {
   }
 };
 
+// One stage: acc[g] += 16 rows x the tokens of group g over four blocks of K.
+//   xp[g]: this lane's token row at its K elements of the first block, null: no token
+//   sp[g][2]: scales of its two accumulator columns' rows at the first block, null: no column
+//   FULL: all four blocks are whole; else left < 512 values of K are left
+template <int G, int ROWS, bool FULL>
+__device__ __forceinline__ void stage_product(float (&acc)[G][4], const uint8_t* st, const uint8_t* const (&xp)[G],
+                                              const float* const (&sp)[G][2], uint32_t ld_scale, const float* s0,
+                                              const float* s1, int left, uint32_t bar, uint32_t parity, bool& ok,
+                                              volatile int* abort, int32_t* err) {
+  const int lane = threadIdx.x & 31, k_lane = (lane & 3) * 16;
+  // up to 16 tokens: everything but the weights is loaded before they are waited for
+  constexpr bool kAhead = G <= 2;
+  uint4 v[kAhead ? G : 1][kChunkB][2];
+  float xs[kAhead ? G : 1][kChunkB][2], f0[kChunkB], f1[kChunkB];
+  auto tokens = [&](int g, int i, uint4 (&q)[2], float (&sc)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      q[h] = make_uint4(0u, 0u, 0u, 0u);
+      if (xp[g] != nullptr && (FULL || i * kQB + h * 64 + k_lane < left))
+        q[h] = *reinterpret_cast<const uint4*>(xp[g] + i * kQB + h * 64);
+      sc[h] = 0.f;
+      if (sp[g][h] != nullptr && (FULL || i * kQB < left)) sc[h] = sp[g][h][i * ld_scale];
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kChunkB; ++i) {
+    f0[i] = FULL || i * kQB < left ? __ldg(s0 + i) : 0.f;
+    f1[i] = f0[i];
+    if (s1 != s0) f1[i] = FULL || i * kQB < left ? __ldg(s1 + i) : 0.f;
+    if (kAhead) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) tokens(g, i, v[g][i], xs[g][i]);
+    }
+  }
+  if (!mbar_wait_inline(bar, parity, abort, err)) ok = false;
+  const uint8_t* w = st + (lane >> 2) * kChunkK + k_lane;
+#pragma unroll
+  for (int i = 0; i < kChunkB; ++i) {
+    if (!FULL && i * kQB >= left) break;
+    uint4 a0[2], a1[2] = {};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      a0[h] = *reinterpret_cast<const uint4*>(w + i * kQB + h * 64);
+      if (ROWS == 16) a1[h] = *reinterpret_cast<const uint4*>(w + 8 * kChunkK + i * kQB + h * 64);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float part[4] = {};
+      uint4 q[2];
+      float sc[2];
+      if (!kAhead) tokens(g, i, q, sc);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 t = kAhead ? v[kAhead ? g : 0][i][h] : q[h];
+        mma_16832(part, a0[h].x, a1[h].x, a0[h].y, a1[h].y, t.x, t.y);
+        mma_16832(part, a0[h].z, a1[h].z, a0[h].w, a1[h].w, t.z, t.w);
+      }
+      const float x0 = kAhead ? xs[kAhead ? g : 0][i][0] : sc[0], x1 = kAhead ? xs[kAhead ? g : 0][i][1] : sc[1];
+      acc[g][0] = fmaf(part[0], x0 * f0[i], acc[g][0]);
+      acc[g][1] = fmaf(part[1], x1 * f0[i], acc[g][1]);
+      acc[g][2] = fmaf(part[2], x0 * f1[i], acc[g][2]);
+      acc[g][3] = fmaf(part[3], x1 * f1[i], acc[g][3]);
+    }
+  }
+}
+
+// One item: rows i * 8 .. of gate and up, or i * ROWS .. of down, of the ai-th active expert.
+template <bool UP, int ROWS, int G>
+__device__ __forceinline__ bool run_item(const FewArgs& a, const Table& tb, Stream<UP, ROWS>& sm, int ai, int i,
+                                         uint32_t& it, volatile int* abort_flag) {
+  const int lane = threadIdx.x & 31, n = a.k * a.T, K = UP ? a.H : a.F, N = UP ? a.F : a.H;
+  const int nb = (K + kQB - 1) / kQB, nbn = (N + kQB - 1) / kQB;
+  const int e = tb.expert[ai], c0 = tb.start[ai], c = tb.start[ai + 1] - c0;
+  const int* rows = (UP ? tb.tokens : tb.slots) + c0;  // of the token operand
+  const uint32_t ld = UP ? a.T : n;
+  const uint8_t* xp[G];
+  const float* sp[G][2];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const int t = g * 8 + (lane >> 2), u = g * 8 + (lane & 3) * 2;
+    xp[g] = t < c ? (UP ? a.xq : a.hq) + (int64_t)rows[t] * K + (lane & 3) * 16 : nullptr;
+    sp[g][0] = u < c ? (UP ? a.xs : a.hs) + rows[u] : nullptr;
+    sp[g][1] = u + 1 < c ? (UP ? a.xs : a.hs) + rows[u + 1] : nullptr;
+  }
+  const int64_t so = ((int64_t)e * nbn + i * (UP ? 8 : ROWS) / kQB) * nb;
+  const float* s0 = (UP ? a.s_gate : a.s_down) + so;
+  const float* s1 = (UP ? a.s_up : a.s_down) + so;
+  float acc[G][4] = {};
+  bool ok = true;
+#pragma unroll 1
+  for (int left = K; left > 0 && ok; left -= kChunkK, ++it) {
+    const uint32_t s = it % kStages, parity = (it / kStages) & 1u;
+    const uint8_t* st = sm.smem + s * kStageBytes;
+    if (left >= kChunkK)
+      stage_product<G, UP ? 16 : ROWS, true>(acc, st, xp, sp, ld, s0, s1, left, sm.bar + 8 * s, parity, ok, abort_flag,
+                                             a.err);
+    else
+      stage_product<G, UP ? 16 : ROWS, false>(acc, st, xp, sp, ld, s0, s1, left, sm.bar + 8 * s, parity, ok,
+                                              abort_flag, a.err);
+    __syncwarp();
+    if (lane == 0 && ok) sm.issue();
+    s0 += kChunkB;
+    s1 += kChunkB;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if (xp[g] != nullptr) xp[g] += kChunkK;
+      if (sp[g][0] != nullptr) sp[g][0] += kChunkB * ld;
+      if (sp[g][1] != nullptr) sp[g][1] += kChunkB * ld;
+    }
+  }
+  if (!ok) return false;
+  if constexpr (UP) {
+    // h of 8 columns: column lane / 4, this lane's two tokens of each group
+    const int f = i * 8 + (lane >> 2), fb = i * 8 / kQB;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int t = g * 8 + (lane & 3) * 2 + j;
+        if (t < c) a.h[(int64_t)tb.slots[c0 + t] * a.F + f] = acc[g][j] * silu_ref(acc[g][2 + j]);
+      }
+    __threadfence();
+    __syncwarp();
+    int old = 0;
+    if (lane == 0) old = atomicAdd(a.count + (int64_t)e * nbn + fb, 1);
+    old = __shfl_sync(0xffffffffu, old, 0);
+    if (old == min(kQB / 8, sm.per - fb * (kQB / 8)) - 1) {
+      // the block's last item: its 128 values of every slot, four a lane
+      __threadfence();
+      const int fq = fb * kQB + lane * 4;
+#pragma unroll 4
+      for (int t = 0; t < c; ++t) {
+        const int slot = tb.slots[c0 + t];
+        float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (fq < a.F) q = __ldcg(reinterpret_cast<const float4*>(a.h + (int64_t)slot * a.F + fq));
+        const BlockScale sc = block_scale(__reduce_max_sync(
+            0xffffffffu, max(max(abs_bits(q.x), abs_bits(q.y)), max(abs_bits(q.z), abs_bits(q.w)))));
+        if (fq < a.F)
+          *reinterpret_cast<uint32_t*>(a.hq + (int64_t)slot * a.F + fq) =
+              e4m3x4(q.x * sc.inv, q.y * sc.inv, q.z * sc.inv, q.w * sc.inv);
+        if (lane == 0) a.hs[(int64_t)fb * n + slot] = sc.scale;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int t = g * 8 + (lane & 3) * 2 + j;
+        if (t < c) {
+          const int slot = tb.slots[c0 + t];
+          const float w = a.w[slot];
+          float* d = a.d + (int64_t)slot * a.H + i * ROWS + (lane >> 2);
+          d[0] = acc[g][j] * w;
+          if (ROWS == 16) d[8] = acc[g][2 + j] * w;
+        }
+      }
+  }
+  return true;
+}
+
 template <bool UP, int ROWS>
 __global__ void __launch_bounds__(kFewThreads, 1)
 few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ FewArgs a) {
@@ -429,16 +514,16 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
   pdl_launch();
   build_table(a, tb, sid, sums);  // and the barriers are initialised
 
-  const int n = a.k * a.T, K = UP ? a.H : a.F, N = UP ? a.F : a.H;
-  const int nb = (K + kQB - 1) / kQB, nbn = (N + kQB - 1) / kQB;
+  // F and H are multiples of 16: no item is short
+  const int K = UP ? a.H : a.F, N = UP ? a.F : a.H;
   Stream<UP, ROWS> sm;
   sm.maps = &maps;
   sm.tb = &tb;
   sm.smem = smem + warp * kStages * kStageBytes;
   sm.bar = smem_u32(&bars[warp * kStages]);
-  sm.per = (N + (UP ? 8 : ROWS) - 1) / (UP ? 8 : ROWS);
+  sm.per = N / (UP ? 8 : ROWS);
   sm.items = tb.nact * sm.per;
-  sm.chunks = (nb + kChunkB - 1) / kChunkB;
+  sm.chunks = (K + kChunkK - 1) / kChunkK;
   sm.step = gridDim.x * kWarps;
   sm.next = blockIdx.x + gridDim.x * warp;  // neighbouring items on different SMs
   sm.chunk = 0;
@@ -449,88 +534,16 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
   uint32_t it = 0;
   bool ok = true;
   for (int item = first; item < sm.items && ok; item += sm.step) {
-    const int ai = item / sm.per, i = item % sm.per, e = tb.expert[ai];
-    const int c0 = tb.start[ai], c = tb.start[ai + 1] - c0;
-    int tok[kMaxGroups], col[kMaxGroups][2];
-#pragma unroll
-    for (int g = 0; g < kMaxGroups; ++g) {
-      const int t = g * 8 + (lane >> 2), u = g * 8 + (lane & 3) * 2;
-      tok[g] = t < c ? tb.slots[c0 + t] : -1;
-      col[g][0] = u < c ? tb.slots[c0 + u] : -1;
-      col[g][1] = u + 1 < c ? tb.slots[c0 + u + 1] : -1;
-      if (UP) {  // slots of one token share its row
-        if (tok[g] >= 0) tok[g] %= a.T;
-        if (col[g][0] >= 0) col[g][0] %= a.T;
-        if (col[g][1] >= 0) col[g][1] %= a.T;
-      }
-    }
-    const int64_t so = ((int64_t)e * nbn + i * (UP ? 8 : ROWS) / kQB) * nb;
-    const float* s0 = (UP ? a.s_gate : a.s_down) + so;
-    const float* s1 = (UP ? a.s_up : a.s_down) + so;
-    const uint8_t* x = UP ? a.xq : a.hq;
-    const float* x_scale = UP ? a.xs : a.hs;
-    const int64_t ld = UP ? a.T : n;
-    float acc[kMaxGroups][4] = {};
-    for (int ch = 0; ch < sm.chunks && ok; ++ch, ++it) {
-      const uint32_t s = it % kStages, parity = (it / kStages) & 1u;
-      const uint8_t* st = sm.smem + s * kStageBytes;
-#define FRANK_STAGE(G)                                                                                             \
-  stage_product<G, UP ? 16 : ROWS>(acc, st, x, x_scale, ld, s0, s1, tok, col, K, ch * kChunkB, nb, sm.bar + 8 * s, \
-                                   parity, ok, abort_flag, a.err)
-      if (c <= 8) FRANK_STAGE(1);
-      else if (c <= 16) FRANK_STAGE(2);
-      else if (c <= 32) FRANK_STAGE(4);
-      else FRANK_STAGE(8);
-#undef FRANK_STAGE
-      __syncwarp();
-      if (lane == 0 && ok) sm.issue();
-    }
-    if (!ok) break;
-    if constexpr (UP) {
-      // h of 8 columns: row lane / 4, this lane's two tokens of each group
-      const int f = i * 8 + (lane >> 2), fb = i * 8 / kQB;
-#pragma unroll
-      for (int g = 0; g < kMaxGroups; ++g)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int t = g * 8 + (lane & 3) * 2 + j;
-          if (t < c && f < a.F) a.h[(int64_t)tb.slots[c0 + t] * a.F + f] = acc[g][j] * silu_ref(acc[g][2 + j]);
-        }
-      __threadfence();
-      __syncwarp();
-      int old = 0;
-      if (lane == 0) old = atomicAdd(a.count + (int64_t)e * nbn + fb, 1);
-      old = __shfl_sync(0xffffffffu, old, 0);
-      if (old == min(kQB / 8, sm.per - fb * (kQB / 8)) - 1) {
-        // the block's last item: its 128 values of every slot, four a lane
-        __threadfence();
-        const int fq = fb * kQB + lane * 4;
-#pragma unroll 4
-        for (int t = 0; t < c; ++t) {
-          const int slot = tb.slots[c0 + t];
-          float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (fq < a.F) q = __ldcg(reinterpret_cast<const float4*>(a.h + (int64_t)slot * a.F + fq));
-          const BlockScale sc = block_scale(__reduce_max_sync(
-              0xffffffffu, max(max(abs_bits(q.x), abs_bits(q.y)), max(abs_bits(q.z), abs_bits(q.w)))));
-          if (fq < a.F)
-            *reinterpret_cast<uint32_t*>(a.hq + (int64_t)slot * a.F + fq) =
-                e4m3x4(q.x * sc.inv, q.y * sc.inv, q.z * sc.inv, q.w * sc.inv);
-          if (lane == 0) a.hs[(int64_t)fb * n + slot] = sc.scale;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int g = 0; g < kMaxGroups; ++g)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int slot = col[g][j & 1], r = i * ROWS + (lane >> 2) + (j >> 1) * 8;
-          if (slot >= 0 && (j < 2 || ROWS == 16) && r < a.H) a.d[(int64_t)slot * a.H + r] = acc[g][j] * a.w[slot];
-        }
-    }
+    const int ai = item / sm.per, i = item - ai * sm.per, c = tb.start[ai + 1] - tb.start[ai];
+    if (c <= 8) ok = run_item<UP, ROWS, 1>(a, tb, sm, ai, i, it, abort_flag);
+    else if (c <= 16) ok = run_item<UP, ROWS, 2>(a, tb, sm, ai, i, it, abort_flag);
+    else if (c <= 32) ok = run_item<UP, ROWS, 4>(a, tb, sm, ai, i, it, abort_flag);
+    else ok = run_item<UP, ROWS, 8>(a, tb, sm, ai, i, it, abort_flag);
   }
   if (!ok) {  // no copy may land after this CTA is gone; these waits are bounded too
     abort_word = 0;
-    for (uint32_t s = it; s < __shfl_sync(0xffffffffu, sm.issued, 0); ++s)
+    const uint32_t issued = __shfl_sync(0xffffffffu, sm.issued, 0);
+    for (uint32_t s = it; s < issued; ++s)
       mbar_wait(sm.bar + 8 * (s % kStages), (s / kStages) & 1u, abort_flag, a.err);
   }
 }
