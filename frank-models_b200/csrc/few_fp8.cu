@@ -6,17 +6,19 @@
 //               CTAs take 8 tokens, each CTA an eighth of H.  The sums of squares and
 //               the partial logits are exchanged through distributed shared memory
 //               and added in CTA order.
-//   few_up      h = gate * silu(up) for items of 8 columns of F of one expert; the
-//               last of the 16 items of a quantisation block quantises it
-//   few_down    d[slot] = route weight * down(h[slot]) for items of 16 rows of one expert
+//   few_product<UP>    h = gate * silu(up), quantised: tiles of 128 columns of F (one
+//               quantisation block) of one expert, for all T tokens
+//   few_product<DOWN>  d[slot] = route weight * down(h[slot]): tiles of 128 rows of H of
+//               one expert, for its slots; along a long F in several parts, which
+//               the combine adds in order
 //
-// few_up and few_down are persistent, 8 warps an SM.  A warp takes an item by itself: its
-// weight rows come by TMA, 8 KB (16 rows x 512 values) a stage, three stages a warp,
-// so 192 KB an SM are under way and no warp waits for another one.  A warp
-// multiplies 16 weight rows (8 of gate and the same 8 of up, or 16 of down) with 8
-// tokens by mma.m16n8k32 (e4m3, fp32 sums); one K block is summed and then
-// scaled.  Lane t of a quad holds K elements 16 t .. 16 t + 15 of a row: the MMA's
-// K index is permuted alike for weights and tokens, which leaves the sum.
+// Weights and tokens change places: the 128 weight rows are the M of
+// tcgen05.mma.kind::f8f6f4 (UP: one MMA for gate, one for up), the tokens, 16 to 64
+// of them, its N.  So the weights go from TMA to the tensor core without passing
+// through a register, and a K block of 128 costs the epilogue 16 to 64 columns: they
+// are scaled and summed in fp32 registers from four TMEM buffers.  The ring of K
+// blocks keeps up to 190 KB an SM under way.  (An earlier form multiplied in warps by
+// mma.sync: 610 instructions for 8 KB of weights, 2.5 to 4 TB/s.)
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -85,7 +87,6 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
   pdl_wait();
   pdl_launch();
   cluster_arrive();  // every CTA has started before its memory is written
-  for (int i = blockIdx.x * kRouteThreads + threadIdx.x; i < a.n_count; i += gridDim.x * kRouteThreads) a.count[i] = 0;
   // one (token, block) a warp: a vector of 4 for each lane
   for (int i = warp; i < kRouteTok * sb; i += kWarps) {
     const int t = i / sb, b = i % sb, h = h0 + b * kQB + lane * 4;
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
     if (t < nt && h < a.H) {
       *reinterpret_cast<uint32_t*>(a.xq + (int64_t)(t0 + t) * a.H + h) =
           e4m3x4(v.x * s.inv, v.y * s.inv, v.z * s.inv, v.w * s.inv);
-      if (lane == 0) a.xs[(int64_t)(h / kQB) * a.T + t0 + t] = s.scale;
+      if (lane == 0) a.xs[(int64_t)(h / kQB) * kFewMaxT + t0 + t] = s.scale;
     }
   }
   if (a.wr == nullptr) return;  // the routing is given
@@ -240,41 +241,41 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
 }
 
 // ------------------------------------------------------------- products --
-__device__ __forceinline__ void mma_16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-constexpr int kWarps = 8, kFewThreads = 32 * kWarps;
-constexpr int kChunkK = 512, kChunkB = kChunkK / kQB;      // values and blocks along K of a stage
-constexpr int kRows = 16, kStages = 3;
-constexpr int kStageBytes = kRows * kChunkK;
-static_assert(kFewMaxT <= 64, "an expert has at most 8 groups of 8 tokens");
+constexpr int kFewThreads = 256;  // warp 0: TMA, warp 1: MMA, warps 4..7: epilogue
+constexpr uint32_t kTile = 128 * kQB;  // bytes of 128 weight rows of a K block
+constexpr int kMaxStages = 12, kBufs = 4, kBufCols = 128;
+constexpr uint32_t kTmemCols = kBufs * kBufCols;
 
 struct FewMaps {
-  CUtensorMap a, b;  // few_up: gate and up; few_down: down
+  CUtensorMap w, w2;   // UP: gate and up; DOWN: down (boxes of 128 rows)
+  CUtensorMap x[3];    // tokens: boxes of 16, 32 and 64 rows
 };
 
-// The routing as every CTA sees it: the experts that have tokens, ascending, and their slots.
+// The tokens a tile takes: as many as a stage has rows for (also where a caller's ids
+// name an expert twice for one token, and it has more slots than there are tokens).
+__host__ __device__ __forceinline__ int tile_tokens(int T) { return T <= 16 ? 16 : T <= 32 ? 32 : 64; }
+
+// The routing as every CTA sees it: the experts that have tokens, ascending, and their
+// slots, at most tile_tokens an entry.  An entry's rows of h start at a multiple of 16.
+constexpr int kMaxEntries = kFewMaxE + kFewMaxSlots / 16;
 struct Table {
-  int nact;
-  int expert[kFewMaxE];
-  int start[kFewMaxE + 1];
+  int entries;
+  int expert[kMaxEntries];
+  int first[kMaxEntries + 1];  // of its slots
+  int row[kMaxEntries];        // of h
   int slots[kFewMaxSlots];
-  int tokens[kFewMaxSlots];  // of the slots
 };
 
 __device__ __forceinline__ void build_table(const FewArgs& a, Table& tb, int* sid, int* sums) {
   const int n = a.k * a.T, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  static_assert(kFewThreads == kFewMaxE, "a thread counts an expert");
   for (int s = tid; s < n; s += kFewThreads) sid[s] = min(max(a.ids[s], 0), a.E - 1);
   __syncthreads();
-  // thread e counts expert e
   int c = 0;
   for (int s = 0; s < n; ++s) c += sid[s] == tid;
-  int v = c | (c != 0) << 16;  // slots and experts before this one
+  // before this expert: slots (bits 0..9), entries (10..18) and groups of 16 rows (19..)
+  const int cap = tile_tokens(a.T), mine = c | (c + cap - 1) / cap << 10 | (c + 15) / 16 << 19;
+  int v = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -282,269 +283,295 @@ __device__ __forceinline__ void build_table(const FewArgs& a, Table& tb, int* si
   }
   if (lane == 31) sums[warp] = v;
   __syncthreads();
-  int before = v - (c | (c != 0) << 16), total = 0;
-  for (int w = 0; w < kWarps; ++w) {
+  int before = v - mine, total = 0;
+  for (int w = 0; w < kFewThreads / 32; ++w) {
     if (w < warp) before += sums[w];
     total += sums[w];
   }
-  if (c != 0) {
-    int at = before & 0xffff;
-    tb.expert[before >> 16] = tid;
-    tb.start[before >> 16] = at;
-    for (int s = 0; s < n; ++s)
-      if (sid[s] == tid) tb.slots[at] = s, tb.tokens[at++] = s % a.T;
+  int at = before & 1023;
+  for (int i = 0; i * cap < c; ++i) {
+    const int entry = (before >> 10 & 511) + i;
+    tb.expert[entry] = tid;
+    tb.first[entry] = at + i * cap;
+    tb.row[entry] = (before >> 19) * 16 + i * cap;
   }
-  if (tid == 0) tb.nact = total >> 16, tb.start[total >> 16] = n;
-  __syncthreads();
+  if (c != 0)
+    for (int s = 0; s < n; ++s)
+      if (sid[s] == tid) tb.slots[at++] = s;
+  if (tid == 0) tb.entries = total >> 10 & 511, tb.first[total >> 10 & 511] = n;
 }
 
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int k8, int row, int e, uint32_t bar) {
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
           dst),
-      "l"(map), "r"(k8), "r"(row), "r"(e), "r"(bar)
+      "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// Weights are read once: first to leave L2.
+__device__ __forceinline__ void load_weights(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar,
+                                             uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, "
+      "%4}], [%5], %6;" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// K-major operand, 128-byte swizzle: rows of 128 bytes, groups of 8 rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// The stream of one warp's stages: item after item, chunk after chunk along K.  Lane 0
-// issues the loads, three stages ahead; the warp that read a stage refills it.
-//   UP: 8 rows of map a over 8 rows of map b; else ROWS rows of map a
-template <bool UP, int ROWS>
-struct Stream {
-  const FewMaps* maps;
-  const Table* tb;
-  uint8_t* smem;      // this warp's stages
-  uint32_t bar;       // this warp's barriers
-  int items, per;     // items in all, items an expert
-  int chunks;         // chunks of an item
-  int next, chunk, step;
-  uint32_t issued;
-
-  __device__ __forceinline__ void issue() {
-    if (next >= items) return;
-    const uint32_t s = issued % kStages, dst = smem_u32(smem + s * kStageBytes), b = bar + 8 * s;
-    const int e = tb->expert[next / per], i = next % per, k8 = chunk * (kChunkK / 8);
-    mbar_expect_tx(b, (UP ? 16 : ROWS) * kChunkK);
-    load_box(dst, &maps->a, k8, i * (UP ? 8 : ROWS), e, b);
-    if (UP) load_box(dst + 8 * kChunkK, &maps->b, k8, i * 8, e, b);
-    ++issued;
-    if (++chunk == chunks) chunk = 0, next += step;
-  }
+// One unit of work: tile `n` (128 rows) of the ai-th entry, K blocks [kb0, kb1).
+struct Unit {
+  int ai, n, part, kb0, kb1;
 };
-
-// One stage: acc[g] += 16 rows x the tokens of group g over four blocks of K.
-//   xp[g]: this lane's token row at its K elements of the first block, null: no token
-//   sp[g][2]: scales of its two accumulator columns' rows at the first block, null: no column
-//   FULL: all four blocks are whole; else left < 512 values of K are left
-template <int G, int ROWS, bool FULL>
-__device__ __forceinline__ void stage_product(float (&acc)[G][4], const uint8_t* st, const uint8_t* const (&xp)[G],
-                                              const float* const (&sp)[G][2], uint32_t ld_scale, const float* s0,
-                                              const float* s1, int left, uint32_t bar, uint32_t parity, bool& ok,
-                                              volatile int* abort, int32_t* err) {
-  const int lane = threadIdx.x & 31, k_lane = (lane & 3) * 16;
-  // up to 16 tokens: everything but the weights is loaded before they are waited for
-  constexpr bool kAhead = G <= 2;
-  uint4 v[kAhead ? G : 1][kChunkB][2];
-  float xs[kAhead ? G : 1][kChunkB][2], f0[kChunkB], f1[kChunkB];
-  auto tokens = [&](int g, int i, uint4 (&q)[2], float (&sc)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      q[h] = make_uint4(0u, 0u, 0u, 0u);
-      if (xp[g] != nullptr && (FULL || i * kQB + h * 64 + k_lane < left))
-        q[h] = *reinterpret_cast<const uint4*>(xp[g] + i * kQB + h * 64);
-      sc[h] = 0.f;
-      if (sp[g][h] != nullptr && (FULL || i * kQB < left)) sc[h] = sp[g][h][i * ld_scale];
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kChunkB; ++i) {
-    f0[i] = FULL || i * kQB < left ? __ldg(s0 + i) : 0.f;
-    f1[i] = f0[i];
-    if (s1 != s0) f1[i] = FULL || i * kQB < left ? __ldg(s1 + i) : 0.f;
-    if (kAhead) {
-#pragma unroll
-      for (int g = 0; g < G; ++g) tokens(g, i, v[g][i], xs[g][i]);
-    }
-  }
-  if (!mbar_wait_inline(bar, parity, abort, err)) ok = false;
-  const uint8_t* w = st + (lane >> 2) * kChunkK + k_lane;
-#pragma unroll
-  for (int i = 0; i < kChunkB; ++i) {
-    if (!FULL && i * kQB >= left) break;
-    uint4 a0[2], a1[2] = {};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      a0[h] = *reinterpret_cast<const uint4*>(w + i * kQB + h * 64);
-      if (ROWS == 16) a1[h] = *reinterpret_cast<const uint4*>(w + 8 * kChunkK + i * kQB + h * 64);
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      float part[4] = {};
-      uint4 q[2];
-      float sc[2];
-      if (!kAhead) tokens(g, i, q, sc);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 t = kAhead ? v[kAhead ? g : 0][i][h] : q[h];
-        mma_16832(part, a0[h].x, a1[h].x, a0[h].y, a1[h].y, t.x, t.y);
-        mma_16832(part, a0[h].z, a1[h].z, a0[h].w, a1[h].w, t.z, t.w);
-      }
-      const float x0 = kAhead ? xs[kAhead ? g : 0][i][0] : sc[0], x1 = kAhead ? xs[kAhead ? g : 0][i][1] : sc[1];
-      acc[g][0] = fmaf(part[0], x0 * f0[i], acc[g][0]);
-      acc[g][1] = fmaf(part[1], x1 * f0[i], acc[g][1]);
-      acc[g][2] = fmaf(part[2], x0 * f1[i], acc[g][2]);
-      acc[g][3] = fmaf(part[3], x1 * f1[i], acc[g][3]);
-    }
-  }
+__device__ __forceinline__ Unit unit_at(const FewArgs& a, int u, int tiles, int parts, int nb) {
+  Unit t;
+  t.part = u % parts;
+  t.n = u / parts % tiles;
+  t.ai = u / parts / tiles;
+  t.kb0 = nb * t.part / parts;
+  t.kb1 = nb * (t.part + 1) / parts;
+  return t;
 }
 
-// One item: rows i * 8 .. of gate and up, or i * ROWS .. of down, of the ai-th active expert.
-template <bool UP, int ROWS, int G>
-__device__ __forceinline__ bool run_item(const FewArgs& a, const Table& tb, Stream<UP, ROWS>& sm, int ai, int i,
-                                         uint32_t& it, volatile int* abort_flag) {
-  const int lane = threadIdx.x & 31, n = a.k * a.T, K = UP ? a.H : a.F, N = UP ? a.F : a.H;
-  const int nb = (K + kQB - 1) / kQB, nbn = (N + kQB - 1) / kQB;
-  const int e = tb.expert[ai], c0 = tb.start[ai], c = tb.start[ai + 1] - c0;
-  const int* rows = (UP ? tb.tokens : tb.slots) + c0;  // of the token operand
-  const uint32_t ld = UP ? a.T : n;
-  const uint8_t* xp[G];
-  const float* sp[G][2];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const int t = g * 8 + (lane >> 2), u = g * 8 + (lane & 3) * 2;
-    xp[g] = t < c ? (UP ? a.xq : a.hq) + (int64_t)rows[t] * K + (lane & 3) * 16 : nullptr;
-    sp[g][0] = u < c ? (UP ? a.xs : a.hs) + rows[u] : nullptr;
-    sp[g][1] = u + 1 < c ? (UP ? a.xs : a.hs) + rows[u + 1] : nullptr;
-  }
-  const int64_t so = ((int64_t)e * nbn + i * (UP ? 8 : ROWS) / kQB) * nb;
-  const float* s0 = (UP ? a.s_gate : a.s_down) + so;
-  const float* s1 = (UP ? a.s_up : a.s_down) + so;
-  float acc[G][4] = {};
-  bool ok = true;
-#pragma unroll 1
-  for (int left = K; left > 0 && ok; left -= kChunkK, ++it) {
-    const uint32_t s = it % kStages, parity = (it / kStages) & 1u;
-    const uint8_t* st = sm.smem + s * kStageBytes;
-    if (left >= kChunkK)
-      stage_product<G, UP ? 16 : ROWS, true>(acc, st, xp, sp, ld, s0, s1, left, sm.bar + 8 * s, parity, ok, abort_flag,
-                                             a.err);
-    else
-      stage_product<G, UP ? 16 : ROWS, false>(acc, st, xp, sp, ld, s0, s1, left, sm.bar + 8 * s, parity, ok,
-                                              abort_flag, a.err);
-    __syncwarp();
-    if (lane == 0 && ok) sm.issue();
-    s0 += kChunkB;
-    s1 += kChunkB;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      if (xp[g] != nullptr) xp[g] += kChunkK;
-      if (sp[g][0] != nullptr) sp[g][0] += kChunkB * ld;
-      if (sp[g][1] != nullptr) sp[g][1] += kChunkB * ld;
-    }
-  }
-  if (!ok) return false;
-  if constexpr (UP) {
-    // h of 8 columns: column lane / 4, this lane's two tokens of each group
-    const int f = i * 8 + (lane >> 2), fb = i * 8 / kQB;
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int t = g * 8 + (lane & 3) * 2 + j;
-        if (t < c) a.h[(int64_t)tb.slots[c0 + t] * a.F + f] = acc[g][j] * silu_ref(acc[g][2 + j]);
-      }
-    __threadfence();
-    __syncwarp();
-    int old = 0;
-    if (lane == 0) old = atomicAdd(a.count + (int64_t)e * nbn + fb, 1);
-    old = __shfl_sync(0xffffffffu, old, 0);
-    if (old == min(kQB / 8, sm.per - fb * (kQB / 8)) - 1) {
-      // the block's last item: its 128 values of every slot, four a lane
-      __threadfence();
-      const int fq = fb * kQB + lane * 4;
-#pragma unroll 4
-      for (int t = 0; t < c; ++t) {
-        const int slot = tb.slots[c0 + t];
-        float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (fq < a.F) q = __ldcg(reinterpret_cast<const float4*>(a.h + (int64_t)slot * a.F + fq));
-        const BlockScale sc = block_scale(__reduce_max_sync(
-            0xffffffffu, max(max(abs_bits(q.x), abs_bits(q.y)), max(abs_bits(q.z), abs_bits(q.w)))));
-        if (fq < a.F)
-          *reinterpret_cast<uint32_t*>(a.hq + (int64_t)slot * a.F + fq) =
-              e4m3x4(q.x * sc.inv, q.y * sc.inv, q.z * sc.inv, q.w * sc.inv);
-        if (lane == 0) a.hs[(int64_t)fb * n + slot] = sc.scale;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int t = g * 8 + (lane & 3) * 2 + j;
-        if (t < c) {
-          const int slot = tb.slots[c0 + t];
-          const float w = a.w[slot];
-          float* d = a.d + (int64_t)slot * a.H + i * ROWS + (lane >> 2);
-          d[0] = acc[g][j] * w;
-          if (ROWS == 16) d[8] = acc[g][2 + j] * w;
-        }
-      }
-  }
-  return true;
-}
-
-template <bool UP, int ROWS>
+template <bool UP>
 __global__ void __launch_bounds__(kFewThreads, 1)
-few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ FewArgs a) {
+few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ FewArgs a, int stages,
+                   uint32_t stage_bytes) {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* hbuf = reinterpret_cast<float*>(smem + stages * stage_bytes);  // UP: [tokens][128]
   __shared__ Table tb;
-  __shared__ int sid[kFewMaxSlots], sums[kWarps];
-  __shared__ uint64_t bars[kWarps * kStages];
+  __shared__ int sid[kFewMaxSlots], sums[kFewThreads / 32];
+  __shared__ uint64_t bars[2 * kMaxStages + 2 * kBufs + 1];
+  __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t bar0 = smem_u32(bars);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
+  auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * kMaxStages + b); };
+  auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * kMaxStages + kBufs + b); };
+  const uint32_t tile_bar = bar0 + 8u * (2 * kMaxStages + 2 * kBufs);
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kWarps * kStages; ++i) mbar_init(smem_u32(&bars[i]), 1);
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < kBufs; ++b) {
+      mbar_init(tfull_bar(b), 1);
+      mbar_init(tempty_bar(b), 4);
+    }
+    mbar_init(tile_bar, 4);
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
   }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   pdl_wait();
   pdl_launch();
-  build_table(a, tb, sid, sums);  // and the barriers are initialised
+  build_table(a, tb, sid, sums);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
 
-  // F and H are multiples of 16: no item is short
-  const int K = UP ? a.H : a.F, N = UP ? a.F : a.H;
-  Stream<UP, ROWS> sm;
-  sm.maps = &maps;
-  sm.tb = &tb;
-  sm.smem = smem + warp * kStages * kStageBytes;
-  sm.bar = smem_u32(&bars[warp * kStages]);
-  sm.per = N / (UP ? 8 : ROWS);
-  sm.items = tb.nact * sm.per;
-  sm.chunks = (K + kChunkK - 1) / kChunkK;
-  sm.step = gridDim.x * kWarps;
-  sm.next = blockIdx.x + gridDim.x * warp;  // neighbouring items on different SMs
-  sm.chunk = 0;
-  sm.issued = 0;
-  const int first = sm.next;
-  if (lane == 0)
-    for (int s = 0; s < kStages; ++s) sm.issue();
-  uint32_t it = 0;
-  bool ok = true;
-  for (int item = first; item < sm.items && ok; item += sm.step) {
-    const int ai = item / sm.per, i = item - ai * sm.per, c = tb.start[ai + 1] - tb.start[ai];
-    if (c <= 8) ok = run_item<UP, ROWS, 1>(a, tb, sm, ai, i, it, abort_flag);
-    else if (c <= 16) ok = run_item<UP, ROWS, 2>(a, tb, sm, ai, i, it, abort_flag);
-    else if (c <= 32) ok = run_item<UP, ROWS, 4>(a, tb, sm, ai, i, it, abort_flag);
-    else ok = run_item<UP, ROWS, 8>(a, tb, sm, ai, i, it, abort_flag);
+  const int K = UP ? a.H : a.F, N = UP ? a.F : a.H, n = a.k * a.T;
+  const int nb = (K + kQB - 1) / kQB, tiles = (N + kQB - 1) / kQB, parts = UP ? 1 : a.parts;
+  const int units = tb.entries * tiles * parts;
+  // columns of a unit: all tokens, or the expert's slots, to a multiple of 16
+  auto columns = [&](const Unit& t) { return UP ? (a.T + 15) & ~15 : (tb.first[t.ai + 1] - tb.first[t.ai] + 15) & ~15; };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------------------------ TMA producer --
+      uint64_t policy;
+      asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+      uint32_t it = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const Unit t = unit_at(a, u, tiles, parts, nb);
+        const int e = tb.expert[t.ai], cols = columns(t), box = cols <= 16 ? 0 : cols <= 32 ? 1 : 2;
+        const uint32_t x_bytes = (16u << box) * kQB;
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+          const int s = it % stages;
+          if (!mbar_wait_inline(empty_bar(s), ((it / stages) & 1u) ^ 1u, abort_flag, a.err)) {
+            ok = false;
+            break;
+          }
+          const uint32_t st = smem_u32(smem + s * stage_bytes);
+          mbar_expect_tx(full_bar(s), (UP ? 2 : 1) * kTile + x_bytes);
+          load_weights(st, &maps.w, kb * kQB, t.n * 128, e, full_bar(s), policy);
+          if (UP) load_weights(st + kTile, &maps.w2, kb * kQB, t.n * 128, e, full_bar(s), policy);
+          load_2d(st + (UP ? 2 : 1) * kTile, &maps.x[box], kb * kQB, UP ? 0 : tb.row[t.ai], full_bar(s));
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // -------------------------------------------------- MMA issuer --
+      uint32_t it = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const Unit t = unit_at(a, u, tiles, parts, nb);
+        // kind::f8f6f4: D fp32, A and B e4m3, N >> 3 at [17,23), M >> 4 at [24,29)
+        const uint32_t idesc = (1u << 4) | ((uint32_t)(columns(t) >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+          const int s = it % stages, b = it % kBufs;
+          if (!mbar_wait_inline(tempty_bar(b), ((it / kBufs) & 1u) ^ 1u, abort_flag, a.err) ||
+              !mbar_wait_inline(full_bar(s), (it / stages) & 1u, abort_flag, a.err)) {
+            ok = false;
+            break;
+          }
+          fence_after();
+          const uint32_t st = smem_u32(smem + s * stage_bytes);
+          const uint64_t wd = smem_desc(st), w2d = smem_desc(st + kTile), xd = smem_desc(st + (UP ? 2 : 1) * kTile);
+#pragma unroll
+          for (int j = 0; j < kQB / 32; ++j) {  // 32 bytes along K inside the swizzled row
+            mma(tmem + b * kBufCols, wd + (uint64_t)(2 * j), xd + (uint64_t)(2 * j), idesc, j != 0);
+            if (UP) mma(tmem + b * kBufCols + 64, w2d + (uint64_t)(2 * j), xd + (uint64_t)(2 * j), idesc, j != 0);
+          }
+          commit(empty_bar(s));
+          commit(tfull_bar(b));
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------------------------------------------- epilogue --
+    const int quad = warp & 3, row = quad * 32 + lane;  // this thread's weight row of the tile
+    const uint32_t my_tmem = tmem + ((uint32_t)(quad * 32) << 16);
+    uint32_t it = 0, meets = 0;
+    bool ok = true;
+    // the four warps of the epilogue meet (bounded, unlike a named barrier)
+    auto meet = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tile_bar);
+      if (!mbar_wait_inline(tile_bar, meets++ & 1u, abort_flag, a.err)) ok = false;
+    };
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      const Unit t = unit_at(a, u, tiles, parts, nb);
+      const int e = tb.expert[t.ai], f = tb.first[t.ai], c = tb.first[t.ai + 1] - f, cols = columns(t);
+      uint32_t need = 0;  // groups of 16 columns that are used
+      for (int i = 0; i < c; ++i) need |= 1u << (UP ? tb.slots[f + i] % a.T / 16 : i / 16);
+      const int64_t so = ((int64_t)e * tiles + t.n) * nb;
+      const float* s0 = (UP ? a.s_gate : a.s_down) + so;
+      const float* s1 = UP ? a.s_up + so : s0;
+      const float* xs = UP ? a.xs : a.hs + tb.row[t.ai];
+      const int ld = UP ? kFewMaxT : a.h_rows;
+      float acc[UP ? 2 : 1][4][16] = {};
+#pragma unroll 1
+      for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+        const int b = it % kBufs;
+        const float w0 = __ldg(s0 + kb), w1 = UP ? __ldg(s1 + kb) : 0.f;
+        float4 sc[4];
+        const float* xk = xs + (int64_t)kb * ld;
+        if (need & 1u) {  // the first group's scales before the wait
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[i] = *reinterpret_cast<const float4*>(xk + 4 * i);
+        }
+        if (!mbar_wait_inline(tfull_bar(b), (it / kBufs) & 1u, abort_flag, a.err)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (need >> g & 1u) {
+            if (g > 0) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sc[i] = *reinterpret_cast<const float4*>(xk + g * 16 + 4 * i);
+            }
+            uint32_t v[UP ? 2 : 1][16];
+            tmem_ld16(my_tmem + b * kBufCols + g * 16, v[0]);
+            if constexpr (UP) tmem_ld16(my_tmem + b * kBufCols + 64 + g * 16, v[UP ? 1 : 0]);
+            tmem_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float* s4 = reinterpret_cast<const float*>(&sc[i >> 2]);
+              acc[0][g][i] = fmaf(__uint_as_float(v[0][i]), s4[i & 3] * w0, acc[0][g][i]);
+              if constexpr (UP)
+                acc[UP ? 1 : 0][g][i] = fmaf(__uint_as_float(v[UP ? 1 : 0][i]), s4[i & 3] * w1, acc[UP ? 1 : 0][g][i]);
+            }
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty_bar(b));
+      }
+      if (!ok) break;
+      if constexpr (UP) {
+        // h to shared memory, then one warp a slot: its 128 values share a scale
+        const bool in = t.n * 128 + row < a.F;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (need >> g & 1u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (g * 16 + i < cols)
+                hbuf[(g * 16 + i) * 128 + row] = in ? acc[0][g][i] * silu_ref(acc[UP ? 1 : 0][g][i]) : 0.f;
+          }
+        meet();
+        if (!ok) break;
+        const int col = t.n * 128 + lane * 4;
+        for (int i = quad; i < c; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(hbuf + tb.slots[f + i] % a.T * 128 + lane * 4);
+          const BlockScale s = block_scale(__reduce_max_sync(
+              0xffffffffu, max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)))));
+          const int64_t r = tb.row[t.ai] + i;
+          if (col < a.F)
+            *reinterpret_cast<uint32_t*>(a.hq + r * a.F + col) =
+                e4m3x4(v.x * s.inv, v.y * s.inv, v.z * s.inv, v.w * s.inv);
+          if (lane == 0) a.hs[(int64_t)t.n * a.h_rows + r] = s.scale;
+        }
+        meet();  // before the next tile's values
+      } else if (t.n * 128 + row < a.H) {
+        float* d = a.d + ((int64_t)t.part * n) * a.H + t.n * 128 + row;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (g * 16 + i < c) {
+              const int slot = tb.slots[f + g * 16 + i];
+              d[(int64_t)slot * a.H] = acc[0][g][i] * a.w[slot];
+            }
+      }
+    }
   }
-  if (!ok) {  // no copy may land after this CTA is gone; these waits are bounded too
-    abort_word = 0;
-    const uint32_t issued = __shfl_sync(0xffffffffu, sm.issued, 0);
-    for (uint32_t s = it; s < issued; ++s)
-      mbar_wait(sm.bar + 8 * (s % kStages), (s / kStages) & 1u, abort_flag, a.err);
+  fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
 }
 
@@ -571,8 +598,8 @@ int launch_few_route(const FewRoute& a, cudaStream_t st) {
   return FRANK_OK;
 }
 
-// Map of e4m3 [E, N, K] as 8-byte elements, box 512 bytes x rows.
-static int few_map(CUtensorMap* m, const void* base, int64_t E, int64_t N, int64_t K, uint32_t rows) {
+// Map of bytes [E, R, K] (or [R, K]), box 128 bytes x rows, 128-byte swizzle.
+static int few_map(CUtensorMap* m, const void* base, int64_t E, int64_t R, int64_t K, uint32_t rows, bool three) {
   static PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -585,47 +612,72 @@ static int few_map(CUtensorMap* m, const void* base, int64_t E, int64_t N, int64
     set_error("cuTensorMapEncodeTiled unavailable");
     return FRANK_ECUDA;
   }
-  const cuuint64_t dims[3] = {(cuuint64_t)K / 8, (cuuint64_t)N, (cuuint64_t)E};
-  const cuuint64_t strides[2] = {(cuuint64_t)K, (cuuint64_t)(N * K)};
-  const cuuint32_t box[3] = {kChunkK / 8, rows, 1}, estr[3] = {1, 1, 1};
-  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_INT64, 3, const_cast<void*>(base), dims, strides, box, estr,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)R, (cuuint64_t)E};
+  const cuuint64_t strides[2] = {(cuuint64_t)K, (cuuint64_t)(R * K)};
+  const cuuint32_t box[3] = {kQB, rows, 1}, estr[3] = {1, 1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, three ? 3 : 2, const_cast<void*>(base), dims, strides, box,
+                         estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
-    set_error("cuTensorMapEncodeTiled([%lld, %lld, %lld] bytes) failed: %d", (long long)E, (long long)N, (long long)K,
+    set_error("cuTensorMapEncodeTiled([%lld, %lld, %lld] bytes) failed: %d", (long long)E, (long long)R, (long long)K,
               (int)r);
     return FRANK_ECUDA;
   }
   return FRANK_OK;
 }
 
-template <bool UP, int ROWS>
+// 227 KB an SM less the static tables; the rest is the ring and UP's values of h.
+constexpr size_t kFewSmem = 232448 - 12288;
+
+template <bool UP>
 static int launch_few_product(const FewMaps& maps, const FewArgs& a, cudaStream_t st) {
-  const size_t smem = 128 + (size_t)kWarps * kStages * kStageBytes;
-  FRANK_CUDA_TRY(
-      cudaFuncSetAttribute(few_product_kernel<UP, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  FRANK_CUDA_TRY(
-      launch_chained(few_product_kernel<UP, ROWS>, dim3(num_sms()), dim3(kFewThreads), smem, st, 1, maps, a));
+  const int cols = (a.T + 15) & ~15, box = tile_tokens(a.T);
+  const uint32_t stage = (UP ? 2 : 1) * kTile + box * kQB;
+  const size_t hbuf = UP ? (size_t)cols * 128 * 4 : 0;
+  const int fit = (int)((kFewSmem - 1024 - hbuf) / stage), stages = fit < kMaxStages ? fit : kMaxStages;
+  FRANK_CUDA_TRY(cudaFuncSetAttribute(few_product_kernel<UP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)kFewSmem));
+  FRANK_CUDA_TRY(launch_chained(few_product_kernel<UP>, dim3(num_sms()), dim3(kFewThreads),
+                                1024 + hbuf + (size_t)stages * stage, st, 1, maps, a, stages, stage));
   FRANK_LAUNCH_CHECK();
   return FRANK_OK;
+}
+
+// The combine adds `parts` partial sums a slot: where the tiles of H alone cannot
+// keep the SMs busy, F is divided, into parts of 8 K blocks or more.
+int few_parts(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
+  const int64_t tiles = (k * T < E ? k * T : E) * q_blocks(H), most = q_blocks(F) / 8;
+  if (tiles <= 0) return 1;
+  const int64_t want = (4 * num_sms() + tiles - 1) / tiles;
+  const int64_t parts = want < most ? want : most;
+  return (int)(parts < 1 ? 1 : parts > kFewMaxParts ? kFewMaxParts : parts);
+}
+
+int64_t few_h_rows(int64_t T, int64_t E, int64_t k) {
+  const int64_t n = k * T;  // up to 15 rows of padding for each expert that has slots
+  return (n + 15 * (n < E ? n : E) + 15) / 16 * 16;
 }
 
 int launch_few_experts(const FewArgs& args, int32_t* err, cudaStream_t st) {
   FewArgs a = args;
   a.err = device_error_word();
+  a.parts = few_parts(a.T, a.E, a.k, a.H, a.F);
+  a.h_rows = (int)few_h_rows(a.T, a.E, a.k);
   if (err != nullptr) {
     FRANK_CUDA_TRY(launch_chained(few_check_ids_kernel, dim3(1), dim3(256), 0, st, 1, a.ids, a.k * a.T, a.E, err));
     FRANK_LAUNCH_CHECK();
   }
   FewMaps up, down;
-  FRANK_TRY(few_map(&up.a, a.w_gate, a.E, a.F, a.H, 8));
-  FRANK_TRY(few_map(&up.b, a.w_up, a.E, a.F, a.H, 8));
-  FRANK_TRY((launch_few_product<true, 16>(up, a, st)));
-  // An item of 16 rows of 4096 values or more holds an SM's last warp too long: 8 rows then.
-  const bool wide = a.F < 4096;
-  FRANK_TRY(few_map(&down.a, a.w_down, a.E, a.H, a.F, wide ? 16 : 8));
-  down.b = down.a;
-  return wide ? launch_few_product<false, 16>(down, a, st) : launch_few_product<false, 8>(down, a, st);
+  FRANK_TRY(few_map(&up.w, a.w_gate, a.E, a.F, a.H, 128, true));
+  FRANK_TRY(few_map(&up.w2, a.w_up, a.E, a.F, a.H, 128, true));
+  FRANK_TRY(few_map(&down.w, a.w_down, a.E, a.H, a.F, 128, true));
+  down.w2 = down.w;
+  for (int i = 0; i < 3; ++i) {
+    FRANK_TRY(few_map(&up.x[i], a.xq, 1, a.T, a.H, 16u << i, false));
+    FRANK_TRY(few_map(&down.x[i], a.hq, 1, a.h_rows, a.F, 16u << i, false));
+  }
+  FRANK_TRY(launch_few_product<true>(up, a, st));
+  return launch_few_product<false>(down, a, st);
 }
 
 }  // namespace frank

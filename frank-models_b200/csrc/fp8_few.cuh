@@ -7,7 +7,7 @@ namespace frank {
 
 constexpr int kFewMaxE = (int)kFp8MaxE;
 constexpr int kFewMaxT = 64, kFewMaxSlots = 512;
-constexpr int64_t kFewMaxCounts = 1 << 16;  // E * ceil(F/128)
+constexpr int kFewMaxParts = 4;
 
 struct FewRoute {
   const void* x;  // [T, H]
@@ -18,11 +18,9 @@ struct FewRoute {
   int wr_dtype;
   int T, H, E, k, normalize;
   uint8_t* xq;   // [T, H]
-  float* xs;     // [ceil(H/128), T]
+  float* xs;     // [ceil(H/128), kFewMaxT]
   float* w;      // [k, T]
   int32_t* ids;  // [k, T]
-  int32_t* count;  // [E, ceil(F/128)], zeroed
-  int n_count;
 };
 
 struct FewArgs {
@@ -30,17 +28,18 @@ struct FewArgs {
   const float *s_up, *s_gate, *s_down;
   const uint8_t* xq;  // [T, H]
   const float* xs;
-  int32_t* count;  // items of a block of h that are done
-  float* h;        // [k T, F]
-  uint8_t* hq;     // [k T, F]
-  float* hs;    // [ceil(F/128), k T]
-  float* d;     // [k T, H]
+  uint8_t* hq;  // [few_h_rows, F], the slots sorted by expert, each expert at a multiple of 16
+  float* hs;    // [ceil(F/128), few_h_rows]
+  float* d;     // [few_parts, k T, H]
   const float* w;
   const int32_t* ids;
   int T, E, k, H, F;
-  int32_t* err;  // device error word
+  int parts, h_rows;  // set by launch_few_experts
+  int32_t* err;       // device error word
 };
 
+int few_parts(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F);
+int64_t few_h_rows(int64_t T, int64_t E, int64_t k);
 int launch_few_route(const FewRoute& a, cudaStream_t st);
 int launch_few_experts(const FewArgs& a, int32_t* err, cudaStream_t st);
 

@@ -70,7 +70,7 @@ __device__ __forceinline__ float inv_rms(const float4 (&v)[V], int64_t H, float 
   return 1.f / sqrtf(row_sum<GS>(ss, red) / (float)H + eps);
 }
 
-template <int GS, int V>
+template <int GS, int V, bool SLOTS>
 __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormRows a) {
   __shared__ float red[2][kThreads / 32];
   const int tid = threadIdx.x % GS;
@@ -84,23 +84,39 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormRows a) {
   for (int i = 0; i < V; ++i) {
     const int64_t h = 4 * (int64_t)(tid + i * GS);
     v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (h < H && a.d == nullptr) v[i] = load4(a.y, a.y_dtype, t * H + h);
+    if (!SLOTS && h < H) v[i] = load4(a.y, a.y_dtype, t * H + h);
   }
-  if (a.d != nullptr) {
-    for (int j = 0; j < a.k; ++j) {
-      const int64_t s = (int64_t)j * a.T + t;
-      const float* row = a.d + (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * H;
+  if (SLOTS) {
+    // rows in order, the loads of several at a time
+    constexpr int kAhead = V <= 2 ? 4 : V <= 4 ? 2 : 1;
+    const int rows = a.k * a.parts;
+    for (int j0 = 0; j0 < rows; j0 += kAhead) {
+      float4 u[kAhead][V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int64_t h = 4 * (int64_t)(tid + i * GS);
-        if (h < H) {
-          const float4 u = *reinterpret_cast<const float4*>(row + h);
-          v[i].x += u.x;
-          v[i].y += u.y;
-          v[i].z += u.z;
-          v[i].w += u.w;
+      for (int q = 0; q < kAhead; ++q) {
+        const int j = (j0 + q) / a.parts, part = j0 + q - j * a.parts;
+        const int64_t s = (int64_t)j * a.T + t;
+        const float* row = a.d;
+        if (j0 + q < rows)
+          row += ((int64_t)part * a.k * a.T + (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s)) * H;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int64_t h = 4 * (int64_t)(tid + i * GS);
+          u[q][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (h < H && j0 + q < rows) u[q][i] = *reinterpret_cast<const float4*>(row + h);
         }
       }
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q)
+        if (j0 + q < rows) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            v[i].x += u[q][i].x;
+            v[i].y += u[q][i].y;
+            v[i].z += u[q][i].z;
+            v[i].w += u[q][i].w;
+          }
+        }
     }
   }
   float r = 1.f;
@@ -164,7 +180,9 @@ int launch_norm_rows(const NormRows& a, cudaStream_t st) {
   const int64_t per = warp_rows ? kThreads / 32 : 1;
   const dim3 grid((unsigned)((a.T + per - 1) / per)), block(kThreads);
   cudaError_t e;
-#define FRANK_NORM(GS, V) e = launch_chained(norm_rows_kernel<GS, V>, grid, block, 0, st, 1, a)
+#define FRANK_NORM(GS, V)                                                                      \
+  e = a.d != nullptr ? launch_chained(norm_rows_kernel<GS, V, true>, grid, block, 0, st, 1, a) \
+                     : launch_chained(norm_rows_kernel<GS, V, false>, grid, block, 0, st, 1, a)
   if (warp_rows) {
     if (vec <= 1) FRANK_NORM(32, 1);
     else if (vec <= 2) FRANK_NORM(32, 2);

@@ -94,6 +94,13 @@ def test_library_accepts_nothing_to_do(lib):
     assert lib.frank_fp8_moe_experts(*[None] * 9, 0, 8, 2, 128, 128, 0, None, None, None, 0, None) == 0
 
 
+def test_workspace_size_of_anything(lib):
+    """A size query is host arithmetic: it answers for no tokens, no experts and nonsense alike."""
+    assert lib.frank_fp8_moe_workspace_size(1, 2048, 768, 128, 8) > 8 * 2048 * 4
+    for shape in ((0, 128, 128, 8, 2), (4, 0, 0, 8, 2), (4, 128, 128, 0, 0), (4, 128, 128, 8, 0), (-1, 128, 128, 8, 2)):
+        lib.frank_fp8_moe_workspace_size(*shape)
+
+
 def test_python_refusals():
     import frank_b200 as fb
 

@@ -454,3 +454,14 @@ def test_layer_from_params():
     assert torch.equal(layer(x), b(x))
     res = randn(gen(15), 5, H)
     assert torch.equal(layer.sublayer(res, 1e-5), b.sublayer(res, dev["blk.0.ffn_norm.weight"], 1e-5))
+
+
+def test_experts_the_same_id_twice():
+    """A token that names an expert twice gets it twice, however many slots the expert has."""
+    g = gen(16)
+    for T, k, E in ((10, 8, 9), (64, 8, 8), (3, 2, 2), (200, 3, 4)):
+        b = block(g, T, 256, 144, E, k, out_dtype=F32)
+        x = randn(g, T, 256, dtype=BF16)
+        rid = torch.randint(0, 2, (k, T), generator=g, device=DEV, dtype=torch.int32)
+        rw = torch.rand((k, T), generator=g, device=DEV)
+        within(b.experts(x, rw, rid), *want_moe(b, x, rw, rid))
