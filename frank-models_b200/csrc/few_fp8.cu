@@ -49,12 +49,6 @@ __device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
 __device__ __forceinline__ void st_peer(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
-__device__ __forceinline__ float ld_peer(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 __device__ __forceinline__ float4 load4(const void* p, int dtype, int64_t i) {
   if (dtype == FRANK_F32) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
   const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + i));
@@ -65,9 +59,11 @@ __device__ __forceinline__ float4 load4(const void* p, int dtype, int64_t i) {
 // -------------------------------------------------------------- route --
 constexpr int kRouteCtas = 8, kRouteTok = 8, kRouteThreads = 512;
 
+// PER: experts a lane of the top-k, E <= 32 PER
+template <int PER>
 __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute a) {
   extern __shared__ float xs[];  // [8 tokens][slice]
-  __shared__ float part[kFewMaxE][kRouteTok];
+  __shared__ float part[kRouteCtas][kFewMaxE];  // of this CTA's token, from every slice
   __shared__ float ssq_block[kRouteTok][16], ssq[kRouteCtas][kRouteTok];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kWarps = kRouteThreads / 32;
@@ -84,9 +80,24 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
   }
   const int nb = (a.H + kQB - 1) / kQB, sb = (nb + kRouteCtas - 1) / kRouteCtas;  // blocks of a row, of a slice
   const int slice = sb * kQB, h0 = (int)rank * slice;
+  // A warp's router weights: four experts, one block of columns a step, loaded two steps
+  // ahead; the first two before the stream's last kernel is done.
+  const int steps = ((a.E + 4 * kWarps - 1) / (4 * kWarps)) * sb;
+  auto router = [&](int q, float4 (&w)[4]) {
+    const int e0 = (q / sb * kWarps + warp) * 4, c = h0 + q % sb * kQB + lane * 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (q < steps && e0 + j < a.E && c < a.H) w[j] = load4(a.wr, a.wr_dtype, (int64_t)(e0 + j) * a.H + c);
+    }
+  };
+  float4 w0[4], w1[4];
+  if (a.wr != nullptr) router(0, w0), router(1, w1);
   pdl_wait();
   pdl_launch();
   cluster_arrive();  // every CTA has started before its memory is written
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < a.n_count; i += kRouteThreads) a.count[i] = 0;
   // one (token, block) a warp: a vector of 4 for each lane
   for (int i = warp; i < kRouteTok * sb; i += kWarps) {
     const int t = i / sb, b = i % sb, h = h0 + b * kQB + lane * 4;
@@ -138,31 +149,22 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
   }
   if (a.wr == nullptr) return;  // the routing is given
   __syncthreads();
-  // partial logits of this slice: four experts a warp, 8 tokens each
-  for (int e0 = warp * 4; e0 < a.E; e0 += kWarps * 4) {
-    float acc[32];
+  // partial logits of this slice: four experts a warp, 8 tokens each; the sums go to the token's CTA
+  float acc[32] = {};
+  auto step = [&](int q, const float4 (&w)[4]) {
+    if (q >= steps) return;
+    const int b = q % sb;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-#pragma unroll 2
-    for (int b = 0; b < sb; ++b) {
-      const int c = b * kQB + lane * 4;
-      float4 w[4];
+    for (int t = 0; t < kRouteTok; ++t) {
+      if (t < nt) {
+        const float4 v = *reinterpret_cast<const float4*>(xs + t * slice + b * kQB + lane * 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (e0 + j < a.E && h0 + c < a.H) w[j] = load4(a.wr, a.wr_dtype, (int64_t)(e0 + j) * a.H + h0 + c);
-      }
-#pragma unroll
-      for (int t = 0; t < kRouteTok; ++t) {
-        if (t < nt) {
-          const float4 v = *reinterpret_cast<const float4*>(xs + t * slice + c);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[j * 8 + t] =
-                fmaf(v.w, w[j].w, fmaf(v.z, w[j].z, fmaf(v.y, w[j].y, fmaf(v.x, w[j].x, acc[j * 8 + t]))));
-        }
+        for (int j = 0; j < 4; ++j)
+          acc[j * 8 + t] =
+              fmaf(v.w, w[j].w, fmaf(v.z, w[j].z, fmaf(v.y, w[j].y, fmaf(v.x, w[j].x, acc[j * 8 + t]))));
       }
     }
+    if (b < sb - 1) return;
     // 32 sums over 32 lanes: each step halves the values a lane still carries; lane l ends with sum l
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -174,22 +176,31 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
         acc[i] = (up ? acc[i + o] : acc[i]) + got;
       }
     }
-    if (e0 + (lane >> 3) < a.E) part[e0 + (lane >> 3)][lane & 7] = acc[0];
+    const int e = (q / sb * kWarps + warp) * 4 + (lane >> 3), t = lane & 7;
+    if (e < a.E && t < nt) st_peer(peer_addr(&part[rank][e], (uint32_t)t), __float_as_uint(acc[0]));
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+  };
+#pragma unroll 1
+  for (int q = 0; q < steps; q += 2) {
+    step(q, w0);
+    router(q + 2, w0);
+    step(q + 1, w1);
+    router(q + 3, w1);
   }
   cluster_sync();
   // softmax and top-k of token `rank`, one warp; ties go to the lowest index
   if (warp == 0 && (int)rank < nt) {
-    constexpr int kPer = kFewMaxE / 32;
-    float p[kPer];
+    float p[PER];
     float mx = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < PER; ++i) {
       const int e = lane + 32 * i;
       p[i] = -INFINITY;
       if (e < a.E) {
         float s = 0.f;
 #pragma unroll
-        for (int r = 0; r < kRouteCtas; ++r) s += ld_peer(peer_addr(&part[e][rank], (uint32_t)r));
+        for (int r = 0; r < kRouteCtas; ++r) s += part[r][e];
         p[i] = s;
       }
       mx = fmaxf(mx, p[i]);
@@ -197,7 +208,7 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < PER; ++i) {
       p[i] = lane + 32 * i < a.E ? expf(p[i] - mx) : 0.f;
       sum += p[i];
     }
@@ -206,10 +217,11 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
     // order by bits + 1 (probabilities are >= 0), 0 for no expert; a token whose logits are no numbers takes
     // experts 0 .. k-1 with weights that are none either
     const bool bad = !(sum < INFINITY);
-    uint32_t key[kPer];
+    const float inv = 1.f / sum;
+    uint32_t key[PER];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      p[i] = p[i] / sum;
+    for (int i = 0; i < PER; ++i) {
+      p[i] *= inv;
       key[i] = lane + 32 * i < a.E ? (bad ? 1u : __float_as_uint(p[i]) + 1u) : 0u;
     }
     float mine = 0.f, wsum = 0.f;  // lane j: the weight of choice j
@@ -217,15 +229,15 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
     for (int j = 0; j < a.k; ++j) {
       uint32_t best = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
+      for (int i = 0; i < PER; ++i) best = max(best, key[i]);
       best = __reduce_max_sync(0xffffffffu, best);
       uint32_t id = 0xffffffffu;
 #pragma unroll
-      for (int i = kPer - 1; i >= 0; --i)
+      for (int i = PER - 1; i >= 0; --i)
         if (key[i] == best) id = lane + 32 * i;
       id = __reduce_min_sync(0xffffffffu, id);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
+      for (int i = 0; i < PER; ++i)
         if (lane + 32 * i == (int)id) key[i] = 0u;
       const float v = bad ? __uint_as_float(0x7fc00000u) : __uint_as_float(best - 1u);
       wsum += v;
@@ -237,13 +249,12 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
       a.ids[s] = my_id;
     }
   }
-  cluster_sync();  // the others' sums stay until they are read
 }
 
 // ------------------------------------------------------------- products --
-constexpr int kFewThreads = 256;  // warp 0: TMA, warp 1: MMA, warps 4..7: epilogue
+constexpr int kFewThreads = 256;  // warp 0: TMA, warp 1: MMA, warp 2: scales, warps 4..7: epilogue
 constexpr uint32_t kTile = 128 * kQB;  // bytes of 128 weight rows of a K block
-constexpr int kMaxStages = 12, kBufs = 4, kBufCols = 128;
+constexpr int kMaxStages = 12, kBufs = 4, kBufCols = 128, kScaleSlots = 8;
 constexpr uint32_t kTmemCols = kBufs * kBufCols;
 
 struct FewMaps {
@@ -264,15 +275,38 @@ struct Table {
   int first[kMaxEntries + 1];  // of its slots
   int row[kMaxEntries];        // of h
   int slots[kFewMaxSlots];
+  int tokens[kFewMaxSlots];    // of the slots
 };
 
-__device__ __forceinline__ void build_table(const FewArgs& a, Table& tb, int* sid, int* sums) {
+// A stable counting sort of the slots: ranks inside 32 slots by a warp match, one thread
+// an expert adds up the chunks.  at: scratch [kFewMaxSlots / 32][kFewMaxE].
+__device__ __forceinline__ void build_table(const FewArgs& a, Table& tb, uint16_t (*at)[kFewMaxE], int* sums) {
   const int n = a.k * a.T, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  static_assert(kFewThreads == kFewMaxE, "a thread counts an expert");
-  for (int s = tid; s < n; s += kFewThreads) sid[s] = min(max(a.ids[s], 0), a.E - 1);
+  constexpr int kWarps = kFewThreads / 32, kChunks = kFewMaxSlots / 32;
+  static_assert(kFewThreads == kFewMaxE && kChunks == 2 * kWarps, "a thread an expert, two chunks a warp");
+  const int chunks = (n + 31) / 32;
+  int id[2], rank[2], size[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int s = (warp + i * kWarps) * 32 + lane;
+    id[i] = s < n ? min(max(__ldcg(a.ids + s), 0), a.E - 1) : -1;
+  }
+  for (int c = 0; c < chunks; ++c) at[c][tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t m = __match_any_sync(0xffffffffu, id[i]);
+    rank[i] = __popc(m & ((1u << lane) - 1u));
+    size[i] = __popc(m);
+    if (id[i] >= 0 && rank[i] == 0) at[warp + i * kWarps][id[i]] = (uint16_t)size[i];
+  }
   __syncthreads();
   int c = 0;
-  for (int s = 0; s < n; ++s) c += sid[s] == tid;
+  for (int i = 0; i < chunks; ++i) {
+    const int t = at[i][tid];
+    at[i][tid] = (uint16_t)c;
+    c += t;
+  }
   // before this expert: slots (bits 0..9), entries (10..18) and groups of 16 rows (19..)
   const int cap = tile_tokens(a.T), mine = c | (c + cap - 1) / cap << 10 | (c + 15) / 16 << 19;
   int v = mine;
@@ -284,21 +318,30 @@ __device__ __forceinline__ void build_table(const FewArgs& a, Table& tb, int* si
   if (lane == 31) sums[warp] = v;
   __syncthreads();
   int before = v - mine, total = 0;
-  for (int w = 0; w < kFewThreads / 32; ++w) {
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += sums[w];
     total += sums[w];
   }
-  int at = before & 1023;
+  const int first = before & 1023;
   for (int i = 0; i * cap < c; ++i) {
     const int entry = (before >> 10 & 511) + i;
     tb.expert[entry] = tid;
-    tb.first[entry] = at + i * cap;
+    tb.first[entry] = first + i * cap;
     tb.row[entry] = (before >> 19) * 16 + i * cap;
   }
   if (c != 0)
-    for (int s = 0; s < n; ++s)
-      if (sid[s] == tid) tb.slots[at++] = s;
+    for (int i = 0; i < chunks; ++i) at[i][tid] += (uint16_t)first;
   if (tid == 0) tb.entries = total >> 10 & 511, tb.first[total >> 10 & 511] = n;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (id[i] >= 0) {
+      const int s = (warp + i * kWarps) * 32 + lane, p = at[warp + i * kWarps][id[i]] + rank[i];
+      tb.slots[p] = s;
+      tb.tokens[p] = s % a.T;
+    }
+  }
 }
 
 __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -316,6 +359,11 @@ __device__ __forceinline__ void load_weights(uint32_t dst, const CUtensorMap* ma
       "%4}], [%5], %6;" ::"r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
       : "memory");
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -364,12 +412,13 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
                    uint32_t stage_bytes) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* hbuf = reinterpret_cast<float*>(smem + stages * stage_bytes);  // UP: [tokens][128]
+  float* hbuf = reinterpret_cast<float*>(smem + stages * stage_bytes);  // UP: [16][gate, up][128]
   __shared__ Table tb;
-  __shared__ int sid[kFewMaxSlots], sums[kFewThreads / 32];
-  __shared__ uint64_t bars[2 * kMaxStages + 2 * kBufs + 1];
+  __shared__ int sums[kFewThreads / 32];
+  __shared__ uint64_t bars[2 * kMaxStages + 2 * kBufs + 2 * kScaleSlots + 1];
+  __shared__ alignas(128) float scales[kScaleSlots][kFewMaxT];  // of the token operand, a slot for each K block
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word;
+  __shared__ int abort_word, last_word;
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t bar0 = smem_u32(bars);
@@ -377,7 +426,9 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
   auto empty_bar = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
   auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * kMaxStages + b); };
   auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * kMaxStages + kBufs + b); };
-  const uint32_t tile_bar = bar0 + 8u * (2 * kMaxStages + 2 * kBufs);
+  auto sfull_bar = [&](int i) { return bar0 + 8u * (2 * kMaxStages + 2 * kBufs + i); };
+  auto sempty_bar = [&](int i) { return bar0 + 8u * (2 * kMaxStages + 2 * kBufs + kScaleSlots + i); };
+  const uint32_t tile_bar = bar0 + 8u * (2 * kMaxStages + 2 * kBufs + 2 * kScaleSlots);
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(full_bar(s), 1);
@@ -386,6 +437,10 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
     for (int b = 0; b < kBufs; ++b) {
       mbar_init(tfull_bar(b), 1);
       mbar_init(tempty_bar(b), 4);
+    }
+    for (int i = 0; i < kScaleSlots; ++i) {
+      mbar_init(sfull_bar(i), 1);
+      mbar_init(sempty_bar(i), 4);
     }
     mbar_init(tile_bar, 4);
     abort_word = 0;
@@ -398,16 +453,19 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_wait();
+  // DOWN needs nothing of UP but h: UP started after the routing was complete, and this
+  // kernel after all of UP's CTAs had started, so the table and the first weights need no wait.
+  if (UP) pdl_wait();
   pdl_launch();
-  build_table(a, tb, sid, sums);
+  build_table(a, tb, reinterpret_cast<uint16_t(*)[kFewMaxE]>(smem), sums);
+  fence_proxy_async_smem();  // the scratch becomes the ring
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_slot;
 
   const int K = UP ? a.H : a.F, N = UP ? a.F : a.H, n = a.k * a.T;
-  const int nb = (K + kQB - 1) / kQB, tiles = (N + kQB - 1) / kQB, parts = UP ? 1 : a.parts;
+  const int nb = (K + kQB - 1) / kQB, tiles = (N + kQB - 1) / kQB, parts = UP ? a.up_parts : a.parts;
   const int units = tb.entries * tiles * parts;
   // columns of a unit: all tokens, or the expert's slots, to a multiple of 16
   auto columns = [&](const Unit& t) { return UP ? (a.T + 15) & ~15 : (tb.first[t.ai + 1] - tb.first[t.ai] + 15) & ~15; };
@@ -417,25 +475,46 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
       // ------------------------------------------------ TMA producer --
       uint64_t policy;
       asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-      uint32_t it = 0;
-      bool ok = true;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        const Unit t = unit_at(a, u, tiles, parts, nb);
-        const int e = tb.expert[t.ai], cols = columns(t), box = cols <= 16 ? 0 : cols <= 32 ? 1 : 2;
-        const uint32_t x_bytes = (16u << box) * kQB;
-        for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+      // The ring is filled with weights first; the token operand of a stage follows, at once
+      // or, for the first stages of DOWN, when h is there.
+      int u = blockIdx.x, kb = 0, fu = u, fkb = 0;  // next weights, next tokens
+      uint32_t it = 0, fit = 0;
+      bool ok = true, waited = UP;
+      Unit t, ft;
+      if (u < units) t = ft = unit_at(a, u, tiles, parts, nb), kb = fkb = t.kb0;
+      while (fu < units && ok) {
+        if (u < units && (waited ? it == fit : it < (uint32_t)stages)) {
           const int s = it % stages;
           if (!mbar_wait_inline(empty_bar(s), ((it / stages) & 1u) ^ 1u, abort_flag, a.err)) {
             ok = false;
             break;
           }
+          const int e = tb.expert[t.ai], cols = columns(t), box = cols <= 16 ? 0 : cols <= 32 ? 1 : 2;
           const uint32_t st = smem_u32(smem + s * stage_bytes);
-          mbar_expect_tx(full_bar(s), (UP ? 2 : 1) * kTile + x_bytes);
+          mbar_expect_tx(full_bar(s), (UP ? 2 : 1) * kTile + (16u << box) * kQB);
           load_weights(st, &maps.w, kb * kQB, t.n * 128, e, full_bar(s), policy);
           if (UP) load_weights(st + kTile, &maps.w2, kb * kQB, t.n * 128, e, full_bar(s), policy);
-          load_2d(st + (UP ? 2 : 1) * kTile, &maps.x[box], kb * kQB, UP ? 0 : tb.row[t.ai], full_bar(s));
+          ++it;
+          if (++kb == t.kb1) {
+            u += gridDim.x;
+            if (u < units) t = unit_at(a, u, tiles, parts, nb), kb = t.kb0;
+          }
+          if (!waited) continue;
+        }
+        if (!waited) {
+          pdl_wait();
+          waited = true;
+        }
+        const int s = fit % stages, cols = columns(ft), box = cols <= 16 ? 0 : cols <= 32 ? 1 : 2;
+        load_2d(smem_u32(smem + s * stage_bytes) + (UP ? 2 : 1) * kTile, &maps.x[box], fkb * kQB,
+                UP ? 0 : tb.row[ft.ai], full_bar(s));
+        ++fit;
+        if (++fkb == ft.kb1) {
+          fu += gridDim.x;
+          if (fu < units) ft = unit_at(a, fu, tiles, parts, nb), fkb = ft.kb0;
         }
       }
+      if (!waited) pdl_wait();
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -466,6 +545,28 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
         }
       }
     }
+  } else if (warp == 2) {
+    if (lane == 0) {
+      // ------------------------------------------- token scales --
+      if (!UP) pdl_wait();
+      uint32_t it = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const Unit t = unit_at(a, u, tiles, parts, nb);
+        const float* src = UP ? a.xs : a.hs + tb.row[t.ai];
+        const int64_t ld = UP ? kFewMaxT : a.h_rows;
+        const uint32_t bytes = columns(t) * 4;
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+          const int i = it % kScaleSlots;
+          if (!mbar_wait_inline(sempty_bar(i), ((it / kScaleSlots) & 1u) ^ 1u, abort_flag, a.err)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(sfull_bar(i), bytes);
+          bulk_copy(smem_u32(scales[i]), src + kb * ld, bytes, sfull_bar(i));
+        }
+      }
+    }
   } else if (warp >= 4) {
     // ---------------------------------------------------- epilogue --
     const int quad = warp & 3, row = quad * 32 + lane;  // this thread's weight row of the tile
@@ -478,28 +579,47 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
       if (lane == 0) mbar_arrive(tile_bar);
       if (!mbar_wait_inline(tile_bar, meets++ & 1u, abort_flag, a.err)) ok = false;
     };
+    // Scales of the weights: lane l holds those of K block kb0 + l (of 32 at a time), read a
+    // unit ahead; DOWN also the route weights of slots l and l + 32.
+    float w0n = 0.f, w1n = 0.f, r0n = 0.f, r1n = 0.f;
+    auto weight_scales = [&](const Unit& t, int kb, float& w0, float& w1) {
+      const int64_t so = ((int64_t)tb.expert[t.ai] * tiles + t.n) * nb + kb + lane;
+      w0 = kb + lane < t.kb1 ? __ldg((UP ? a.s_gate : a.s_down) + so) : 0.f;
+      if (UP) w1 = kb + lane < t.kb1 ? __ldg(a.s_up + so) : 0.f;
+    };
+    auto prefetch = [&](int u) {
+      if (u >= units) return;
+      const Unit t = unit_at(a, u, tiles, parts, nb);
+      weight_scales(t, t.kb0, w0n, w1n);
+      if (!UP) {
+        const int f = tb.first[t.ai], c = tb.first[t.ai + 1] - f;
+        r0n = lane < c ? a.w[tb.slots[f + lane]] : 0.f;
+        r1n = lane + 32 < c ? a.w[tb.slots[f + lane + 32]] : 0.f;
+      }
+    };
+    prefetch(blockIdx.x);
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const Unit t = unit_at(a, u, tiles, parts, nb);
-      const int e = tb.expert[t.ai], f = tb.first[t.ai], c = tb.first[t.ai + 1] - f, cols = columns(t);
-      uint32_t need = 0;  // groups of 16 columns that are used
-      for (int i = 0; i < c; ++i) need |= 1u << (UP ? tb.slots[f + i] % a.T / 16 : i / 16);
-      const int64_t so = ((int64_t)e * tiles + t.n) * nb;
-      const float* s0 = (UP ? a.s_gate : a.s_down) + so;
-      const float* s1 = UP ? a.s_up + so : s0;
-      const float* xs = UP ? a.xs : a.hs + tb.row[t.ai];
-      const int ld = UP ? kFewMaxT : a.h_rows;
+      const int f = tb.first[t.ai], c = tb.first[t.ai + 1] - f, cols = columns(t);
+      uint32_t need = (1u << (cols >> 4)) - 1u;  // groups of 16 columns that are used, and the columns
+      uint64_t used = 0;
+      if (UP) {
+        for (int i = 0; i < c; ++i) used |= 1ull << tb.tokens[f + i];
+        need = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) need |= (used >> (16 * g) & 0xffffu) ? 1u << g : 0u;
+      }
+      float w0s = w0n, w1s = w1n;
+      const float r0 = r0n, r1 = r1n;
+      prefetch(u + gridDim.x);
       float acc[UP ? 2 : 1][4][16] = {};
 #pragma unroll 1
       for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-        const int b = it % kBufs;
-        const float w0 = __ldg(s0 + kb), w1 = UP ? __ldg(s1 + kb) : 0.f;
-        float4 sc[4];
-        const float* xk = xs + (int64_t)kb * ld;
-        if (need & 1u) {  // the first group's scales before the wait
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sc[i] = *reinterpret_cast<const float4*>(xk + 4 * i);
-        }
-        if (!mbar_wait_inline(tfull_bar(b), (it / kBufs) & 1u, abort_flag, a.err)) {
+        const int b = it % kBufs, i = it % kScaleSlots, l = kb - t.kb0 & 31;
+        if (l == 0 && kb > t.kb0) weight_scales(t, kb, w0s, w1s);
+        const float w0 = __shfl_sync(0xffffffffu, w0s, l), w1 = UP ? __shfl_sync(0xffffffffu, w1s, l) : 0.f;
+        if (!mbar_wait_inline(sfull_bar(i), (it / kScaleSlots) & 1u, abort_flag, a.err) ||
+            !mbar_wait_inline(tfull_bar(b), (it / kBufs) & 1u, abort_flag, a.err)) {
           ok = false;
           break;
         }
@@ -507,63 +627,107 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           if (need >> g & 1u) {
-            if (g > 0) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) sc[i] = *reinterpret_cast<const float4*>(xk + g * 16 + 4 * i);
-            }
             uint32_t v[UP ? 2 : 1][16];
             tmem_ld16(my_tmem + b * kBufCols + g * 16, v[0]);
             if constexpr (UP) tmem_ld16(my_tmem + b * kBufCols + 64 + g * 16, v[UP ? 1 : 0]);
+            float4 sc[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sc[q] = *reinterpret_cast<const float4*>(&scales[i][g * 16 + 4 * q]);
             tmem_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float* s4 = reinterpret_cast<const float*>(&sc[i >> 2]);
-              acc[0][g][i] = fmaf(__uint_as_float(v[0][i]), s4[i & 3] * w0, acc[0][g][i]);
+            for (int q = 0; q < 16; ++q) {
+              const float s4 = reinterpret_cast<const float*>(&sc[q >> 2])[q & 3];
+              acc[0][g][q] = fmaf(__uint_as_float(v[0][q]), s4 * w0, acc[0][g][q]);
               if constexpr (UP)
-                acc[UP ? 1 : 0][g][i] = fmaf(__uint_as_float(v[UP ? 1 : 0][i]), s4[i & 3] * w1, acc[UP ? 1 : 0][g][i]);
+                acc[UP ? 1 : 0][g][q] = fmaf(__uint_as_float(v[UP ? 1 : 0][q]), s4 * w1, acc[UP ? 1 : 0][g][q]);
             }
           }
         }
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(tempty_bar(b));
+        if (lane == 0) mbar_arrive(tempty_bar(b)), mbar_arrive(sempty_bar(i));
       }
       if (!ok) break;
       if constexpr (UP) {
-        // h to shared memory, then one warp a slot: its 128 values share a scale
-        const bool in = t.n * 128 + row < a.F;
+        if (parts > 1) {
+          // Partial sums along K: the last of the tile's CTAs adds them in order.
+          const int tile = t.ai * tiles + t.n;
+          float* mine = a.partial + ((int64_t)tile * parts + t.part) * kFewPartialCols * 256 + row;
+          const int64_t stride = (int64_t)kFewPartialCols * 256;
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          if (need >> g & 1u) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (g * 16 + i < cols)
-                hbuf[(g * 16 + i) * 128 + row] = in ? acc[0][g][i] * silu_ref(acc[UP ? 1 : 0][g][i]) : 0.f;
+          for (int i = 0; i < kFewPartialCols; ++i)
+            if (used >> i & 1) mine[i * 256] = acc[0][0][i], mine[i * 256 + 128] = acc[UP ? 1 : 0][0][i];
+          __threadfence();
+          meet();
+          if (!ok) break;
+          if (warp == 4 && lane == 0) {
+            last_word = atomicAdd(a.count + tile, 1) == parts - 1;
+            __threadfence();
           }
-        meet();
-        if (!ok) break;
-        const int col = t.n * 128 + lane * 4;
-        for (int i = quad; i < c; i += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(hbuf + tb.slots[f + i] % a.T * 128 + lane * 4);
-          const BlockScale s = block_scale(__reduce_max_sync(
-              0xffffffffu, max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)))));
-          const int64_t r = tb.row[t.ai] + i;
-          if (col < a.F)
-            *reinterpret_cast<uint32_t*>(a.hq + r * a.F + col) =
-                e4m3x4(v.x * s.inv, v.y * s.inv, v.z * s.inv, v.w * s.inv);
-          if (lane == 0) a.hs[(int64_t)t.n * a.h_rows + r] = s.scale;
+          meet();
+          if (!ok) break;
+          if (!*reinterpret_cast<volatile int*>(&last_word)) continue;
+          const float* all = a.partial + (int64_t)tile * parts * stride + row;
+#pragma unroll
+          for (int i = 0; i < kFewPartialCols; ++i)
+            if (used >> i & 1) {
+              float g = 0.f, up = 0.f;
+              for (int q = 0; q < parts; ++q) {
+                g += __ldcg(all + q * stride + i * 256);
+                up += __ldcg(all + q * stride + i * 256 + 128);
+              }
+              acc[0][0][i] = g, acc[UP ? 1 : 0][0][i] = up;
+            }
         }
-        meet();  // before the next tile's values
-      } else if (t.n * 128 + row < a.H) {
+        // gate and up of 16 used columns at a time to shared memory; then a warp a slot
+        // computes its 128 values of h, which share a scale
+        const int col = t.n * 128 + lane * 4;
+        const bool in = col < a.F;
+        for (int c0 = 0; c0 < __popcll(used) && ok; c0 += 16) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            if (need >> g & 1u) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int at = __popcll(used & ((1ull << (g * 16 + i)) - 1ull)) - c0;  // place among the used ones
+                if ((used >> (g * 16 + i) & 1) && at >= 0 && at < 16) {
+                  hbuf[at * 256 + row] = acc[0][g][i];
+                  hbuf[at * 256 + 128 + row] = acc[UP ? 1 : 0][g][i];
+                }
+              }
+            }
+          meet();
+          if (!ok) break;
+          for (int i = quad; i < c; i += 4) {
+            const int at = __popcll(used & ((1ull << tb.tokens[f + i]) - 1ull)) - c0;
+            if (at < 0 || at >= 16) continue;
+            const float4 g = *reinterpret_cast<const float4*>(hbuf + at * 256 + lane * 4);
+            const float4 p = *reinterpret_cast<const float4*>(hbuf + at * 256 + 128 + lane * 4);
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (in) v = make_float4(g.x * silu_ref(p.x), g.y * silu_ref(p.y), g.z * silu_ref(p.z), g.w * silu_ref(p.w));
+            const BlockScale s = block_scale(__reduce_max_sync(
+                0xffffffffu, max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)))));
+            const int64_t r = tb.row[t.ai] + i;
+            if (in)
+              *reinterpret_cast<uint32_t*>(a.hq + r * a.F + col) =
+                  e4m3x4(v.x * s.inv, v.y * s.inv, v.z * s.inv, v.w * s.inv);
+            if (lane == 0) a.hs[(int64_t)t.n * a.h_rows + r] = s.scale;
+          }
+          meet();  // before the next values
+        }
+      } else if (t.n * 128 + quad * 32 < a.H) {  // H is a multiple of 16: a warp may be cut
+        const bool in = t.n * 128 + row < a.H;
         float* d = a.d + ((int64_t)t.part * n) * a.H + t.n * 128 + row;
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int g = 0; g < 4; ++g) {
+          if (g * 16 >= c) break;
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (g * 16 + i < c) {
-              const int slot = tb.slots[f + g * 16 + i];
-              d[(int64_t)slot * a.H] = acc[0][g][i] * a.w[slot];
+              const float w = __shfl_sync(0xffffffffu, g < 2 ? r0 : r1, (g & 1) * 16 + i);
+              if (in) d[(int64_t)tb.slots[f + g * 16 + i] * a.H] = acc[0][g][i] * w;
             }
+        }
       }
     }
   }
@@ -590,10 +754,11 @@ namespace frank {
 int launch_few_route(const FewRoute& a, cudaStream_t st) {
   const int nb = (a.H + kQB - 1) / kQB, slice = (nb + kRouteCtas - 1) / kRouteCtas * kQB;
   const size_t smem = (size_t)kRouteTok * slice * 4;
-  FRANK_CUDA_TRY(cudaFuncSetAttribute(few_route_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  const auto kern = a.E <= 128 ? few_route_kernel<4> : few_route_kernel<8>;
+  FRANK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)(kRouteTok * kNormMaxH / kRouteCtas * 4)));
   const dim3 grid((unsigned)((a.T + kRouteTok - 1) / kRouteTok * kRouteCtas));
-  FRANK_CUDA_TRY(launch_chained(few_route_kernel, grid, dim3(kRouteThreads), smem, st, kRouteCtas, a));
+  FRANK_CUDA_TRY(launch_chained(kern, grid, dim3(kRouteThreads), smem, st, kRouteCtas, a));
   FRANK_LAUNCH_CHECK();
   return FRANK_OK;
 }
@@ -631,9 +796,9 @@ constexpr size_t kFewSmem = 232448 - 12288;
 
 template <bool UP>
 static int launch_few_product(const FewMaps& maps, const FewArgs& a, cudaStream_t st) {
-  const int cols = (a.T + 15) & ~15, box = tile_tokens(a.T);
+  const int box = tile_tokens(a.T);
   const uint32_t stage = (UP ? 2 : 1) * kTile + box * kQB;
-  const size_t hbuf = UP ? (size_t)cols * 128 * 4 : 0;
+  const size_t hbuf = UP ? 16 * 256 * 4 : 0;
   const int fit = (int)((kFewSmem - 1024 - hbuf) / stage), stages = fit < kMaxStages ? fit : kMaxStages;
   FRANK_CUDA_TRY(cudaFuncSetAttribute(few_product_kernel<UP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)kFewSmem));
@@ -653,6 +818,20 @@ int few_parts(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
   return (int)(parts < 1 ? 1 : parts > kFewMaxParts ? kFewMaxParts : parts);
 }
 
+// The gate/up tiles of one or two tokens leave SMs idle (one SM draws 51 GB/s of
+// weights through the MMA): K is divided then.
+int few_up_parts(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
+  const int64_t tiles = (k * T < E ? k * T : E) * q_blocks(F), most = q_blocks(H) / 4;
+  if (tiles <= 0 || T > kFewPartialCols) return 1;
+  const int64_t want = num_sms() / tiles, parts = want < most ? want : most;
+  return (int)(parts < 1 ? 1 : parts > kFewMaxParts ? kFewMaxParts : parts);
+}
+
+// Floats of the partial sums, and counters, of few_up_parts > 1.
+int64_t few_partial_tiles(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
+  return few_up_parts(T, E, k, H, F) > 1 ? (k * T < E ? k * T : E) * q_blocks(F) : 0;
+}
+
 int64_t few_h_rows(int64_t T, int64_t E, int64_t k) {
   const int64_t n = k * T;  // up to 15 rows of padding for each expert that has slots
   return (n + 15 * (n < E ? n : E) + 15) / 16 * 16;
@@ -661,6 +840,7 @@ int64_t few_h_rows(int64_t T, int64_t E, int64_t k) {
 int launch_few_experts(const FewArgs& args, int32_t* err, cudaStream_t st) {
   FewArgs a = args;
   a.err = device_error_word();
+  a.up_parts = few_up_parts(a.T, a.E, a.k, a.H, a.F);
   a.parts = few_parts(a.T, a.E, a.k, a.H, a.F);
   a.h_rows = (int)few_h_rows(a.T, a.E, a.k);
   if (err != nullptr) {

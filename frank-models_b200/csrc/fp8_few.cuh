@@ -7,7 +7,7 @@ namespace frank {
 
 constexpr int kFewMaxE = (int)kFp8MaxE;
 constexpr int kFewMaxT = 64, kFewMaxSlots = 512;
-constexpr int kFewMaxParts = 4;
+constexpr int kFewMaxParts = 4, kFewPartialCols = 4;  // divisions of K; tokens where gate/up is divided
 
 struct FewRoute {
   const void* x;  // [T, H]
@@ -21,6 +21,8 @@ struct FewRoute {
   float* xs;     // [ceil(H/128), kFewMaxT]
   float* w;      // [k, T]
   int32_t* ids;  // [k, T]
+  int32_t* count;  // zeroed for few_product
+  int n_count;
 };
 
 struct FewArgs {
@@ -34,11 +36,14 @@ struct FewArgs {
   const float* w;
   const int32_t* ids;
   int T, E, k, H, F;
-  int parts, h_rows;  // set by launch_few_experts
+  float* partial;  // [few_partial_tiles, parts, kFewPartialCols, 256]
+  int32_t* count;  // [few_partial_tiles]
+  int up_parts, parts, h_rows;  // set by launch_few_experts
   int32_t* err;       // device error word
 };
 
 int few_parts(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F);
+int64_t few_partial_tiles(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F);
 int64_t few_h_rows(int64_t T, int64_t E, int64_t k);
 int launch_few_route(const FewRoute& a, cudaStream_t st);
 int launch_few_experts(const FewArgs& a, int32_t* err, cudaStream_t st);

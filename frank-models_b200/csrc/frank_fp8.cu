@@ -50,6 +50,8 @@ struct Fp8MoeWs {
   uint8_t* hq;            // [n, F]
   float* hs;              // [F/128, n]
   float* d;               // [n, H]
+  float* partial;         // a few tokens: partial sums of gate/up, and their counters
+  int32_t* count;
   float* logits;
   void* perm;
   size_t perm_bytes;
@@ -74,6 +76,9 @@ static size_t fp8_moe_layout(int64_t T, int64_t H, int64_t F, int64_t E, int64_t
   l.hq = c.take<uint8_t>(h_rows * F);
   l.hs = c.take<float>(h_rows * q_blocks(F));
   l.d = c.take<float>(parts * n * H);
+  const int64_t tiles = few ? few_partial_tiles(T, E, k, H, F) : 0;
+  l.partial = c.take<float>(tiles * kFewMaxParts * kFewPartialCols * 256);
+  l.count = c.take<int32_t>(tiles);
   l.logits = c.take<float>(router_scratch_bytes(FRANK_BF16, T, H, E) / sizeof(float) + 1);
   l.perm_bytes = permute_workspace_size(n, E);
   l.perm = c.take<char>(l.perm_bytes);
@@ -114,6 +119,8 @@ static FewArgs few_args(const Fp8Weights& W, int64_t T, int64_t E, int64_t k, in
   a.s_down = W.s_down;
   a.xq = L.xq;
   a.xs = L.xs;
+  a.partial = L.partial;
+  a.count = L.count;
   a.hq = L.hq;
   a.hs = L.hs;
   a.d = L.d;
@@ -146,6 +153,8 @@ static FewRoute few_route(int x_dtype, const void* x, const float* norm_w, float
   r.xs = L.xs;
   r.w = w;
   r.ids = ids;
+  r.count = L.count;
+  r.n_count = (int)few_partial_tiles(T, E, k, H, F);
   return r;
 }
 
