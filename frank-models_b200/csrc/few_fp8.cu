@@ -7,18 +7,21 @@
 //               the partial logits are exchanged through distributed shared memory
 //               and added in CTA order.
 //   few_product<UP>    h = gate * silu(up), quantised: tiles of 128 columns of F (one
-//               quantisation block) of one expert, for all T tokens
+//               quantisation block) of one expert
 //   few_product<DOWN>  d[slot] = route weight * down(h[slot]): tiles of 128 rows of H of
-//               one expert, for its slots; along a long F in several parts, which
-//               the combine adds in order
+//               one expert
 //
 // Weights and tokens change places: the 128 weight rows are the M of
-// tcgen05.mma.kind::f8f6f4 (UP: one MMA for gate, one for up), the tokens, 16 to 64
-// of them, its N.  So the weights go from TMA to the tensor core without passing
-// through a register, and a K block of 128 costs the epilogue 16 to 64 columns: they
-// are scaled and summed in fp32 registers from four TMEM buffers.  The ring of K
-// blocks keeps up to 190 KB an SM under way.  (An earlier form multiplied in warps by
-// mma.sync: 610 instructions for 8 KB of weights, 2.5 to 4 TB/s.)
+// tcgen05.mma.kind::f8f6f4 (UP: one MMA for gate, one for up), the expert's tokens, 16
+// or 32 of them, its N.  So the weights go from TMA to the tensor core without passing
+// through a register, and a K block of 128 costs the epilogue 16 or 32 columns: they
+// are scaled and summed in fp32 registers from eight TMEM buffers.  The ring of K
+// blocks keeps up to 190 KB an SM under way.  An MMA reads 128 weight rows in 80 ns
+// whatever its N, so one SM draws 51 GB/s and all of them 7.5 TB/s: the K blocks have
+// to be spread evenly over the SMs.  Where whole tiles would not, every SM takes the same
+// number of K blocks in a row, and the last SM of a divided tile adds its partial sums
+// in order.  (An earlier form multiplied in warps by mma.sync: 610 instructions for 8 KB
+// of weights, 2.5 to 4 TB/s.)
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -96,8 +99,7 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
   pdl_wait();
   pdl_launch();
   cluster_arrive();  // every CTA has started before its memory is written
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < a.n_count; i += kRouteThreads) a.count[i] = 0;
+  for (int i = blockIdx.x * kRouteThreads + threadIdx.x; i < a.n_count; i += gridDim.x * kRouteThreads) a.count[i] = 0;
   // one (token, block) a warp: a vector of 4 for each lane
   for (int i = warp; i < kRouteTok * sb; i += kWarps) {
     const int t = i / sb, b = i % sb, h = h0 + b * kQB + lane * 4;
@@ -252,19 +254,23 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
 }
 
 // ------------------------------------------------------------- products --
-constexpr int kFewThreads = 256;  // warp 0: TMA, warp 1: MMA, warp 2: scales, warps 4..7: epilogue
+// warp 0: TMA, warp 1: MMA, warp 2: scales of h (DOWN), warp 3: token rows and their scales
+// (UP), warps 4..7 and 8..11: epilogue of every other tile
+constexpr int kFewThreads = 384, kGroupWarps = 4;
 constexpr uint32_t kTile = 128 * kQB;  // bytes of 128 weight rows of a K block
-constexpr int kMaxStages = 12, kBufs = 4, kBufCols = 128, kScaleSlots = 8;
+// TMEM buffers and scale slots: half of them for each epilogue group, which then sees every
+// phase of its barriers (a wait by parity must not miss one)
+constexpr int kMaxStages = 12, kBufs = 8, kGroupBufs = 4, kBufCols = 64, kScaleSlots = 16, kGroupSlots = 8;
+constexpr int kMaxTokens = 32;  // of a tile
 constexpr uint32_t kTmemCols = kBufs * kBufCols;
 
 struct FewMaps {
-  CUtensorMap w, w2;   // UP: gate and up; DOWN: down (boxes of 128 rows)
-  CUtensorMap x[3];    // tokens: boxes of 16, 32 and 64 rows
+  CUtensorMap w, w2;  // UP: gate and up; DOWN: down (boxes of 128 rows)
+  CUtensorMap x[2];   // DOWN: rows of h, boxes of 16 and 32
 };
 
-// The tokens a tile takes: as many as a stage has rows for (also where a caller's ids
-// name an expert twice for one token, and it has more slots than there are tokens).
-__host__ __device__ __forceinline__ int tile_tokens(int T) { return T <= 16 ? 16 : T <= 32 ? 32 : 64; }
+// The slots that a tile takes at once.
+__host__ __device__ __forceinline__ int tile_tokens(int T) { return T <= 16 ? 16 : kMaxTokens; }
 
 // The routing as every CTA sees it: the experts that have tokens, ascending, and their
 // slots, at most tile_tokens an entry.  An entry's rows of h start at a multiple of 16.
@@ -282,16 +288,18 @@ struct Table {
 // an expert adds up the chunks.  at: scratch [kFewMaxSlots / 32][kFewMaxE].
 __device__ __forceinline__ void build_table(const FewArgs& a, Table& tb, uint16_t (*at)[kFewMaxE], int* sums) {
   const int n = a.k * a.T, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int kWarps = kFewThreads / 32, kChunks = kFewMaxSlots / 32;
-  static_assert(kFewThreads == kFewMaxE && kChunks == 2 * kWarps, "a thread an expert, two chunks a warp");
+  constexpr int kWarps = kFewMaxE / 32, kChunks = kFewMaxSlots / 32;  // of the threads that work here
+  static_assert(kFewThreads >= kFewMaxE && kChunks == 2 * kWarps, "a thread an expert, two chunks a warp");
+  const bool works = tid < kFewMaxE;
   const int chunks = (n + 31) / 32;
   int id[2], rank[2], size[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int s = (warp + i * kWarps) * 32 + lane;
-    id[i] = s < n ? min(max(__ldcg(a.ids + s), 0), a.E - 1) : -1;
+    id[i] = works && s < n ? min(max(__ldcg(a.ids + s), 0), a.E - 1) : -1;
   }
-  for (int c = 0; c < chunks; ++c) at[c][tid] = 0;
+  if (works)
+    for (int c = 0; c < chunks; ++c) at[c][tid] = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -302,11 +310,12 @@ __device__ __forceinline__ void build_table(const FewArgs& a, Table& tb, uint16_
   }
   __syncthreads();
   int c = 0;
-  for (int i = 0; i < chunks; ++i) {
-    const int t = at[i][tid];
-    at[i][tid] = (uint16_t)c;
-    c += t;
-  }
+  if (works)
+    for (int i = 0; i < chunks; ++i) {
+      const int t = at[i][tid];
+      at[i][tid] = (uint16_t)c;
+      c += t;
+    }
   // before this expert: slots (bits 0..9), entries (10..18) and groups of 16 rows (19..)
   const int cap = tile_tokens(a.T), mine = c | (c + cap - 1) / cap << 10 | (c + 15) / 16 << 19;
   int v = mine;
@@ -315,7 +324,7 @@ __device__ __forceinline__ void build_table(const FewArgs& a, Table& tb, uint16_
     const int u = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += u;
   }
-  if (lane == 31) sums[warp] = v;
+  if (works && lane == 31) sums[warp] = v;
   __syncthreads();
   int before = v - mine, total = 0;
 #pragma unroll
@@ -391,34 +400,82 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// One unit of work: tile `n` (128 rows) of the ai-th entry, K blocks [kb0, kb1).
-struct Unit {
-  int ai, n, part, kb0, kb1;
-};
-__device__ __forceinline__ Unit unit_at(const FewArgs& a, int u, int tiles, int parts, int nb) {
-  Unit t;
-  t.part = u % parts;
-  t.n = u / parts % tiles;
-  t.ai = u / parts / tiles;
-  t.kb0 = nb * t.part / parts;
-  t.kb1 = nb * (t.part + 1) / parts;
-  return t;
+// After the wait: keeps what uses the values behind it.
+template <int N>
+__device__ __forceinline__ void pin(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
+
+// A CTA's way through the K blocks of all tiles (entry after entry, tile after tile):
+// every gridDim.x-th whole tile, or an equal run of K blocks that may begin and end
+// inside a tile.
+// Where it stands: tile n (128 rows) of entry ai, K blocks [kb0, kb1()).
+struct Walk {
+  int nb, tiles, ai, n, kb0, todo, dai, dn;  // todo: K blocks; dai, dn: the step to the next tile
+
+  // slack: K blocks that a CTA may have more than the mean before tiles are divided
+  __device__ __forceinline__ Walk(int entries, int tiles_, int nb_, int slack) : nb(nb_), tiles(tiles_) {
+    const int G = gridDim.x, all = entries * tiles, total = all * nb, b = blockIdx.x;
+    const bool whole = total < G || (all + G - 1) / G * nb - total / G <= slack;  // a run is never empty
+    const int first = whole ? b : start(b, total) / nb;
+    kb0 = whole ? 0 : start(b, total) - first * nb;
+    todo = whole ? (b < all ? (all - b + G - 1) / G * nb : 0) : start(b + 1, total) - start(b, total);
+    ai = first / tiles;
+    n = first - ai * tiles;
+    dai = whole ? G / tiles : 0;
+    dn = whole ? G - dai * tiles : 1;
+  }
+  static __device__ __forceinline__ int start(int cta, int total) {
+    const int q = total / (int)gridDim.x;
+    return cta * q + min(cta, total - q * (int)gridDim.x);
+  }
+  // The CTA whose run holds K block x (no run is empty).
+  static __device__ __forceinline__ int cta_of(int x, int total) {
+    const int q = total / (int)gridDim.x, r = total - q * (int)gridDim.x;
+    return x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q;
+  }
+  __device__ __forceinline__ bool more() const { return todo > 0; }
+  __device__ __forceinline__ int kb1() const { return min(nb, kb0 + todo); }
+  __device__ __forceinline__ void advance() {
+    todo -= kb1() - kb0;
+    kb0 = 0;
+    ai += dai;
+    n += dn;
+    if (n >= tiles) n -= tiles, ++ai;
+  }
+};
+
+// K blocks of the tiles of each epilogue group so far; tiles alternate.
+struct Turns {
+  uint32_t mine = 0, other = 0;
+  int group = 0;
+  __device__ __forceinline__ uint32_t buf() const { return group * kGroupBufs + mine % kGroupBufs; }
+  __device__ __forceinline__ uint32_t buf_parity() const { return mine / kGroupBufs & 1u; }
+  __device__ __forceinline__ uint32_t slot() const { return group * kGroupSlots + mine % kGroupSlots; }
+  __device__ __forceinline__ uint32_t slot_parity() const { return mine / kGroupSlots & 1u; }
+  __device__ __forceinline__ void next_tile() {
+    const uint32_t t = mine;
+    mine = other;
+    other = t;
+    group ^= 1;
+  }
+};
 
 template <bool UP>
 __global__ void __launch_bounds__(kFewThreads, 1)
 few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ FewArgs a, int stages,
                    uint32_t stage_bytes) {
+  constexpr int kSums = UP ? 256 : 128;  // of a column: 128 rows of gate and of up, or of down
+  constexpr uint32_t kWeights = (UP ? 2 : 1) * kTile;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* hbuf = reinterpret_cast<float*>(smem + stages * stage_bytes);  // UP: [16][gate, up][128]
   __shared__ Table tb;
-  __shared__ int sums[kFewThreads / 32];
-  __shared__ uint64_t bars[2 * kMaxStages + 2 * kBufs + 2 * kScaleSlots + 1];
-  __shared__ alignas(128) float scales[kScaleSlots][kFewMaxT];  // of the token operand, a slot for each K block
+  __shared__ int sums[kFewMaxE / 32];
+  __shared__ uint64_t bars[2 * kMaxStages + 2 * kBufs + 2 * kScaleSlots + 2];
+  __shared__ alignas(128) float scales[kScaleSlots][kMaxTokens];  // of the tokens, a slot for each K block
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word, last_word;
+  __shared__ int abort_word, last_word[2];
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t bar0 = smem_u32(bars);
@@ -428,21 +485,21 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
   auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * kMaxStages + kBufs + b); };
   auto sfull_bar = [&](int i) { return bar0 + 8u * (2 * kMaxStages + 2 * kBufs + i); };
   auto sempty_bar = [&](int i) { return bar0 + 8u * (2 * kMaxStages + 2 * kBufs + kScaleSlots + i); };
-  const uint32_t tile_bar = bar0 + 8u * (2 * kMaxStages + 2 * kBufs + 2 * kScaleSlots);
+  auto tile_bar = [&](int g) { return bar0 + 8u * (2 * kMaxStages + 2 * kBufs + 2 * kScaleSlots + g); };
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
-      mbar_init(full_bar(s), 1);
+      mbar_init(full_bar(s), UP ? 2 : 1);  // the bytes of TMA; UP: and the rows of warp 3
       mbar_init(empty_bar(s), 1);
     }
     for (int b = 0; b < kBufs; ++b) {
       mbar_init(tfull_bar(b), 1);
-      mbar_init(tempty_bar(b), 4);
+      mbar_init(tempty_bar(b), kGroupWarps);
     }
     for (int i = 0; i < kScaleSlots; ++i) {
       mbar_init(sfull_bar(i), 1);
-      mbar_init(sempty_bar(i), 4);
+      mbar_init(sempty_bar(i), kGroupWarps);
     }
-    mbar_init(tile_bar, 4);
+    for (int g = 0; g < 2; ++g) mbar_init(tile_bar(g), kGroupWarps);
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
@@ -464,40 +521,39 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
   fence_after();
   const uint32_t tmem = tmem_slot;
 
-  const int K = UP ? a.H : a.F, N = UP ? a.F : a.H, n = a.k * a.T;
-  const int nb = (K + kQB - 1) / kQB, tiles = (N + kQB - 1) / kQB, parts = UP ? a.up_parts : a.parts;
-  const int units = tb.entries * tiles * parts;
-  // columns of a unit: all tokens, or the expert's slots, to a multiple of 16
-  auto columns = [&](const Unit& t) { return UP ? (a.T + 15) & ~15 : (tb.first[t.ai + 1] - tb.first[t.ai] + 15) & ~15; };
+  const int K = UP ? a.H : a.F, N = UP ? a.F : a.H;
+  const int nb = (K + kQB - 1) / kQB, tiles = (N + kQB - 1) / kQB;
+  // dividing a tile costs about 3 us: 5 K blocks of UP, 10 of DOWN
+  const Walk walk(tb.entries, tiles, nb, UP ? 5 : 10);
+  auto tokens_of = [&](const Walk& t) { return tb.first[t.ai + 1] - tb.first[t.ai]; };
 
   if (warp == 0) {
     if (lane == 0) {
       // ------------------------------------------------ TMA producer --
       uint64_t policy;
       asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-      // The ring is filled with weights first; the token operand of a stage follows, at once
-      // or, for the first stages of DOWN, when h is there.
-      int u = blockIdx.x, kb = 0, fu = u, fkb = 0;  // next weights, next tokens
+      // The ring is filled with weights first; DOWN's rows of h follow, at once or, for the
+      // first stages, when they are there.
+      Walk w = walk, fw = walk;  // of the weights, of h
+      int kb = w.kb0, fkb = w.kb0;
       uint32_t it = 0, fit = 0;
       bool ok = true, waited = UP;
-      Unit t, ft;
-      if (u < units) t = ft = unit_at(a, u, tiles, parts, nb), kb = fkb = t.kb0;
-      while (fu < units && ok) {
-        if (u < units && (waited ? it == fit : it < (uint32_t)stages)) {
+      while (fw.more() && ok) {
+        if (w.more() && (waited ? it == fit : it < (uint32_t)stages)) {
           const int s = it % stages;
           if (!mbar_wait_inline(empty_bar(s), ((it / stages) & 1u) ^ 1u, abort_flag, a.err)) {
             ok = false;
             break;
           }
-          const int e = tb.expert[t.ai], cols = columns(t), box = cols <= 16 ? 0 : cols <= 32 ? 1 : 2;
+          const int e = tb.expert[w.ai];
           const uint32_t st = smem_u32(smem + s * stage_bytes);
-          mbar_expect_tx(full_bar(s), (UP ? 2 : 1) * kTile + (16u << box) * kQB);
-          load_weights(st, &maps.w, kb * kQB, t.n * 128, e, full_bar(s), policy);
-          if (UP) load_weights(st + kTile, &maps.w2, kb * kQB, t.n * 128, e, full_bar(s), policy);
+          mbar_expect_tx(full_bar(s), kWeights + (UP ? 0 : tokens_of(w) <= 16 ? 16 * kQB : 32 * kQB));
+          load_weights(st, &maps.w, kb * kQB, w.n * 128, e, full_bar(s), policy);
+          if (UP) load_weights(st + kTile, &maps.w2, kb * kQB, w.n * 128, e, full_bar(s), policy);
           ++it;
-          if (++kb == t.kb1) {
-            u += gridDim.x;
-            if (u < units) t = unit_at(a, u, tiles, parts, nb), kb = t.kb0;
+          if (++kb == w.kb1()) {
+            w.advance();
+            kb = 0;
           }
           if (!waited) continue;
         }
@@ -505,13 +561,15 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
           pdl_wait();
           waited = true;
         }
-        const int s = fit % stages, cols = columns(ft), box = cols <= 16 ? 0 : cols <= 32 ? 1 : 2;
-        load_2d(smem_u32(smem + s * stage_bytes) + (UP ? 2 : 1) * kTile, &maps.x[box], fkb * kQB,
-                UP ? 0 : tb.row[ft.ai], full_bar(s));
+        if (!UP) {
+          const int s = fit % stages;
+          load_2d(smem_u32(smem + s * stage_bytes) + kWeights, &maps.x[tokens_of(fw) <= 16 ? 0 : 1], fkb * kQB,
+                  tb.row[fw.ai], full_bar(s));
+        }
         ++fit;
-        if (++fkb == ft.kb1) {
-          fu += gridDim.x;
-          if (fu < units) ft = unit_at(a, fu, tiles, parts, nb), fkb = ft.kb0;
+        if (++fkb == fw.kb1()) {
+          fw.advance();
+          fkb = 0;
         }
       }
       if (!waited) pdl_wait();
@@ -520,25 +578,27 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
     if (lane == 0) {
       // -------------------------------------------------- MMA issuer --
       uint32_t it = 0;
+      Turns turn;
       bool ok = true;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        const Unit t = unit_at(a, u, tiles, parts, nb);
+      for (Walk t = walk; t.more() && ok; t.advance(), turn.next_tile()) {
         // kind::f8f6f4: D fp32, A and B e4m3, N >> 3 at [17,23), M >> 4 at [24,29)
-        const uint32_t idesc = (1u << 4) | ((uint32_t)(columns(t) >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-        for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-          const int s = it % stages, b = it % kBufs;
-          if (!mbar_wait_inline(tempty_bar(b), ((it / kBufs) & 1u) ^ 1u, abort_flag, a.err) ||
+        const uint32_t cols = tokens_of(t) <= 16 ? 16 : 32;
+        const uint32_t idesc = (1u << 4) | (cols >> 3 << 17) | ((uint32_t)(128 >> 4) << 24);
+        for (int kb = t.kb0, kb1 = t.kb1(); kb < kb1; ++kb, ++it, ++turn.mine) {
+          const int s = it % stages, b = turn.buf();
+          if (!mbar_wait_inline(tempty_bar(b), turn.buf_parity() ^ 1u, abort_flag, a.err) ||
               !mbar_wait_inline(full_bar(s), (it / stages) & 1u, abort_flag, a.err)) {
             ok = false;
             break;
           }
           fence_after();
           const uint32_t st = smem_u32(smem + s * stage_bytes);
-          const uint64_t wd = smem_desc(st), w2d = smem_desc(st + kTile), xd = smem_desc(st + (UP ? 2 : 1) * kTile);
+          const uint64_t wd = smem_desc(st), w2d = smem_desc(st + kTile), xd = smem_desc(st + kWeights);
 #pragma unroll
           for (int j = 0; j < kQB / 32; ++j) {  // 32 bytes along K inside the swizzled row
             mma(tmem + b * kBufCols, wd + (uint64_t)(2 * j), xd + (uint64_t)(2 * j), idesc, j != 0);
-            if (UP) mma(tmem + b * kBufCols + 64, w2d + (uint64_t)(2 * j), xd + (uint64_t)(2 * j), idesc, j != 0);
+            if (UP)
+              mma(tmem + b * kBufCols + kMaxTokens, w2d + (uint64_t)(2 * j), xd + (uint64_t)(2 * j), idesc, j != 0);
           }
           commit(empty_bar(s));
           commit(tfull_bar(b));
@@ -546,187 +606,251 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
       }
     }
   } else if (warp == 2) {
-    if (lane == 0) {
-      // ------------------------------------------- token scales --
-      if (!UP) pdl_wait();
-      uint32_t it = 0;
+    if (!UP && lane == 0) {
+      // --------------------------------------------- scales of h --
+      pdl_wait();
+      Turns turn;
       bool ok = true;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        const Unit t = unit_at(a, u, tiles, parts, nb);
-        const float* src = UP ? a.xs : a.hs + tb.row[t.ai];
-        const int64_t ld = UP ? kFewMaxT : a.h_rows;
-        const uint32_t bytes = columns(t) * 4;
-        for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-          const int i = it % kScaleSlots;
-          if (!mbar_wait_inline(sempty_bar(i), ((it / kScaleSlots) & 1u) ^ 1u, abort_flag, a.err)) {
+      for (Walk t = walk; t.more() && ok; t.advance(), turn.next_tile()) {
+        const float* src = a.hs + tb.row[t.ai];
+        const uint32_t bytes = (tokens_of(t) + 15) / 16 * 64;
+        for (int kb = t.kb0, kb1 = t.kb1(); kb < kb1; ++kb, ++turn.mine) {
+          const int i = turn.slot();
+          if (!mbar_wait_inline(sempty_bar(i), turn.slot_parity() ^ 1u, abort_flag, a.err)) {
             ok = false;
             break;
           }
           mbar_expect_tx(sfull_bar(i), bytes);
-          bulk_copy(smem_u32(scales[i]), src + kb * ld, bytes, sfull_bar(i));
+          bulk_copy(smem_u32(scales[i]), src + (int64_t)kb * a.h_rows, bytes, sfull_bar(i));
         }
       }
     }
-  } else if (warp >= 4) {
+  } else if (warp == 3) {
+    if (UP) {
+      // ------------------------------- token rows and their scales --
+      // 16 bytes a lane, eight lanes a row, into the swizzled tile; three K blocks under way
+      constexpr int kAhead = 3;
+      const int r0 = lane >> 3, chunk = lane & 7;
+      uint32_t it = 0, done = 0;
+      int slots_under_way[kAhead] = {};  // their scale slots, the oldest first
+      Turns turn;
+      bool ok = true;
+      auto arrive = [&]() {  // K block `done` is in shared memory
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full_bar(done % stages)), mbar_arrive(sfull_bar(slots_under_way[0]));
+#pragma unroll
+        for (int i = 0; i + 1 < kAhead; ++i) slots_under_way[i] = slots_under_way[i + 1];
+        ++done;
+      };
+      for (Walk t = walk; t.more() && ok; t.advance(), turn.next_tile()) {
+        const int c = tokens_of(t), *tok = tb.tokens + tb.first[t.ai];
+        for (int kb = t.kb0, kb1 = t.kb1(); kb < kb1; ++kb, ++turn.mine) {
+          const int s = it % stages, i = turn.slot();
+          if (!mbar_wait_inline(empty_bar(s), ((it / stages) & 1u) ^ 1u, abort_flag, a.err) ||
+              !mbar_wait_inline(sempty_bar(i), turn.slot_parity() ^ 1u, abort_flag, a.err)) {
+            ok = false;
+            break;
+          }
+          const uint32_t st = smem_u32(smem + s * stage_bytes) + kWeights;
+          const int k = kb * kQB + chunk * 16;
+          for (int r = r0; r < c; r += 4) {
+            const uint8_t* src = a.xq + (int64_t)tok[r] * a.H + (k < a.H ? k : 0);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(st + r * kQB + ((chunk ^ (r & 7)) << 4)),
+                         "l"(src), "r"(k < a.H ? 16 : 0)
+                         : "memory");
+          }
+          if (lane < c)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&scales[i][lane])),
+                         "l"(a.xs + (int64_t)kb * kFewMaxT + tok[lane])
+                         : "memory");
+          asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+          for (int q = 0; q < kAhead; ++q)
+            if (q == (int)(it - done)) slots_under_way[q] = i;
+          ++it;
+          if (it - done >= kAhead) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+            arrive();
+          }
+        }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      while (ok && done < it) arrive();
+    }
+  } else {
     // ---------------------------------------------------- epilogue --
-    const int quad = warp & 3, row = quad * 32 + lane;  // this thread's weight row of the tile
+    const int quad = warp & 3, group = (warp - 4) >> 2;
+    const int row = quad * 32 + lane;  // this thread's weight row of the tile
     const uint32_t my_tmem = tmem + ((uint32_t)(quad * 32) << 16);
-    uint32_t it = 0, meets = 0;
+    float* sums_buf = reinterpret_cast<float*>(smem + stages * stage_bytes) + group * 16 * kSums;
+    uint32_t it = 0, meets = 0;  // K blocks of this group's tiles
     bool ok = true;
-    // the four warps of the epilogue meet (bounded, unlike a named barrier)
+    // the four warps of a group meet (bounded, unlike a named barrier)
     auto meet = [&]() {
       __syncwarp();
-      if (lane == 0) mbar_arrive(tile_bar);
-      if (!mbar_wait_inline(tile_bar, meets++ & 1u, abort_flag, a.err)) ok = false;
+      if (lane == 0) mbar_arrive(tile_bar(group));
+      if (!mbar_wait_inline(tile_bar(group), meets++ & 1u, abort_flag, a.err)) ok = false;
     };
-    // Scales of the weights: lane l holds those of K block kb0 + l (of 32 at a time), read a
-    // unit ahead; DOWN also the route weights of slots l and l + 32.
-    float w0n = 0.f, w1n = 0.f, r0n = 0.f, r1n = 0.f;
-    auto weight_scales = [&](const Unit& t, int kb, float& w0, float& w1) {
-      const int64_t so = ((int64_t)tb.expert[t.ai] * tiles + t.n) * nb + kb + lane;
-      w0 = kb + lane < t.kb1 ? __ldg((UP ? a.s_gate : a.s_down) + so) : 0.f;
-      if (UP) w1 = kb + lane < t.kb1 ? __ldg(a.s_up + so) : 0.f;
-    };
-    auto prefetch = [&](int u) {
-      if (u >= units) return;
-      const Unit t = unit_at(a, u, tiles, parts, nb);
-      weight_scales(t, t.kb0, w0n, w1n);
-      if (!UP) {
-        const int f = tb.first[t.ai], c = tb.first[t.ai + 1] - f;
-        r0n = lane < c ? a.w[tb.slots[f + lane]] : 0.f;
-        r1n = lane + 32 < c ? a.w[tb.slots[f + lane + 32]] : 0.f;
-      }
-    };
-    prefetch(blockIdx.x);
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-      const Unit t = unit_at(a, u, tiles, parts, nb);
-      const int f = tb.first[t.ai], c = tb.first[t.ai + 1] - f, cols = columns(t);
-      uint32_t need = (1u << (cols >> 4)) - 1u;  // groups of 16 columns that are used, and the columns
-      uint64_t used = 0;
-      if (UP) {
-        for (int i = 0; i < c; ++i) used |= 1ull << tb.tokens[f + i];
-        need = 0;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) need |= (used >> (16 * g) & 0xffffu) ? 1u << g : 0u;
-      }
-      float w0s = w0n, w1s = w1n;
-      const float r0 = r0n, r1 = r1n;
-      prefetch(u + gridDim.x);
-      float acc[UP ? 2 : 1][4][16] = {};
+    int turn = 0;
+    for (Walk t = walk; t.more() && ok; t.advance()) {
+      const int kb1 = t.kb1();
+      if ((turn++ & 1) != group) continue;  // the other group's tile
+      const int f = tb.first[t.ai], c = tokens_of(t);
+      // scales of the weights: lane l holds those of K block kb0 + l, of 32 at a time
+      const int64_t so = ((int64_t)tb.expert[t.ai] * tiles + t.n) * nb + lane;
+      float w0s = 0.f, w1s = 0.f;
+      auto weight_scales = [&](int kb) {
+        w0s = kb + lane < kb1 ? __ldg((UP ? a.s_gate : a.s_down) + so + kb) : 0.f;
+        if (UP) w1s = kb + lane < kb1 ? __ldg(a.s_up + so + kb) : 0.f;
+      };
+      weight_scales(t.kb0);
+      const float route_w = !UP && lane < c ? __ldcg(a.w + tb.slots[f + lane]) : 0.f;
+      float acc[UP ? 2 : 1][2][16] = {};
+      // Two K blocks at a time where there are two: one round of waits and TMEM loads for both.
 #pragma unroll 1
-      for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-        const int b = it % kBufs, i = it % kScaleSlots, l = kb - t.kb0 & 31;
-        if (l == 0 && kb > t.kb0) weight_scales(t, kb, w0s, w1s);
-        const float w0 = __shfl_sync(0xffffffffu, w0s, l), w1 = UP ? __shfl_sync(0xffffffffu, w1s, l) : 0.f;
-        if (!mbar_wait_inline(sfull_bar(i), (it / kScaleSlots) & 1u, abort_flag, a.err) ||
-            !mbar_wait_inline(tfull_bar(b), (it / kBufs) & 1u, abort_flag, a.err)) {
+      for (int kb = t.kb0; kb < kb1;) {
+        const int l = kb - t.kb0 & 31, two = l < 31 && kb + 1 < kb1;
+        if (l == 0 && kb > t.kb0) weight_scales(kb);
+        const uint32_t itl = it + two;
+        const int b0 = group * kGroupBufs + it % kGroupBufs, b1 = group * kGroupBufs + itl % kGroupBufs;
+        const int i0 = group * kGroupSlots + it % kGroupSlots, i1 = group * kGroupSlots + itl % kGroupSlots;
+        if (!mbar_wait_inline(sfull_bar(i0), it / kGroupSlots & 1u, abort_flag, a.err) ||
+            !mbar_wait_inline(sfull_bar(i1), itl / kGroupSlots & 1u, abort_flag, a.err) ||
+            !mbar_wait_inline(tfull_bar(b0), it / kGroupBufs & 1u, abort_flag, a.err) ||
+            !mbar_wait_inline(tfull_bar(b1), itl / kGroupBufs & 1u, abort_flag, a.err)) {
           ok = false;
           break;
         }
         fence_after();
+        const float w00 = __shfl_sync(0xffffffffu, w0s, l), w01 = __shfl_sync(0xffffffffu, w0s, l + two);
+        const float w10 = UP ? __shfl_sync(0xffffffffu, w1s, l) : 0.f;
+        const float w11 = UP ? __shfl_sync(0xffffffffu, w1s, l + two) : 0.f;
+        const uint32_t t0 = my_tmem + b0 * kBufCols, t1 = my_tmem + b1 * kBufCols;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          if (need >> g & 1u) {
-            uint32_t v[UP ? 2 : 1][16];
-            tmem_ld16(my_tmem + b * kBufCols + g * 16, v[0]);
-            if constexpr (UP) tmem_ld16(my_tmem + b * kBufCols + 64 + g * 16, v[UP ? 1 : 0]);
-            float4 sc[4];
+        for (int g = 0; g < 2; ++g) {
+          if (g == 0 || c > 16) {
+            uint32_t v[2][UP ? 2 : 1][16];
+            tmem_ld16(t0 + g * 16, v[0][0]);
+            if constexpr (UP) tmem_ld16(t0 + kMaxTokens + g * 16, v[0][UP ? 1 : 0]);
+            if (two) {
+              tmem_ld16(t1 + g * 16, v[1][0]);
+              if constexpr (UP) tmem_ld16(t1 + kMaxTokens + g * 16, v[1][UP ? 1 : 0]);
+            }
+            auto add = [&](const uint32_t (&u)[UP ? 2 : 1][16], const float* sc, float f0, float f1) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) sc[q] = *reinterpret_cast<const float4*>(&scales[i][g * 16 + 4 * q]);
+              for (int q = 0; q < 4; ++q) {
+                const float4 s = *reinterpret_cast<const float4*>(sc + g * 16 + 4 * q);
+                const float s4[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  acc[0][g][4 * q + j] = fmaf(__uint_as_float(u[0][4 * q + j]), s4[j] * f0, acc[0][g][4 * q + j]);
+                  if constexpr (UP)
+                    acc[UP ? 1 : 0][g][4 * q + j] =
+                        fmaf(__uint_as_float(u[UP ? 1 : 0][4 * q + j]), s4[j] * f1, acc[UP ? 1 : 0][g][4 * q + j]);
+                }
+              }
+            };
             tmem_wait();
-#pragma unroll
-            for (int q = 0; q < 16; ++q) {
-              const float s4 = reinterpret_cast<const float*>(&sc[q >> 2])[q & 3];
-              acc[0][g][q] = fmaf(__uint_as_float(v[0][q]), s4 * w0, acc[0][g][q]);
-              if constexpr (UP)
-                acc[UP ? 1 : 0][g][q] = fmaf(__uint_as_float(v[UP ? 1 : 0][q]), s4 * w1, acc[UP ? 1 : 0][g][q]);
+            pin(v[0][0]), pin(v[0][UP ? 1 : 0]);
+            add(v[0], scales[i0], w00, w10);
+            if (two) {
+              pin(v[1][0]), pin(v[1][UP ? 1 : 0]);
+              add(v[1], scales[i1], w01, w11);
             }
           }
         }
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(tempty_bar(b)), mbar_arrive(sempty_bar(i));
+        if (lane == 0) {
+          mbar_arrive(tempty_bar(b0)), mbar_arrive(sempty_bar(i0));
+          if (two) mbar_arrive(tempty_bar(b1)), mbar_arrive(sempty_bar(i1));
+        }
+        kb += 1 + two;
+        it += 1 + two;
       }
       if (!ok) break;
-      if constexpr (UP) {
-        if (parts > 1) {
-          // Partial sums along K: the last of the tile's CTAs adds them in order.
-          const int tile = t.ai * tiles + t.n;
-          float* mine = a.partial + ((int64_t)tile * parts + t.part) * kFewPartialCols * 256 + row;
-          const int64_t stride = (int64_t)kFewPartialCols * 256;
+      // this thread's sums of columns [16 g, c) and on, a column after the other
+      auto put = [&](float* to, int g, const float (&v)[16], const float (&v2)[16]) {
 #pragma unroll
-          for (int i = 0; i < kFewPartialCols; ++i)
-            if (used >> i & 1) mine[i * 256] = acc[0][0][i], mine[i * 256 + 128] = acc[UP ? 1 : 0][0][i];
+        for (int i = 0; i < 16; ++i)
+          if (g * 16 + i < c) {
+            to[i * kSums] = v[i];
+            if (UP) to[i * kSums + 128] = v2[i];
+          }
+      };
+      // What becomes of the four sums (UP: of gate and of up) that a lane has of slot i: h, quantised, or d.
+      const int col = t.n * 128 + lane * 4;
+      const bool in = col < N;
+      auto finish = [&](int i, const float4& g, const float4& p) {
+        if constexpr (UP) {
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (in) v = make_float4(g.x * silu_ref(p.x), g.y * silu_ref(p.y), g.z * silu_ref(p.z), g.w * silu_ref(p.w));
+          const BlockScale s = block_scale(__reduce_max_sync(
+              0xffffffffu, max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)))));
+          const int64_t r = tb.row[t.ai] + i;
+          if (in)
+            *reinterpret_cast<uint32_t*>(a.hq + r * a.F + col) =
+                e4m3x4(v.x * s.inv, v.y * s.inv, v.z * s.inv, v.w * s.inv);
+          if (lane == 0) a.hs[(int64_t)t.n * a.h_rows + r] = s.scale;
+        } else {
+          const float r = __shfl_sync(0xffffffffu, route_w, i);
+          if (in)
+            *reinterpret_cast<float4*>(a.d + (int64_t)tb.slots[f + i] * a.H + col) =
+                make_float4(g.x * r, g.y * r, g.z * r, g.w * r);
+        }
+      };
+      if (kb1 - t.kb0 < nb) {
+        // A divided tile: its partial sums go to this CTA's place, the last CTA of the
+        // tile adds all of them in order.  A CTA has two divided tiles at most, the
+        // one its run begins in and the one it ends in.
+        const int total = tb.entries * tiles * nb, tile = t.ai * tiles + t.n, from = tile * nb;
+        const int cta0 = Walk::cta_of(from, total), cta1 = Walk::cta_of(from + nb - 1, total);
+        auto place = [&](int cta) {
+          return a.partial + (2 * cta + (Walk::start(cta, total) >= from ? 0 : 1)) * a.partial_stride;
+        };
+        float* mine = place(blockIdx.x) + row;
+        put(mine, 0, acc[0][0], acc[UP ? 1 : 0][0]);
+        if (c > 16) put(mine + 16 * kSums, 1, acc[0][1], acc[UP ? 1 : 0][1]);
+        __threadfence();
+        meet();
+        if (!ok) break;
+        if (quad == 0 && lane == 0) {
+          last_word[group] = atomicAdd(a.count + (UP ? 0 : a.n_count / 2) + tile, 1) == cta1 - cta0;
           __threadfence();
-          meet();
-          if (!ok) break;
-          if (warp == 4 && lane == 0) {
-            last_word = atomicAdd(a.count + tile, 1) == parts - 1;
-            __threadfence();
-          }
-          meet();
-          if (!ok) break;
-          if (!*reinterpret_cast<volatile int*>(&last_word)) continue;
-          const float* all = a.partial + (int64_t)tile * parts * stride + row;
-#pragma unroll
-          for (int i = 0; i < kFewPartialCols; ++i)
-            if (used >> i & 1) {
-              float g = 0.f, up = 0.f;
-              for (int q = 0; q < parts; ++q) {
-                g += __ldcg(all + q * stride + i * 256);
-                up += __ldcg(all + q * stride + i * 256 + 128);
-              }
-              acc[0][0][i] = g, acc[UP ? 1 : 0][0][i] = up;
-            }
         }
-        // gate and up of 16 used columns at a time to shared memory; then a warp a slot
-        // computes its 128 values of h, which share a scale
-        const int col = t.n * 128 + lane * 4;
-        const bool in = col < a.F;
-        for (int c0 = 0; c0 < __popcll(used) && ok; c0 += 16) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            if (need >> g & 1u) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int at = __popcll(used & ((1ull << (g * 16 + i)) - 1ull)) - c0;  // place among the used ones
-                if ((used >> (g * 16 + i) & 1) && at >= 0 && at < 16) {
-                  hbuf[at * 256 + row] = acc[0][g][i];
-                  hbuf[at * 256 + 128 + row] = acc[UP ? 1 : 0][g][i];
-                }
-              }
+        meet();
+        if (!ok) break;
+        if (!*reinterpret_cast<volatile int*>(&last_word[group])) continue;
+        for (int i = quad; i < c; i += 4) {
+          float4 g = make_float4(0.f, 0.f, 0.f, 0.f), p = g;
+#pragma unroll 4
+          for (int cta = cta0; cta <= cta1; ++cta) {
+            const float4* q = reinterpret_cast<const float4*>(place(cta) + i * kSums) + lane;
+            const float4 u = __ldcg(q);
+            g = make_float4(g.x + u.x, g.y + u.y, g.z + u.z, g.w + u.w);
+            if (UP) {
+              const float4 v = __ldcg(q + 32);
+              p = make_float4(p.x + v.x, p.y + v.y, p.z + v.z, p.w + v.w);
             }
-          meet();
-          if (!ok) break;
-          for (int i = quad; i < c; i += 4) {
-            const int at = __popcll(used & ((1ull << tb.tokens[f + i]) - 1ull)) - c0;
-            if (at < 0 || at >= 16) continue;
-            const float4 g = *reinterpret_cast<const float4*>(hbuf + at * 256 + lane * 4);
-            const float4 p = *reinterpret_cast<const float4*>(hbuf + at * 256 + 128 + lane * 4);
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (in) v = make_float4(g.x * silu_ref(p.x), g.y * silu_ref(p.y), g.z * silu_ref(p.z), g.w * silu_ref(p.w));
-            const BlockScale s = block_scale(__reduce_max_sync(
-                0xffffffffu, max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)))));
-            const int64_t r = tb.row[t.ai] + i;
-            if (in)
-              *reinterpret_cast<uint32_t*>(a.hq + r * a.F + col) =
-                  e4m3x4(v.x * s.inv, v.y * s.inv, v.z * s.inv, v.w * s.inv);
-            if (lane == 0) a.hs[(int64_t)t.n * a.h_rows + r] = s.scale;
           }
-          meet();  // before the next values
+          finish(i, g, p);
         }
-      } else if (t.n * 128 + quad * 32 < a.H) {  // H is a multiple of 16: a warp may be cut
-        const bool in = t.n * 128 + row < a.H;
-        float* d = a.d + ((int64_t)t.part * n) * a.H + t.n * 128 + row;
+      } else {
+        // 16 columns at a time through shared memory: a warp then has the 128 sums of a slot
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          if (g * 16 >= c) break;
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (g * 16 + i < c) {
-              const float w = __shfl_sync(0xffffffffu, g < 2 ? r0 : r1, (g & 1) * 16 + i);
-              if (in) d[(int64_t)tb.slots[f + g * 16 + i] * a.H] = acc[0][g][i] * w;
+        for (int g = 0; g < 2; ++g) {
+          if (g * 16 < c && ok) {
+            put(sums_buf + row, g, acc[0][g], acc[UP ? 1 : 0][g]);
+            meet();
+            if (!ok) break;
+#pragma unroll 1
+            for (int i = quad; i < min(16, c - g * 16); i += 4) {
+              const float4* q = reinterpret_cast<const float4*>(sums_buf + i * kSums) + lane;
+              finish(g * 16 + i, q[0], q[UP ? 32 : 0]);
             }
+            meet();  // before the next values
+          }
         }
       }
     }
@@ -791,46 +915,31 @@ static int few_map(CUtensorMap* m, const void* base, int64_t E, int64_t R, int64
   return FRANK_OK;
 }
 
-// 227 KB an SM less the static tables; the rest is the ring and UP's values of h.
-constexpr size_t kFewSmem = 232448 - 12288;
+// 227 KB an SM less the static tables; the rest is the ring and the epilogue's sums.
+constexpr size_t kFewSmem = 232448 - 13312;
 
 template <bool UP>
 static int launch_few_product(const FewMaps& maps, const FewArgs& a, cudaStream_t st) {
-  const int box = tile_tokens(a.T);
-  const uint32_t stage = (UP ? 2 : 1) * kTile + box * kQB;
-  const size_t hbuf = UP ? 16 * 256 * 4 : 0;
-  const int fit = (int)((kFewSmem - 1024 - hbuf) / stage), stages = fit < kMaxStages ? fit : kMaxStages;
+  const uint32_t stage = (UP ? 2 : 1) * kTile + tile_tokens(a.T) * kQB;
+  const size_t sums = 2 * 16 * (UP ? 256 : 128) * 4;
+  const int fit = (int)((kFewSmem - 1024 - sums) / stage), stages = fit < kMaxStages ? fit : kMaxStages;
   FRANK_CUDA_TRY(cudaFuncSetAttribute(few_product_kernel<UP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)kFewSmem));
   FRANK_CUDA_TRY(launch_chained(few_product_kernel<UP>, dim3(num_sms()), dim3(kFewThreads),
-                                1024 + hbuf + (size_t)stages * stage, st, 1, maps, a, stages, stage));
+                                1024 + sums + (size_t)stages * stage, st, 1, maps, a, stages, stage));
   FRANK_LAUNCH_CHECK();
   return FRANK_OK;
 }
 
-// The combine adds `parts` partial sums a slot: where the tiles of H alone cannot
-// keep the SMs busy, F is divided, into parts of 8 K blocks or more.
-int few_parts(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
-  const int64_t tiles = (k * T < E ? k * T : E) * q_blocks(H), most = q_blocks(F) / 8;
-  if (tiles <= 0) return 1;
-  const int64_t want = (4 * num_sms() + tiles - 1) / tiles;
-  const int64_t parts = want < most ? want : most;
-  return (int)(parts < 1 ? 1 : parts > kFewMaxParts ? kFewMaxParts : parts);
+// Tiles of both products, and their counters: an expert's slots may need several entries.
+int64_t few_counts(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
+  const int64_t n = k * T, entries = (n < E ? n : E) + n / 16;
+  return 2 * entries * (q_blocks(F) > q_blocks(H) ? q_blocks(F) : q_blocks(H));
 }
 
-// The gate/up tiles of one or two tokens leave SMs idle (one SM draws 51 GB/s of
-// weights through the MMA): K is divided then.
-int few_up_parts(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
-  const int64_t tiles = (k * T < E ? k * T : E) * q_blocks(F), most = q_blocks(H) / 4;
-  if (tiles <= 0 || T > kFewPartialCols) return 1;
-  const int64_t want = num_sms() / tiles, parts = want < most ? want : most;
-  return (int)(parts < 1 ? 1 : parts > kFewMaxParts ? kFewMaxParts : parts);
-}
-
-// Floats of the partial sums, and counters, of few_up_parts > 1.
-int64_t few_partial_tiles(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
-  return few_up_parts(T, E, k, H, F) > 1 ? (k * T < E ? k * T : E) * q_blocks(F) : 0;
-}
+// Floats of a CTA's place for partial sums; two places a CTA.
+int64_t few_partial_stride(int64_t T) { return tile_tokens((int)T) * 256; }
+int64_t few_partials(int64_t T) { return 2 * num_sms() * few_partial_stride(T); }
 
 int64_t few_h_rows(int64_t T, int64_t E, int64_t k) {
   const int64_t n = k * T;  // up to 15 rows of padding for each expert that has slots
@@ -840,8 +949,8 @@ int64_t few_h_rows(int64_t T, int64_t E, int64_t k) {
 int launch_few_experts(const FewArgs& args, int32_t* err, cudaStream_t st) {
   FewArgs a = args;
   a.err = device_error_word();
-  a.up_parts = few_up_parts(a.T, a.E, a.k, a.H, a.F);
-  a.parts = few_parts(a.T, a.E, a.k, a.H, a.F);
+  a.partial_stride = few_partial_stride(a.T);
+  a.n_count = (int)few_counts(a.T, a.E, a.k, a.H, a.F);
   a.h_rows = (int)few_h_rows(a.T, a.E, a.k);
   if (err != nullptr) {
     FRANK_CUDA_TRY(launch_chained(few_check_ids_kernel, dim3(1), dim3(256), 0, st, 1, a.ids, a.k * a.T, a.E, err));
@@ -852,10 +961,8 @@ int launch_few_experts(const FewArgs& args, int32_t* err, cudaStream_t st) {
   FRANK_TRY(few_map(&up.w2, a.w_up, a.E, a.F, a.H, 128, true));
   FRANK_TRY(few_map(&down.w, a.w_down, a.E, a.H, a.F, 128, true));
   down.w2 = down.w;
-  for (int i = 0; i < 3; ++i) {
-    FRANK_TRY(few_map(&up.x[i], a.xq, 1, a.T, a.H, 16u << i, false));
-    FRANK_TRY(few_map(&down.x[i], a.hq, 1, a.h_rows, a.F, 16u << i, false));
-  }
+  for (int i = 0; i < 2; ++i) FRANK_TRY(few_map(&down.x[i], a.hq, 1, a.h_rows, a.F, 16u << i, false));
+  up.x[0] = up.x[1] = down.x[0];  // not read
   FRANK_TRY(launch_few_product<true>(up, a, st));
   return launch_few_product<false>(down, a, st);
 }

@@ -16,13 +16,12 @@ inline int64_t q_blocks(int64_t n) { return (n + kQB - 1) / kQB; }
 // Arguments of one pass over rows of H values (norm.cu): each row is read
 // once, kept in registers and leaves in every form that is asked for.
 struct NormRows {
-  // source: y [T, H], or the sum over k slots of d (fp32 rows at slot_pos[j*T+t], or j*T+t), each the sum of
-  // `parts` rows k*T apart
+  // source: y [T, H], or the sum over k slots of d (fp32 rows at slot_pos[j*T+t], or j*T+t)
   int y_dtype = FRANK_F32;
   const void* y = nullptr;
   const float* d = nullptr;
   const int32_t* slot_pos = nullptr;
-  int k = 0, parts = 1;
+  int k = 0;
   // v = residual_scale * residual + gate * (post_w ? rms_norm(v, post_w) : v)
   const float* post_w = nullptr;
   float eps = 0.f;

@@ -7,7 +7,7 @@ namespace frank {
 
 constexpr int kFewMaxE = (int)kFp8MaxE;
 constexpr int kFewMaxT = 64, kFewMaxSlots = 512;
-constexpr int kFewMaxParts = 4, kFewPartialCols = 4;  // divisions of K; tokens where gate/up is divided
+constexpr int64_t kFewMaxBlocksH = 128, kFewMaxBlocksF = 2048;  // their K blocks are counted in 32 bits
 
 struct FewRoute {
   const void* x;  // [T, H]
@@ -32,18 +32,19 @@ struct FewArgs {
   const float* xs;
   uint8_t* hq;  // [few_h_rows, F], the slots sorted by expert, each expert at a multiple of 16
   float* hs;    // [ceil(F/128), few_h_rows]
-  float* d;     // [few_parts, k T, H]
+  float* d;     // [k T, H]
   const float* w;
   const int32_t* ids;
   int T, E, k, H, F;
-  float* partial;  // [few_partial_tiles, parts, kFewPartialCols, 256]
-  int32_t* count;  // [few_partial_tiles]
-  int up_parts, parts, h_rows;  // set by launch_few_experts
+  float* partial;  // [few_partials]
+  int32_t* count;  // [few_counts], zero; set by launch_few_experts:
+  int64_t partial_stride;
+  int n_count, h_rows;
   int32_t* err;       // device error word
 };
 
-int few_parts(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F);
-int64_t few_partial_tiles(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F);
+int64_t few_counts(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F);
+int64_t few_partials(int64_t T);
 int64_t few_h_rows(int64_t T, int64_t E, int64_t k);
 int launch_few_route(const FewRoute& a, cudaStream_t st);
 int launch_few_experts(const FewArgs& a, int32_t* err, cudaStream_t st);

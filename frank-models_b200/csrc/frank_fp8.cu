@@ -33,7 +33,9 @@ struct Fp8Weights {
 };
 
 // A few tokens: the weights bound the call, and few_fp8.cu reads them once.
-static bool few_tokens(int64_t T, int64_t k) { return T <= kFewMaxT && k * T <= kFewMaxSlots; }
+static bool few_tokens(int64_t T, int64_t k, int64_t H, int64_t F) {
+  return T <= kFewMaxT && k * T <= kFewMaxSlots && q_blocks(H) <= kFewMaxBlocksH && q_blocks(F) <= kFewMaxBlocksF;
+}
 
 // Workspace of one call; the same for a block, its experts and its sub-layer
 // (which adds the normalised tokens).
@@ -50,7 +52,7 @@ struct Fp8MoeWs {
   uint8_t* hq;            // [n, F]
   float* hs;              // [F/128, n]
   float* d;               // [n, H]
-  float* partial;         // a few tokens: partial sums of gate/up, and their counters
+  float* partial;         // a few tokens: partial sums of divided tiles, and their counters
   int32_t* count;
   float* logits;
   void* perm;
@@ -69,16 +71,15 @@ static size_t fp8_moe_layout(int64_t T, int64_t H, int64_t F, int64_t E, int64_t
   l.slot_pos = c.take<int32_t>(n);
   l.wsorted = c.take<float>(n);
   l.xn = c.take<__nv_bfloat16>(T * H);
-  const bool few = few_tokens(T, k);
-  const int64_t h_rows = few ? few_h_rows(T, E, k) : n, parts = few ? few_parts(T, E, k, H, F) : 1;
+  const bool few = few_tokens(T, k, H, F);
+  const int64_t h_rows = few ? few_h_rows(T, E, k) : n;
   l.xq = c.take<uint8_t>(n * H);
   l.xs = c.take<float>((few ? kFewMaxT : n) * q_blocks(H));
   l.hq = c.take<uint8_t>(h_rows * F);
   l.hs = c.take<float>(h_rows * q_blocks(F));
-  l.d = c.take<float>(parts * n * H);
-  const int64_t tiles = few ? few_partial_tiles(T, E, k, H, F) : 0;
-  l.partial = c.take<float>(tiles * kFewMaxParts * kFewPartialCols * 256);
-  l.count = c.take<int32_t>(tiles);
+  l.d = c.take<float>(n * H);
+  l.partial = c.take<float>(few ? few_partials(T) : 0);
+  l.count = c.take<int32_t>(few ? few_counts(T, E, k, H, F) : 0);
   l.logits = c.take<float>(router_scratch_bytes(FRANK_BF16, T, H, E) / sizeof(float) + 1);
   l.perm_bytes = permute_workspace_size(n, E);
   l.perm = c.take<char>(l.perm_bytes);
@@ -154,7 +155,7 @@ static FewRoute few_route(int x_dtype, const void* x, const float* norm_w, float
   r.w = w;
   r.ids = ids;
   r.count = L.count;
-  r.n_count = (int)few_partial_tiles(T, E, k, H, F);
+  r.n_count = (int)few_counts(T, E, k, H, F);
   return r;
 }
 
@@ -162,7 +163,7 @@ static FewRoute few_route(int x_dtype, const void* x, const float* norm_w, float
 static int run_experts(const void* x, const float* w, const int32_t* ids, const Fp8Weights& W, int64_t T, int64_t E,
                        int64_t k, int64_t H, int64_t F, int32_t* err, const Fp8MoeWs& L, cudaStream_t st) {
   const int64_t n = k * T;
-  if (few_tokens(T, k)) {
+  if (few_tokens(T, k, H, F)) {
     FRANK_TRY(launch_few_route(few_route(FRANK_BF16, x, nullptr, 0.f, FRANK_F32, nullptr, T, E, k, H, F, 0, nullptr,
                                          nullptr, L), st));
     return launch_few_experts(few_args(W, T, E, k, H, F, w, ids, L), err, st);
@@ -207,8 +208,7 @@ static NormRows combine_of(const Fp8MoeWs& L, int64_t T, int64_t E, int64_t k, i
                            void* out) {
   NormRows a;
   a.d = L.d;
-  a.slot_pos = few_tokens(T, k) ? nullptr : L.slot_pos;
-  a.parts = few_tokens(T, k) ? few_parts(T, E, k, H, F) : 1;
+  a.slot_pos = few_tokens(T, k, H, F) ? nullptr : L.slot_pos;
   a.k = (int)k;
   a.T = T;
   a.H = H;
@@ -228,7 +228,7 @@ static int route_and_run(int x_dtype, const void* x, const float* norm_w, float 
   }
   FRANK_TRY(check_float_dtype(wr_dtype, "fp8_moe router"));
   FRANK_CHECK_ARG(wr != nullptr, "fp8_moe router: null pointer");
-  if (few_tokens(T, k)) {
+  if (few_tokens(T, k, H, F)) {
     FRANK_TRY(launch_few_route(
         few_route(x_dtype, x, norm_w, eps, wr_dtype, wr, T, E, k, H, F, normalize, w, ids, L), st));
     return launch_few_experts(few_args(W, T, E, k, H, F, w, ids, L), nullptr, st);

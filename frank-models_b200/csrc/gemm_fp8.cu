@@ -123,6 +123,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// After the wait: keeps what uses the values behind it.
+__device__ __forceinline__ void pin(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
 
 // acc[0..31] += v[0..31] * s, two lanes of the pair of floats at a time
 __device__ __forceinline__ void scale_add(float* acc, const uint32_t (&v)[32], float s) {
@@ -416,11 +421,13 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
           tmem_ld32(ta + col0, v0);
           tmem_ld32(ta + col0 + 32, v1);
           tmem_wait();
+          pin(v0), pin(v1);
           scale_add(acc, v0, s0);
           tmem_ld32(ta + col1, v0);
           scale_add(acc + 32, v1, s0);
           tmem_ld32(ta + col1 + 32, v1);
           tmem_wait();
+          pin(v0), pin(v1);
         }
         fence_before();
         __syncwarp();

@@ -89,26 +89,23 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormRows a) {
   if (SLOTS) {
     // rows in order, the loads of several at a time
     constexpr int kAhead = V <= 2 ? 4 : V <= 4 ? 2 : 1;
-    const int rows = a.k * a.parts;
-    for (int j0 = 0; j0 < rows; j0 += kAhead) {
+    for (int j0 = 0; j0 < a.k; j0 += kAhead) {
       float4 u[kAhead][V];
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
-        const int j = (j0 + q) / a.parts, part = j0 + q - j * a.parts;
-        const int64_t s = (int64_t)j * a.T + t;
+        const int64_t s = (int64_t)(j0 + q) * a.T + t;
         const float* row = a.d;
-        if (j0 + q < rows)
-          row += ((int64_t)part * a.k * a.T + (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s)) * H;
+        if (j0 + q < a.k) row += (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * H;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const int64_t h = 4 * (int64_t)(tid + i * GS);
           u[q][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (h < H && j0 + q < rows) u[q][i] = *reinterpret_cast<const float4*>(row + h);
+          if (h < H && j0 + q < a.k) u[q][i] = *reinterpret_cast<const float4*>(row + h);
         }
       }
 #pragma unroll
       for (int q = 0; q < kAhead; ++q)
-        if (j0 + q < rows) {
+        if (j0 + q < a.k) {
 #pragma unroll
           for (int i = 0; i < V; ++i) {
             v[i].x += u[q][i].x;

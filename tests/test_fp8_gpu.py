@@ -298,7 +298,7 @@ def test_experts_ids_out_of_range():
 
 BLOCKS = [(1, 2048, 768, 128, 8, False), (1, 256, 128, 4, 4, True), (8, 512, 400, 64, 8, True), (3, 528, 272, 9, 2, True),
           (47, 256, 144, 128, 8, True), (64, 1024, 256, 160, 6, False), (5, 4096, 1040, 8, 2, False),
-          (130, 272, 128, 16, 4, True), (1000, 256, 256, 8, 2, False), (17, 48, 80, 256, 32, True)]
+          (5, 4096, 1024, 8, 2, True), (20, 2048, 2064, 6, 2, False), (130, 272, 128, 16, 4, True), (1000, 256, 256, 8, 2, False), (17, 48, 80, 256, 32, True)]
 
 
 @pytest.mark.parametrize("T,H,F,E,k,normalize", BLOCKS)
