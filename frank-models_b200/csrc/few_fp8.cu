@@ -446,6 +446,15 @@ struct Walk {
   }
 };
 
+// A stage of the ring and the parity of its barriers.
+struct Ring {
+  int s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == stages) s = 0, phase ^= 1u;
+  }
+};
+
 // K blocks of the tiles of each epilogue group so far; tiles alternate.
 struct Turns {
   uint32_t mine = 0, other = 0;
@@ -532,62 +541,62 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
       // ------------------------------------------------ TMA producer --
       uint64_t policy;
       asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-      // The ring is filled with weights first; DOWN's rows of h follow, at once or, for the
-      // first stages, when they are there.
-      Walk w = walk, fw = walk;  // of the weights, of h
-      int kb = w.kb0, fkb = w.kb0;
-      uint32_t it = 0, fit = 0;
-      bool ok = true, waited = UP;
-      while (fw.more() && ok) {
-        if (w.more() && (waited ? it == fit : it < (uint32_t)stages)) {
-          const int s = it % stages;
-          if (!mbar_wait_inline(empty_bar(s), ((it / stages) & 1u) ^ 1u, abort_flag, a.err)) {
+      Ring r;
+      bool ok = true;
+      // One K block: the weights, and DOWN's rows of h.
+      auto weights = [&](int e, int n, int kb, uint32_t x_bytes) {
+        const uint32_t st = smem_u32(smem + r.s * stage_bytes);
+        mbar_expect_tx(full_bar(r.s), kWeights + x_bytes);
+        load_weights(st, &maps.w, kb * kQB, n * 128, e, full_bar(r.s), policy);
+        if (UP) load_weights(st + kTile, &maps.w2, kb * kQB, n * 128, e, full_bar(r.s), policy);
+      };
+      auto rows = [&](int s, int box, int kb, int row) {
+        load_2d(smem_u32(smem + s * stage_bytes) + kWeights, &maps.x[box], kb * kQB, row, full_bar(s));
+      };
+      Walk t = walk;
+      int kb = t.kb0;
+      if (!UP) {
+        // the ring is filled with weights, its rows of h follow when they are there
+        int n = 0;
+        for (; t.more() && n < stages;) {
+          weights(tb.expert[t.ai], t.n, kb, tokens_of(t) <= 16 ? 16 * kQB : 32 * kQB);
+          r.next(stages);
+          ++n;
+          if (++kb == t.kb1()) t.advance(), kb = 0;
+        }
+        pdl_wait();
+        Walk u = walk;
+        for (int m = 0, ukb = u.kb0; m < n; ++m) {
+          rows(m, tokens_of(u) <= 16 ? 0 : 1, ukb, tb.row[u.ai]);
+          if (++ukb == u.kb1()) u.advance(), ukb = 0;
+        }
+      }
+      for (; t.more() && ok; t.advance(), kb = 0) {
+        const int e = tb.expert[t.ai], box = tokens_of(t) <= 16 ? 0 : 1, row = tb.row[t.ai];
+        for (const int kb1 = t.kb1(); kb < kb1; ++kb, r.next(stages)) {
+          if (!mbar_wait_inline(empty_bar(r.s), r.phase ^ 1u, abort_flag, a.err)) {
             ok = false;
             break;
           }
-          const int e = tb.expert[w.ai];
-          const uint32_t st = smem_u32(smem + s * stage_bytes);
-          mbar_expect_tx(full_bar(s), kWeights + (UP ? 0 : tokens_of(w) <= 16 ? 16 * kQB : 32 * kQB));
-          load_weights(st, &maps.w, kb * kQB, w.n * 128, e, full_bar(s), policy);
-          if (UP) load_weights(st + kTile, &maps.w2, kb * kQB, w.n * 128, e, full_bar(s), policy);
-          ++it;
-          if (++kb == w.kb1()) {
-            w.advance();
-            kb = 0;
-          }
-          if (!waited) continue;
-        }
-        if (!waited) {
-          pdl_wait();
-          waited = true;
-        }
-        if (!UP) {
-          const int s = fit % stages;
-          load_2d(smem_u32(smem + s * stage_bytes) + kWeights, &maps.x[tokens_of(fw) <= 16 ? 0 : 1], fkb * kQB,
-                  tb.row[fw.ai], full_bar(s));
-        }
-        ++fit;
-        if (++fkb == fw.kb1()) {
-          fw.advance();
-          fkb = 0;
+          weights(e, t.n, kb, UP ? 0 : (16u << box) * kQB);
+          if (!UP) rows(r.s, box, kb, row);
         }
       }
-      if (!waited) pdl_wait();
     }
   } else if (warp == 1) {
     if (lane == 0) {
       // -------------------------------------------------- MMA issuer --
-      uint32_t it = 0;
+      Ring r;
       Turns turn;
       bool ok = true;
       for (Walk t = walk; t.more() && ok; t.advance(), turn.next_tile()) {
         // kind::f8f6f4: D fp32, A and B e4m3, N >> 3 at [17,23), M >> 4 at [24,29)
         const uint32_t cols = tokens_of(t) <= 16 ? 16 : 32;
         const uint32_t idesc = (1u << 4) | (cols >> 3 << 17) | ((uint32_t)(128 >> 4) << 24);
-        for (int kb = t.kb0, kb1 = t.kb1(); kb < kb1; ++kb, ++it, ++turn.mine) {
-          const int s = it % stages, b = turn.buf();
+        for (int kb = t.kb0, kb1 = t.kb1(); kb < kb1; ++kb, r.next(stages), ++turn.mine) {
+          const int s = r.s, b = turn.buf();
           if (!mbar_wait_inline(tempty_bar(b), turn.buf_parity() ^ 1u, abort_flag, a.err) ||
-              !mbar_wait_inline(full_bar(s), (it / stages) & 1u, abort_flag, a.err)) {
+              !mbar_wait_inline(full_bar(s), r.phase, abort_flag, a.err)) {
             ok = false;
             break;
           }
@@ -631,32 +640,34 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
       // 16 bytes a lane, eight lanes a row, into the swizzled tile; three K blocks under way
       constexpr int kAhead = 3;
       const int r0 = lane >> 3, chunk = lane & 7;
-      uint32_t it = 0, done = 0;
+      uint32_t under_way = 0;
+      Ring r, first;  // of the next K block, of the oldest one under way
       int slots_under_way[kAhead] = {};  // their scale slots, the oldest first
       Turns turn;
       bool ok = true;
-      auto arrive = [&]() {  // K block `done` is in shared memory
+      auto arrive = [&]() {  // the oldest K block is in shared memory
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(full_bar(done % stages)), mbar_arrive(sfull_bar(slots_under_way[0]));
+        if (lane == 0) mbar_arrive(full_bar(first.s)), mbar_arrive(sfull_bar(slots_under_way[0]));
+        first.next(stages);
+        --under_way;
 #pragma unroll
         for (int i = 0; i + 1 < kAhead; ++i) slots_under_way[i] = slots_under_way[i + 1];
-        ++done;
       };
       for (Walk t = walk; t.more() && ok; t.advance(), turn.next_tile()) {
         const int c = tokens_of(t), *tok = tb.tokens + tb.first[t.ai];
         for (int kb = t.kb0, kb1 = t.kb1(); kb < kb1; ++kb, ++turn.mine) {
-          const int s = it % stages, i = turn.slot();
-          if (!mbar_wait_inline(empty_bar(s), ((it / stages) & 1u) ^ 1u, abort_flag, a.err) ||
+          const int s = r.s, i = turn.slot();
+          if (!mbar_wait_inline(empty_bar(s), r.phase ^ 1u, abort_flag, a.err) ||
               !mbar_wait_inline(sempty_bar(i), turn.slot_parity() ^ 1u, abort_flag, a.err)) {
             ok = false;
             break;
           }
           const uint32_t st = smem_u32(smem + s * stage_bytes) + kWeights;
           const int k = kb * kQB + chunk * 16;
-          for (int r = r0; r < c; r += 4) {
-            const uint8_t* src = a.xq + (int64_t)tok[r] * a.H + (k < a.H ? k : 0);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(st + r * kQB + ((chunk ^ (r & 7)) << 4)),
+          for (int q = r0; q < c; q += 4) {
+            const uint8_t* src = a.xq + (int64_t)tok[q] * a.H + (k < a.H ? k : 0);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(st + q * kQB + ((chunk ^ (q & 7)) << 4)),
                          "l"(src), "r"(k < a.H ? 16 : 0)
                          : "memory");
           }
@@ -667,16 +678,16 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
           asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
           for (int q = 0; q < kAhead; ++q)
-            if (q == (int)(it - done)) slots_under_way[q] = i;
-          ++it;
-          if (it - done >= kAhead) {
+            if (q == (int)under_way) slots_under_way[q] = i;
+          r.next(stages);
+          if (++under_way >= kAhead) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
             arrive();
           }
         }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
-      while (ok && done < it) arrive();
+      while (ok && under_way > 0) arrive();
     }
   } else {
     // ---------------------------------------------------- epilogue --
