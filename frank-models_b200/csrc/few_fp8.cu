@@ -796,7 +796,7 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
       auto finish = [&](int i, const float4& g, const float4& p) {
         if constexpr (UP) {
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (in) v = make_float4(g.x * silu_ref(p.x), g.y * silu_ref(p.y), g.z * silu_ref(p.z), g.w * silu_ref(p.w));
+          if (in) v = make_float4(g.x * silu(p.x), g.y * silu(p.y), g.z * silu(p.z), g.w * silu(p.w));
           const BlockScale s = block_scale(__reduce_max_sync(
               0xffffffffu, max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)))));
           const int64_t r = tb.row[t.ai] + i;
@@ -890,8 +890,8 @@ int launch_few_route(const FewRoute& a, cudaStream_t st) {
   const int nb = (a.H + kQB - 1) / kQB, slice = (nb + kRouteCtas - 1) / kRouteCtas * kQB;
   const size_t smem = (size_t)kRouteTok * slice * 4;
   const auto kern = a.E <= 128 ? few_route_kernel<4> : few_route_kernel<8>;
-  FRANK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)(kRouteTok * kNormMaxH / kRouteCtas * 4)));
+  static std::atomic<uint64_t> done[2];
+  FRANK_CUDA_TRY(allow_smem(done[a.E <= 128], kern, kRouteTok * kNormMaxH / kRouteCtas * 4));
   const dim3 grid((unsigned)((a.T + kRouteTok - 1) / kRouteTok * kRouteCtas));
   FRANK_CUDA_TRY(launch_chained(kern, grid, dim3(kRouteThreads), smem, st, kRouteCtas, a));
   FRANK_LAUNCH_CHECK();
@@ -934,8 +934,8 @@ static int launch_few_product(const FewMaps& maps, const FewArgs& a, cudaStream_
   const uint32_t stage = (UP ? 2 : 1) * kTile + tile_tokens(a.T) * kQB;
   const size_t sums = 2 * 16 * (UP ? 256 : 128) * 4;
   const int fit = (int)((kFewSmem - 1024 - sums) / stage), stages = fit < kMaxStages ? fit : kMaxStages;
-  FRANK_CUDA_TRY(cudaFuncSetAttribute(few_product_kernel<UP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)kFewSmem));
+  static std::atomic<uint64_t> done{0};
+  FRANK_CUDA_TRY(allow_smem(done, few_product_kernel<UP>, kFewSmem));
   FRANK_CUDA_TRY(launch_chained(few_product_kernel<UP>, dim3(num_sms()), dim3(kFewThreads),
                                 1024 + sums + (size_t)stages * stage, st, 1, maps, a, stages, stage));
   FRANK_LAUNCH_CHECK();

@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "frank_fp8.h"
 
@@ -16,10 +18,11 @@ inline int64_t q_blocks(int64_t n) { return (n + kQB - 1) / kQB; }
 // Arguments of one pass over rows of H values (norm.cu): each row is read
 // once, kept in registers and leaves in every form that is asked for.
 struct NormRows {
-  // source: y [T, H], or the sum over k slots of d (fp32 rows at slot_pos[j*T+t], or j*T+t)
+  // source: y [T, H], or the sum over k slots of d (rows at slot_pos[j*T+t], or j*T+t)
   int y_dtype = FRANK_F32;
   const void* y = nullptr;
-  const float* d = nullptr;
+  int d_dtype = FRANK_F32;
+  const void* d = nullptr;
   const int32_t* slot_pos = nullptr;
   int k = 0;
   // v = residual_scale * residual + gate * (post_w ? rms_norm(v, post_w) : v)
@@ -50,7 +53,7 @@ int launch_prepack_fp8(int in_dtype, const void* src, int64_t O, int64_t I, int6
 
 // Grouped product of 8-bit rows and weights (gemm_fp8.cu).
 //   PLAIN : out [rows, N] in out_dtype
-//   SCALE : out fp32 [rows, N], row r times wrow[r]
+//   SCALE : out [rows, N] in out_dtype, row r times wrow[r]
 //   SWIGLU: w = gate, w2 = up; h = gate * silu(up) quantised -> out e4m3 [rows, N], h_scale [ceil(N/128), rows]
 enum Fp8Mode { FP8_PLAIN = 0, FP8_SCALE = 1, FP8_SWIGLU = 2 };
 struct Fp8Gemm {
@@ -97,6 +100,9 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t amax) {
   return s;
 }
 
+// silu with CUDA's approximate division (2 ulp): 64 of them end a tile of a product.
+__device__ __forceinline__ float silu(float u) { return __fdividef(u, 1.0f + expf(-u)); }
+
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
@@ -119,6 +125,20 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" :::); }
 
 namespace frank {
+// Raises a kernel's limit of dynamic shared memory, once on each device (a call costs
+// about a microsecond); `done` is the kernel's own mask of devices.
+template <typename Kern>
+inline cudaError_t allow_smem(std::atomic<uint64_t>& done, Kern kern, size_t bytes) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_chained(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                                   unsigned cluster, Args... args) {

@@ -51,7 +51,7 @@ struct Fp8MoeWs {
   float* xs;              // [H/128, n]
   uint8_t* hq;            // [n, F]
   float* hs;              // [F/128, n]
-  float* d;               // [n, H]
+  void* d;                // [n, H], see d_dtype
   float* partial;         // a few tokens: partial sums of divided tiles, and their counters
   int32_t* count;
   float* logits;
@@ -77,7 +77,7 @@ static size_t fp8_moe_layout(int64_t T, int64_t H, int64_t F, int64_t E, int64_t
   l.xs = c.take<float>((few ? kFewMaxT : n) * q_blocks(H));
   l.hq = c.take<uint8_t>(h_rows * F);
   l.hs = c.take<float>(h_rows * q_blocks(F));
-  l.d = c.take<float>(n * H);
+  l.d = c.take<float>(n * H);  // enough for either type
   l.partial = c.take<float>(few ? few_partials(T) : 0);
   l.count = c.take<int32_t>(few ? few_counts(T, E, k, H, F) : 0);
   l.logits = c.take<float>(router_scratch_bytes(FRANK_BF16, T, H, E) / sizeof(float) + 1);
@@ -124,7 +124,7 @@ static FewArgs few_args(const Fp8Weights& W, int64_t T, int64_t E, int64_t k, in
   a.count = L.count;
   a.hq = L.hq;
   a.hs = L.hs;
-  a.d = L.d;
+  a.d = static_cast<float*>(L.d);
   a.w = w;
   a.ids = ids;
   a.T = (int)T;
@@ -159,8 +159,17 @@ static FewRoute few_route(int x_dtype, const void* x, const float* norm_w, float
   return r;
 }
 
+// The products of a prompt's slots leave in the type of the result: for a bf16 result each
+// slot is rounded once more (half a step of bf16 of its own share of the sum) and
+// the 2 k bytes a value written and read are halved, which end the tiles of a short
+// K: 271 -> 205 us for the down product of 65536 slots, 2048 from 768.  A few
+// tokens' slots and fp32 results stay in fp32.
+static int d_dtype(int y_dtype, int64_t T, int64_t k, int64_t H, int64_t F) {
+  return few_tokens(T, k, H, F) ? FRANK_F32 : y_dtype;
+}
+
 // Routed rows through the experts: L.d[r] = w * down(q(h)) for the expert-sorted rows r.
-static int run_experts(const void* x, const float* w, const int32_t* ids, const Fp8Weights& W, int64_t T, int64_t E,
+static int run_experts(int y_dtype, const void* x, const float* w, const int32_t* ids, const Fp8Weights& W, int64_t T, int64_t E,
                        int64_t k, int64_t H, int64_t F, int32_t* err, const Fp8MoeWs& L, cudaStream_t st) {
   const int64_t n = k * T;
   if (few_tokens(T, k, H, F)) {
@@ -199,7 +208,7 @@ static int run_experts(const void* x, const float* w, const int32_t* ids, const 
   d.N = H;
   d.K = F;
   d.wrow = L.wsorted;
-  d.out_dtype = FRANK_F32;
+  d.out_dtype = y_dtype;
   d.out = L.d;
   return launch_fp8_gemm(d, st);
 }
@@ -207,6 +216,7 @@ static int run_experts(const void* x, const float* w, const int32_t* ids, const 
 static NormRows combine_of(const Fp8MoeWs& L, int64_t T, int64_t E, int64_t k, int64_t H, int64_t F, int out_dtype,
                            void* out) {
   NormRows a;
+  a.d_dtype = d_dtype(out_dtype, T, k, H, F);
   a.d = L.d;
   a.slot_pos = few_tokens(T, k, H, F) ? nullptr : L.slot_pos;
   a.k = (int)k;
@@ -218,7 +228,7 @@ static NormRows combine_of(const Fp8MoeWs& L, int64_t T, int64_t E, int64_t k, i
 }
 
 // The block up to L.d: x [T, H] bf16, or with norm_w the residual it is normalised from.
-static int route_and_run(int x_dtype, const void* x, const float* norm_w, float eps, int wr_dtype, const void* wr,
+static int route_and_run(int y_dtype, int x_dtype, const void* x, const float* norm_w, float eps, int wr_dtype, const void* wr,
                          const Fp8Weights& W, int64_t T, int64_t E, int64_t k, int64_t H, int64_t F, int normalize,
                          float* w, int32_t* ids, const Fp8MoeWs& L, cudaStream_t st) {
   const __nv_bfloat16* wr3 = nullptr;
@@ -246,7 +256,7 @@ static int route_and_run(int x_dtype, const void* x, const float* norm_w, float 
     x = L.xn;
   }
   FRANK_TRY(launch_router_topk(FRANK_BF16, x, wr_dtype, wr, T, H, E, k, normalize, w, ids, L.logits, st, wr3));
-  return run_experts(x, w, ids, W, T, E, k, H, F, nullptr, L, st);
+  return run_experts(y_dtype, x, w, ids, W, T, E, k, H, F, nullptr, L, st);
 }
 
 static int check_gate(const char* what, const float* gate, int64_t gate_rows, int64_t T) {
@@ -330,6 +340,24 @@ int frank_fp8_matmul(const void* q, const float* scale, const void* w, const flo
   return launch_fp8_gemm(g, as_stream(stream));
 }
 
+size_t frank_fp8_linear_workspace_size(int64_t rows, int64_t K) {
+  return align_up((size_t)rows * K, 256) + align_up((size_t)rows * q_blocks(K) * 4, 256);
+}
+
+int frank_fp8_linear(int x_dtype, const void* x, const void* w, const float* w_scale, const int32_t* offsets,
+                     int64_t E, int64_t rows, int64_t N, int64_t K, int out_dtype, void* out, void* workspace,
+                     size_t ws_bytes, void* stream) {
+  if (rows == 0) return frank_fp8_matmul(nullptr, nullptr, w, w_scale, offsets, E, 0, N, K, out_dtype, out, stream);
+  if (rows > 0 && K > 0 && (workspace == nullptr || ws_bytes < frank_fp8_linear_workspace_size(rows, K))) {
+    set_error("fp8_linear: workspace %zu < %zu bytes", workspace ? ws_bytes : (size_t)0,
+              frank_fp8_linear_workspace_size(rows, K));
+    return FRANK_ENOSPC;
+  }
+  float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up((size_t)rows * K, 256));
+  FRANK_TRY(frank_quantize_fp8(x_dtype, x, rows, K, workspace, scale, stream));
+  return frank_fp8_matmul(workspace, scale, w, w_scale, offsets, E, rows, N, K, out_dtype, out, stream);
+}
+
 size_t frank_fp8_moe_workspace_size(int64_t T, int64_t H, int64_t F, int64_t E, int64_t k) {
   return fp8_moe_layout(T, H, F, E, k, nullptr, 0, nullptr);
 }
@@ -347,7 +375,7 @@ int frank_fp8_moe_experts(const void* x, const float* route_w, const int32_t* ro
   cudaStream_t st = as_stream(stream);
   Fp8MoeWs L;
   fp8_moe_layout(T, H, F, E, k, workspace, ws_bytes, &L);
-  FRANK_TRY(run_experts(x, route_w, route_ids, W, T, E, k, H, F, err_flag, L, st));
+  FRANK_TRY(run_experts(y_dtype, x, route_w, route_ids, W, T, E, k, H, F, err_flag, L, st));
   return launch_norm_rows(combine_of(L, T, E, k, H, F, y_dtype, y), st);
 }
 
@@ -366,7 +394,7 @@ int frank_fp8_moe_block(const void* x, int wr_dtype, const void* wr, const void*
   fp8_moe_layout(T, H, F, E, k, workspace, ws_bytes, &L);
   float* w = route_w ? route_w : L.w;
   int32_t* ids = route_ids ? route_ids : L.ids;
-  FRANK_TRY(route_and_run(FRANK_BF16, x, nullptr, 0.f, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
+  FRANK_TRY(route_and_run(y_dtype, FRANK_BF16, x, nullptr, 0.f, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
   return launch_norm_rows(combine_of(L, T, E, k, H, F, y_dtype, y), st);
 }
 
@@ -389,7 +417,7 @@ int frank_fp8_moe_sublayer(int res_dtype, const void* residual, const float* nor
   float* w = route_w ? route_w : L.w;
   int32_t* ids = route_ids ? route_ids : L.ids;
   FRANK_TRY(
-      route_and_run(res_dtype, residual, norm_w, eps, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
+      route_and_run(res_dtype, res_dtype, residual, norm_w, eps, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
   NormRows a = combine_of(L, T, E, k, H, F, res_dtype, out);
   a.post_w = post_w;
   a.eps = eps;

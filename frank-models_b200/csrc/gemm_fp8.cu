@@ -198,7 +198,7 @@ __device__ __forceinline__ bool tile_out(const Params& p, const Tile& tl, int ro
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 64; ++i) {
-      acc[i] *= silu_ref(acc[64 + i]);
+      acc[i] *= silu(acc[64 + i]);
       m = max(m, abs_bits(acc[i]));
     }
     // the row's other 64 columns are in the other warp of this quadrant
@@ -481,9 +481,9 @@ int make_map(CUtensorMap* m, const void* base, int64_t E, int64_t R, int64_t K, 
 
 template <int MODE>
 int launch(const Maps& maps, const Params& p, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
   const size_t smem = smem_bytes(p.E);
-  FRANK_CUDA_TRY(
-      cudaFuncSetAttribute(fp8_gemm_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  FRANK_CUDA_TRY(frank::allow_smem(done, fp8_gemm_kernel<MODE>, smem_bytes(frank::kFp8MaxE)));
   FRANK_CUDA_TRY(
       frank::launch_chained(fp8_gemm_kernel<MODE>, dim3(frank::num_sms()), dim3(kThreads), smem, st, 1, maps, p));
   FRANK_LAUNCH_CHECK();

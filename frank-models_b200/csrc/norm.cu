@@ -79,12 +79,14 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormRows a) {
   pdl_launch();
   if (t >= a.T) return;  // GS < kThreads only: whole warps
   const int64_t H = a.H;
-  float4 v[V];
+  // the row and its residual are asked for together: the sum of squares must not stand between them
+  float4 v[V], x[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int64_t h = 4 * (int64_t)(tid + i * GS);
-    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    v[i] = x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (!SLOTS && h < H) v[i] = load4(a.y, a.y_dtype, t * H + h);
+    if (a.residual != nullptr && h < H) x[i] = load4(a.residual, a.out_dtype, t * H + h);
   }
   if (SLOTS) {
     // rows in order, the loads of several at a time
@@ -94,13 +96,13 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormRows a) {
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
         const int64_t s = (int64_t)(j0 + q) * a.T + t;
-        const float* row = a.d;
-        if (j0 + q < a.k) row += (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * H;
+        int64_t row = 0;
+        if (j0 + q < a.k) row = (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * H;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const int64_t h = 4 * (int64_t)(tid + i * GS);
           u[q][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (h < H && j0 + q < a.k) u[q][i] = *reinterpret_cast<const float4*>(row + h);
+          if (h < H && j0 + q < a.k) u[q][i] = load4(a.d, a.d_dtype, row + h);
         }
       }
 #pragma unroll
@@ -132,9 +134,9 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormRows a) {
         v[i] = make_float4(v[i].x * g.x, v[i].y * g.y, v[i].z * g.z, v[i].w * g.w);
       }
       if (a.residual != nullptr) {
-        const float4 x = load4(a.residual, a.out_dtype, t * H + h);
         const float s = a.residual_scale;
-        v[i] = make_float4(fmaf(s, x.x, v[i].x), fmaf(s, x.y, v[i].y), fmaf(s, x.z, v[i].z), fmaf(s, x.w, v[i].w));
+        v[i] = make_float4(fmaf(s, x[i].x, v[i].x), fmaf(s, x[i].y, v[i].y), fmaf(s, x[i].z, v[i].z),
+                           fmaf(s, x[i].w, v[i].w));
       }
       if (a.out != nullptr) {
         if (a.out_dtype == FRANK_BF16) v[i] = round_bf16(v[i]);

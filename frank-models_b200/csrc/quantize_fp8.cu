@@ -2,9 +2,10 @@
 //
 // Rows: bound by HBM (2 or 4 bytes in, 1 out).  16 lanes hold one block of
 // 128 values, 8 each (one 16-byte load of bf16), so the maximum is four
-// shuffles and a warp stores 256 consecutive bytes.  With slot_pos a row is
-// read once and written to each of its k expert-sorted places: the gather of
-// the bf16 path costs no pass of its own.
+// shuffles and a warp stores 256 consecutive bytes; a warp has 1024 values of a
+// row under way, neighbouring warps have neighbouring rows, whose scales are
+// neighbours.  With slot_pos a row is read once and written to each of its k
+// expert-sorted places: the gather of the bf16 path costs no pass of its own.
 #include "fp8.cuh"
 
 namespace {
@@ -28,6 +29,8 @@ __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, flo
   }
 }
 
+constexpr int kPairs = 4;  // pairs of blocks a warp
+
 template <class TX>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const TX* __restrict__ x, int64_t T, int64_t K, int nb, const int32_t* __restrict__ slot_pos,
@@ -35,29 +38,42 @@ quantize_rows_kernel(const TX* __restrict__ x, int64_t T, int64_t K, int nb, con
   pdl_wait();
   pdl_launch();
   const int half = (threadIdx.x >> 4) & 1, l16 = threadIdx.x & 15;
-  const int pairs = (nb + 1) >> 1;
-  const int64_t warp = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), nwarps = (int64_t)gridDim.x * 8;
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t seg = item / T, t = item - seg * T;
+  if (seg * 2 * kPairs >= nb) return;
   const int64_t R = slot_pos != nullptr ? T * k : T;
-  for (int64_t i = warp; i < T * pairs; i += nwarps) {
-    const int64_t t = i / pairs;
-    const int b = (int)(i % pairs) * 2 + half;
-    const int64_t c = (int64_t)b * kQB + l16 * 8;
-    float v[8] = {};
-    if (c < K) load8(x + t * K + c, v);
+  const int b0 = (int)seg * 2 * kPairs + half;
+  float v[kPairs][8];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const int64_t c = (int64_t)(b0 + 2 * i) * kQB + l16 * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    if (c < K) load8(x + t * K + c, v[i]);
+  }
+  uint2 u[kPairs];
+  float sc[kPairs];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
     uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
+    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[i][j]));
 #pragma unroll
     for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const BlockScale s = block_scale(m);
-    uint2 u;
-    u.x = e4m3x4(v[0] * s.inv, v[1] * s.inv, v[2] * s.inv, v[3] * s.inv);
-    u.y = e4m3x4(v[4] * s.inv, v[5] * s.inv, v[6] * s.inv, v[7] * s.inv);
-    if (c < K) {
-      for (int j = 0; j < k; ++j) {
-        const int64_t r = slot_pos != nullptr ? (int64_t)slot_pos[j * T + t] : t;
-        *reinterpret_cast<uint2*>(q + r * K + c) = u;
-        if (l16 == 0) q_scale[b * R + r] = s.scale;
+    sc[i] = s.scale;
+    u[i].x = e4m3x4(v[i][0] * s.inv, v[i][1] * s.inv, v[i][2] * s.inv, v[i][3] * s.inv);
+    u[i].y = e4m3x4(v[i][4] * s.inv, v[i][5] * s.inv, v[i][6] * s.inv, v[i][7] * s.inv);
+  }
+  for (int j = 0; j < k; ++j) {
+    const int64_t r = slot_pos != nullptr ? (int64_t)slot_pos[j * T + t] : t;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const int b = b0 + 2 * i;
+      const int64_t c = (int64_t)b * kQB + l16 * 8;
+      if (c < K) {
+        *reinterpret_cast<uint2*>(q + r * K + c) = u[i];
+        if (l16 == 0) q_scale[b * R + r] = sc[i];
       }
     }
   }
@@ -104,9 +120,12 @@ int launch_quantize_rows(int x_dtype, const void* x, int64_t T, int64_t K, const
                          void* q, float* q_scale, cudaStream_t st) {
   if (T == 0) return FRANK_OK;
   const int nb = (int)q_blocks(K);
-  const int64_t warps = T * ((nb + 1) / 2), cap = (int64_t)num_sms() * 8;
-  const int64_t blocks = (warps + 7) / 8;
-  const dim3 grid((unsigned)(blocks < cap ? blocks : cap));
+  const int64_t warps = T * ((nb + 2 * kPairs - 1) / (2 * kPairs)), blocks = (warps + 7) / 8;
+  if (blocks > 0x7fffffffLL) {
+    set_error("quantize_fp8: T=%lld rows are too many", (long long)T);
+    return FRANK_EINVAL;
+  }
+  const dim3 grid((unsigned)blocks);
   cudaError_t e;
   if (x_dtype == FRANK_F32)
     e = launch_chained(quantize_rows_kernel<float>, grid, dim3(256), 0, st, 1, (const float*)x, T, K, nb, slot_pos,

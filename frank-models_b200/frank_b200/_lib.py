@@ -82,6 +82,9 @@ SIGNATURES = {
     "frank_prepack_experts_fp8": (_c_int, [_c_int, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp]),
     "frank_fp8_matmul": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_vp,
                                   _c_vp]),
+    "frank_fp8_linear_workspace_size": (_c_size, [_c_i64, _c_i64]),
+    "frank_fp8_linear": (_c_int, [_c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_vp,
+                                  _c_vp, _c_size, _c_vp]),
     "frank_fp8_moe_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
     "frank_fp8_moe_experts": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64,
                                        _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_size, _c_vp]),

@@ -10,6 +10,8 @@ graphs do not share one.
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib, ops
@@ -20,13 +22,23 @@ E4M3 = torch.float8_e4m3fn
 FLOATS = (torch.float32, torch.bfloat16)
 
 
+BF16_ONLY, F32_ONLY, I32_ONLY, E4M3_ONLY = ((t,) for t in (torch.bfloat16, torch.float32, torch.int32, E4M3))
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_SAME_DEVICE = contextlib.nullcontext()
+
+
 def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.detach().contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _on(device: torch.device):
+    """The context in which the library's calls go to `device` (nothing to do where it is the current one)."""
+    return _SAME_DEVICE if device.index == _current_device() else torch.cuda.device(device)
+
+
+def _stream() -> int:
+    """The current device's current stream, as a handle."""
+    return torch._C._cuda_getCurrentRawStream(_current_device())
 
 
 def _arg(t, name: str, shape=None, dtypes=FLOATS, device=None) -> torch.Tensor:
@@ -35,14 +47,18 @@ def _arg(t, name: str, shape=None, dtypes=FLOATS, device=None) -> torch.Tensor:
         raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: unsupported dtype {t.dtype}; expected {' or '.join(str(d) for d in dtypes)}")
-    if shape is not None and (t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape))):
-        want = ", ".join("*" if s is None else str(s) for s in shape)
-        raise ValueError(f"{name}: expected shape [{want}], got {tuple(t.shape)}")
+    if shape is not None:
+        got = t.shape
+        if got != shape and (len(got) != len(shape) or [s for s, n in zip(shape, got) if s is not None and s != n]):
+            want = ", ".join("*" if s is None else str(s) for s in shape)
+            raise ValueError(f"{name}: expected shape [{want}], got {tuple(got)}")
     if not t.is_cuda:
         raise ValueError(f"{name}: tensor must be on a CUDA device")
     if device is not None and t.device != device:
         raise ValueError(f"{name}: tensor is on {t.device}, expected {device}")
-    return _aligned(t)
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _out(out, name: str, shape, dtype, device) -> torch.Tensor:
@@ -66,10 +82,10 @@ def quantize_fp8(x: torch.Tensor):
     x = _arg(x, "quantize_fp8: x", (None, None))
     T, K = x.shape
     _multiple(K, "quantize_fp8: K")
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         q = torch.empty((T, K), dtype=E4M3, device=x.device)
         scale = torch.empty((_blocks(K), T), dtype=torch.float32, device=x.device)
-        _lib.check(_lib.load().frank_quantize_fp8(_DT[x.dtype], _ptr(x), T, K, _ptr(q), _ptr(scale), ops._stream()))
+        _lib.check(_lib.load().frank_quantize_fp8(_DT[x.dtype], _ptr(x), T, K, _ptr(q), _ptr(scale), _stream()))
     return q, scale
 
 
@@ -79,13 +95,13 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, return_norm:
     x = _arg(x, "rms_norm_fp8: x", (None, None))
     T, H = x.shape
     _multiple(H, "rms_norm_fp8: H")
-    weight = _arg(weight, "rms_norm_fp8: weight", (H,), (torch.float32,), x.device)
-    with torch.cuda.device(x.device):
+    weight = _arg(weight, "rms_norm_fp8: weight", (H,), F32_ONLY, x.device)
+    with _on(x.device):
         q = torch.empty((T, H), dtype=E4M3, device=x.device)
         scale = torch.empty((_blocks(H), T), dtype=torch.float32, device=x.device)
         xn = torch.empty((T, H), dtype=torch.bfloat16, device=x.device) if return_norm else None
         _lib.check(_lib.load().frank_rms_norm_fp8(_DT[x.dtype], _ptr(x), _ptr(weight), T, H, float(eps), _ptr(xn),
-                                                  _ptr(q), _ptr(scale), ops._stream()))
+                                                  _ptr(q), _ptr(scale), _stream()))
     return (q, scale, xn) if return_norm else (q, scale)
 
 
@@ -95,12 +111,12 @@ class Fp8Experts:
     finite scales (a quantised checkpoint's are used as they are)."""
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
-        q = _arg(q, "Fp8Experts: q", (None, None, None), (E4M3,))
+        q = _arg(q, "Fp8Experts: q", (None, None, None), E4M3_ONLY)
         E, N, K = q.shape
         _multiple(N, "Fp8Experts: n_out")
         _multiple(K, "Fp8Experts: n_in")
         self.q = q
-        self.scale = _arg(scale, "Fp8Experts: scale", (E, _blocks(N), _blocks(K)), (torch.float32,), q.device)
+        self.scale = _arg(scale, "Fp8Experts: scale", (E, _blocks(N), _blocks(K)), F32_ONLY, q.device)
 
     @classmethod
     def from_reference(cls, w_oie: torch.Tensor) -> "Fp8Experts":
@@ -109,11 +125,11 @@ class Fp8Experts:
         O, I, E = w.shape
         _multiple(O, "Fp8Experts: n_out")
         _multiple(I, "Fp8Experts: n_in")
-        with torch.cuda.device(w.device):
+        with _on(w.device):
             q = torch.empty((E, O, I), dtype=E4M3, device=w.device)
             scale = torch.empty((E, _blocks(O), _blocks(I)), dtype=torch.float32, device=w.device)
             _lib.check(_lib.load().frank_prepack_experts_fp8(_DT[w.dtype], _ptr(w), O, I, E, _ptr(q), _ptr(scale),
-                                                             ops._stream()))
+                                                             _stream()))
         return cls(q, scale)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -148,29 +164,38 @@ def fp8_matmul(x, weights: Fp8Experts, offsets: torch.Tensor | None = None,
     dev = weights.q.device
     if out_dtype not in FLOATS:
         raise TypeError(f"fp8_matmul: unsupported output dtype {out_dtype}")
-    if isinstance(x, (tuple, list)):
+    quantised = isinstance(x, (tuple, list))
+    if quantised:
         if len(x) != 2:
             raise ValueError("fp8_matmul: expected (q, scale)")
-        q = _arg(x[0], "fp8_matmul: q", (None, K), (E4M3,), dev)
-        scale = _arg(x[1], "fp8_matmul: scale", (_blocks(K), q.shape[0]), (torch.float32,), dev)
+        q = _arg(x[0], "fp8_matmul: q", (None, K), E4M3_ONLY, dev)
+        R = q.shape[0]
+        scale = _arg(x[1], "fp8_matmul: scale", (_blocks(K), R), F32_ONLY, dev)
     else:
-        q, scale = quantize_fp8(_arg(x, "fp8_matmul: x", (None, K), device=dev))
-    if offsets is None and E != 1:
-        raise ValueError(f"fp8_matmul: offsets may be omitted only for one expert, not {E}")
+        x = _arg(x, "fp8_matmul: x", (None, K), FLOATS, dev)
+        R = x.shape[0]
     if offsets is not None:
-        offsets = _arg(offsets, "fp8_matmul: offsets", (E + 1,), (torch.int32,), dev)
-    R = q.shape[0]
-    with torch.cuda.device(dev):
+        offsets = _arg(offsets, "fp8_matmul: offsets", (E + 1,), I32_ONLY, dev)
+    elif E != 1:
+        raise ValueError(f"fp8_matmul: offsets may be omitted only for one expert, not {E}")
+    lib = _lib.load()
+    with _on(dev):
         y = _out(out, "fp8_matmul", (R, N), out_dtype, dev)
-        _lib.check(_lib.load().frank_fp8_matmul(_ptr(q), _ptr(scale), _ptr(weights.q), _ptr(weights.scale),
-                                                _ptr(offsets), E, R, N, K, _DT[out_dtype], _ptr(y), ops._stream()))
+        if quantised:
+            _lib.check(lib.frank_fp8_matmul(_ptr(q), _ptr(scale), _ptr(weights.q), _ptr(weights.scale),
+                                            _ptr(offsets), E, R, N, K, _DT[out_dtype], _ptr(y), _stream()))
+        else:
+            ws = torch.empty(lib.frank_fp8_linear_workspace_size(R, K), dtype=torch.uint8, device=dev)
+            _lib.check(lib.frank_fp8_linear(_DT[x.dtype], _ptr(x), _ptr(weights.q), _ptr(weights.scale),
+                                            _ptr(offsets), E, R, N, K, _DT[out_dtype], _ptr(y), _ptr(ws), ws.numel(),
+                                            _stream()))
     return y
 
 
 def _gate_arg(gate, name, T, H, device):
     if gate is None:
         return None, 1
-    gate = _arg(gate, f"{name}: gate", None, (torch.float32,), device)
+    gate = _arg(gate, f"{name}: gate", None, F32_ONLY, device)
     if gate.dim() == 1:
         gate = gate[None]
     if gate.dim() != 2 or gate.shape[1] != H or gate.shape[0] < 1 or T % gate.shape[0] != 0:
@@ -204,7 +229,8 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
         self.w_up, self.w_gate, self.w_down = up, gate, down
         self.device = up.q.device
         self.wr = _arg(gate_inp_w, "gate_inp_w", (E, H), device=self.device)
-        with torch.cuda.device(self.device):
+        self._weights = [_ptr(t) for w in (up, gate, down) for t in (w.q, w.scale)]  # kept alive by w_up, w_gate, w_down
+        with _on(self.device):
             self.wr_pack = ops.router_pack(self.wr)
 
     def workspace_bytes(self, T: int) -> int:
@@ -214,9 +240,6 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
         """New for each call: ordered by the stream it is used on, kept by the graph that captures it."""
         return torch.empty(self.workspace_bytes(T) if need is None else need, dtype=torch.uint8, device=device)
 
-    def _weights(self):
-        return [_ptr(t) for w in (self.w_up, self.w_gate, self.w_down) for t in (w.q, w.scale)]
-
     def _routing(self, T, wanted):
         if not wanted:
             return None, None
@@ -225,16 +248,16 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None, return_routing: bool = False):
         """moe_ffn_block on tokens x [T, H] bfloat16 -> y [T, H] in ``out_dtype``."""
-        x = _arg(x, "fp8_moe_block: x", (None, self.H), (torch.bfloat16,), self.device)
+        x = _arg(x, "fp8_moe_block: x", (None, self.H), BF16_ONLY, self.device)
         T = x.shape[0]
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             y = _out(out, "fp8_moe_block", (T, self.H), self.out_dtype, self.device)
             rw, rid = self._routing(T, return_routing)
             ws = self._workspace(T, self.device)
             _lib.check(_lib.load().frank_fp8_moe_block(
-                _ptr(x), _lib.ROUTER_PACKED, _ptr(self.wr_pack), *self._weights(), T, self.E, self.k, self.H, self.F,
+                _ptr(x), _lib.ROUTER_PACKED, _ptr(self.wr_pack), *self._weights, T, self.E, self.k, self.H, self.F,
                 int(self.normalize), _DT[self.out_dtype], _ptr(y), _ptr(rw), _ptr(rid), _ptr(ws), ws.numel(),
-                ops._stream()))
+                _stream()))
         return (y, rw, rid) if return_routing else y
 
     def experts(self, x: torch.Tensor, route_w: torch.Tensor, route_ids: torch.Tensor,
@@ -244,17 +267,17 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
         [T, H] = sum_j route_w[j] * down(gate(x) * silu(up(x))).  With check_ids,
         ids outside [0, E) raise FrankError(EIDS) (this synchronises the stream);
         without, they are clamped."""
-        x = _arg(x, "fp8_moe_experts: x", (None, self.H), (torch.bfloat16,), self.device)
+        x = _arg(x, "fp8_moe_experts: x", (None, self.H), BF16_ONLY, self.device)
         T = x.shape[0]
-        route_w = _arg(route_w, "fp8_moe_experts: route_w", (self.k, T), (torch.float32,), self.device)
-        route_ids = _arg(route_ids, "fp8_moe_experts: route_ids", (self.k, T), (torch.int32,), self.device)
-        with torch.cuda.device(self.device):
+        route_w = _arg(route_w, "fp8_moe_experts: route_w", (self.k, T), F32_ONLY, self.device)
+        route_ids = _arg(route_ids, "fp8_moe_experts: route_ids", (self.k, T), I32_ONLY, self.device)
+        with _on(self.device):
             y = _out(out, "fp8_moe_experts", (T, self.H), self.out_dtype, self.device)
             err = torch.zeros(1, dtype=torch.int32, device=self.device) if check_ids else None
             ws = self._workspace(T, self.device)
             _lib.check(_lib.load().frank_fp8_moe_experts(
-                _ptr(x), _ptr(route_w), _ptr(route_ids), *self._weights(), T, self.E, self.k, self.H, self.F,
-                _DT[self.out_dtype], _ptr(y), _ptr(err), _ptr(ws), ws.numel(), ops._stream()))
+                _ptr(x), _ptr(route_w), _ptr(route_ids), *self._weights, T, self.E, self.k, self.H, self.F,
+                _DT[self.out_dtype], _ptr(y), _ptr(err), _ptr(ws), ws.numel(), _stream()))
             if check_ids and int(err.item()) != 0:
                 raise _lib.FrankError(_lib.EIDS, f"fp8_moe_experts: an expert id is outside [0, {self.E})")
         return y
@@ -270,19 +293,19 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
         each T/G consecutive tokens.  ``out`` may be ``residual``."""
         res = _arg(residual, "fp8_moe_sublayer: residual", (None, self.H), device=self.device)
         T = res.shape[0]
-        ffn_norm_w = _arg(ffn_norm_w, "fp8_moe_sublayer: ffn_norm_w", (self.H,), (torch.float32,), self.device)
+        ffn_norm_w = _arg(ffn_norm_w, "fp8_moe_sublayer: ffn_norm_w", (self.H,), F32_ONLY, self.device)
         if post_norm_w is not None:
-            post_norm_w = _arg(post_norm_w, "fp8_moe_sublayer: post_norm_w", (self.H,), (torch.float32,), self.device)
+            post_norm_w = _arg(post_norm_w, "fp8_moe_sublayer: post_norm_w", (self.H,), F32_ONLY, self.device)
         gate, gate_rows = _gate_arg(gate, "fp8_moe_sublayer", T, self.H, self.device)
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             y = _out(out, "fp8_moe_sublayer", (T, self.H), res.dtype, self.device)
             rw, rid = self._routing(T, return_routing)
             ws = self._workspace(T, self.device)
             _lib.check(_lib.load().frank_fp8_moe_sublayer(
                 _DT[res.dtype], _ptr(res), _ptr(ffn_norm_w), float(rms_eps), _lib.ROUTER_PACKED, _ptr(self.wr_pack),
-                *self._weights(), T, self.E, self.k, self.H, self.F, int(self.normalize), _ptr(post_norm_w),
+                *self._weights, T, self.E, self.k, self.H, self.F, int(self.normalize), _ptr(post_norm_w),
                 _ptr(gate), gate_rows, float(residual_scale), _ptr(y), _ptr(rw), _ptr(rid), _ptr(ws), ws.numel(),
-                ops._stream()))
+                _stream()))
         return (y, rw, rid) if return_routing else y
 
 
@@ -301,16 +324,16 @@ def post_norm_residual(y: torch.Tensor, residual: torch.Tensor, weight: torch.Te
         raise ValueError(f"post_norm_residual: H={H} is not a positive multiple of 4")
     dev = y.device
     res = _arg(residual, "post_norm_residual: residual", (T, H), device=dev)
-    weight = _arg(weight, "post_norm_residual: weight", (H,), (torch.float32,), dev)
+    weight = _arg(weight, "post_norm_residual: weight", (H,), F32_ONLY, dev)
     gate, gate_rows = _gate_arg(gate, "post_norm_residual", T, H, dev)
     if next_dtype not in FLOATS:
         raise TypeError(f"post_norm_residual: unsupported dtype {next_dtype}")
     if next_weight is not None:
-        next_weight = _arg(next_weight, "post_norm_residual: next_weight", (H,), (torch.float32,), dev)
-    with torch.cuda.device(dev):
+        next_weight = _arg(next_weight, "post_norm_residual: next_weight", (H,), F32_ONLY, dev)
+    with _on(dev):
         o = _out(out, "post_norm_residual", (T, H), res.dtype, dev)
         nxt = torch.empty((T, H), dtype=next_dtype, device=dev) if next_weight is not None else None
         _lib.check(_lib.load().frank_post_norm_residual(
             _DT[y.dtype], _ptr(y), _DT[res.dtype], _ptr(res), _ptr(weight), float(eps), _ptr(gate), gate_rows,
-            float(residual_scale), _ptr(o), _ptr(next_weight), _DT[next_dtype], _ptr(nxt), T, H, ops._stream()))
+            float(residual_scale), _ptr(o), _ptr(next_weight), _DT[next_dtype], _ptr(nxt), T, H, _stream()))
     return o if nxt is None else (o, nxt)

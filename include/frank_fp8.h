@@ -71,9 +71,21 @@ int frank_fp8_matmul(const void* q, const float* scale, const void* w,
                      void* out, void* stream);
 
 /*
+ * frank_fp8_matmul of rows x [rows, K] (FRANK_F32 or FRANK_BF16) that are quantised
+ * first, in a workspace of frank_fp8_linear_workspace_size(rows, K) bytes.
+ */
+size_t frank_fp8_linear_workspace_size(int64_t rows, int64_t K);
+int frank_fp8_linear(int x_dtype, const void* x, const void* w,
+                     const float* w_scale, const int32_t* offsets, int64_t E,
+                     int64_t rows, int64_t N, int64_t K, int out_dtype,
+                     void* out, void* workspace, size_t ws_bytes,
+                     void* stream);
+
+/*
  * The expert FFN with the routing given: x [T, H] bf16 is quantised,
  *   h = gate(x) * silu(up(x))   (fp32, then quantised in blocks of 128 of F)
- *   y[t] = sum_j route_w[j, t] * down(h[j, t])     (fp32, j in order)
+ *   y[t] = sum_j route_w[j, t] * down(h[j, t])     (fp32, j in order; with more than
+ *                                      64 tokens and a bf16 y each term is rounded to bf16)
  * route_w [k, T] fp32, route_ids [k, T] int32 in [0, E), the ids of one token
  * distinct; y [T, H] in y_dtype.  An id outside [0, E) is clamped and recorded
  * in *err_flag (device int32, zeroed by the caller; may be NULL).

@@ -95,17 +95,18 @@ def _pair(g, u):
 
 
 def moe_experts(x, route_w, route_ids, w_gate, w_up, w_down):
-    """y[t] = sum_j w[j, t] * ffn(x[t]) and its bound; x [T, H], weights [E, N, K] float64."""
+    """y[t] = sum_j w[j, t] * ffn(x[t]), its bound, and sum_j |w ffn|; x [T, H], weights [E, N, K] float64."""
     xq = quantised(x)
-    y, bound = torch.zeros_like(x), torch.zeros_like(x)
+    y, bound, terms = torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(x)
     k = route_ids.shape[0]
     for e in route_ids.unique().tolist():
         j, t = torch.nonzero(route_ids == e, as_tuple=True)
         d, b = expert_ffn(xq[t], w_gate[e], w_up[e], w_down[e])
         w = route_w[j, t][:, None]
         y.index_add_(0, t, d * w)
+        terms.index_add_(0, t, (d * w).abs())
         bound.index_add_(0, t, (b + (k + 2) * U32 * d.abs()) * w.abs())
-    return y, bound
+    return y, bound, terms
 
 
 def rms_norm(x, w, eps, err=None):

@@ -89,6 +89,7 @@ def test_library_accepts_nothing_to_do(lib):
     """No rows: success without a launch."""
     assert lib.frank_quantize_fp8(0, None, 0, 128, None, None, None) == 0
     assert lib.frank_fp8_matmul(None, None, None, None, None, 1, 0, 128, 128, 0, None, None) == 0
+    assert lib.frank_fp8_linear(0, None, None, None, None, 1, 0, 128, 128, 0, None, None, 0, None) == 0
     assert lib.frank_post_norm_residual(0, None, 0, None, None, 1e-5, None, 1, 1.0, None, None, 0, None, 0, 128,
                                         None) == 0
     assert lib.frank_fp8_moe_experts(*[None] * 9, 0, 8, 2, 128, 128, 0, None, None, None, 0, None) == 0
