@@ -5,45 +5,60 @@
 //   v    = residual_scale * residual + gate * v / sqrt(mean v^2 + eps) * post_w
 //   next = v / sqrt(mean v^2 + eps) * next_w
 //
-// Bound by HBM: every value is read once and kept in registers (H <= 16384:
-// 16 vectors of 4 for each of 256 threads), the two sums of squares are
-// reductions over the row's threads.  Rows of up to 1024 values are one warp
-// each, longer ones one block of 256 threads.  Thread i of a row owns vectors
-// i, i + threads, ...: the 128 values of a quantisation block are one vector of
-// each of a warp's lanes, so the block's maximum is one warp reduction.
+// Bound by HBM, and close behind by issue: every value is read once and kept in
+// registers (H <= 16384: 4 vectors of 4 for each of 1024 threads), the two sums of
+// squares are reductions over the row's threads.  Rows of up to 1024 values are one
+// warp each, longer ones one block of 128 to 1024 threads.  Thread i of a row owns
+// vectors i, i + threads, ...: the 128 values of a quantisation block are one
+// vector of each of a warp's lanes, so the block's maximum is one warp reduction.
+// 16384 rows of 4096, fp32 y, bf16 residual and next: 106 us,
+// 6.36 TB/s.  Slower: two vectors a thread (128 us), a run of rows
+// a block with the weights in shared memory and the next row on its way (217 us).
 #include "fp8.cuh"
 
 namespace {
 using namespace frank;
 
-constexpr int kThreads = 256;
-
-__device__ __forceinline__ float4 load4(const void* p, int dtype, int64_t i) {
-  if (dtype == FRANK_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + i);
-  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-  return make_float4(a.x, a.y, b.x, b.y);
+__device__ __forceinline__ float4 unpack4(uint2 u) {
+  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                     __uint_as_float(u.y & 0xffff0000u));
 }
 
-__device__ __forceinline__ void store4(void* p, int dtype, int64_t i, float4 v) {
-  if (dtype == FRANK_F32)
-    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = v;
-  else
-    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p) + i) =
-        make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+// This thread's V vectors of a row, GS vectors apart (zeros past the row's n), fp32 or bf16.
+template <int GS, int V>
+__device__ __forceinline__ void load_row(float4 (&v)[V], const void* base, int dtype, int64_t row, int tid, int n) {
+  if (dtype == FRANK_F32) {
+    const float4* p = reinterpret_cast<const float4*>(base) + row + tid;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = tid + i * GS < n ? p[i * GS] : make_float4(0.f, 0.f, 0.f, 0.f);
+  } else {
+    const uint2* p = reinterpret_cast<const uint2*>(base) + row + tid;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = unpack4(tid + i * GS < n ? p[i * GS] : make_uint2(0u, 0u));
+  }
 }
 
-__device__ __forceinline__ float4 round_bf16(float4 v) {
-  v.x = __bfloat162float(__float2bfloat16_rn(v.x));
-  v.y = __bfloat162float(__float2bfloat16_rn(v.y));
-  v.z = __bfloat162float(__float2bfloat16_rn(v.z));
-  v.w = __bfloat162float(__float2bfloat16_rn(v.w));
-  return v;
+// Stores them; ROUND: v becomes what the row then holds.
+template <int GS, int V, bool ROUND>
+__device__ __forceinline__ void store_row(float4 (&v)[V], void* base, int dtype, int64_t row, int tid, int n) {
+  if (dtype == FRANK_F32) {
+    float4* p = reinterpret_cast<float4*>(base) + row + tid;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (tid + i * GS < n) p[i * GS] = v[i];
+  } else {
+    uint2* p = reinterpret_cast<uint2*>(base) + row + tid;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint2 u = make_uint2(pack_bf16x2(v[i].x, v[i].y), pack_bf16x2(v[i].z, v[i].w));
+      if (tid + i * GS < n) p[i * GS] = u;
+      if (ROUND) v[i] = unpack4(u);
+    }
+  }
 }
 
-// Sum over the GS threads of a row, the same in every thread; `red`: one
-// array for each sum of a kernel, so that no barrier is needed before it.
+// Sum over the GS threads of a row, the same in every thread; `red`: one array for
+// each sum of a row, so that no barrier is needed before it.
 template <int GS>
 __device__ __forceinline__ float row_sum(float v, float* red) {
 #pragma unroll
@@ -53,12 +68,16 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   __syncthreads();
   float s = 0.f;
 #pragma unroll
-  for (int w = 0; w < GS / 32; ++w) s += red[w];
+  for (int w = 0; w < GS / 32; w += 4) {
+    const float4 q = *reinterpret_cast<const float4*>(red + w);
+    s += (q.x + q.y) + (q.z + q.w);
+  }
   return s;
 }
 
+// 1 / sqrt(mean v^2 + eps); CUDA's rsqrtf is within 2 ulp.
 template <int GS, int V>
-__device__ __forceinline__ float inv_rms(const float4 (&v)[V], int64_t H, float eps, float* red) {
+__device__ __forceinline__ float inv_rms(const float4 (&v)[V], int n, float eps, float* red) {
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -67,43 +86,47 @@ __device__ __forceinline__ float inv_rms(const float4 (&v)[V], int64_t H, float 
     ss = fmaf(v[i].z, v[i].z, ss);
     ss = fmaf(v[i].w, v[i].w, ss);
   }
-  return 1.f / sqrtf(row_sum<GS>(ss, red) / (float)H + eps);
+  return rsqrtf(row_sum<GS>(ss, red) / (float)(4 * n) + eps);
+}
+
+// v *= r * w, w a row of n vectors
+template <int GS, int V>
+__device__ __forceinline__ void scale_row(float4 (&v)[V], float r, const float* w, int tid, int n) {
+  const float4* p = reinterpret_cast<const float4*>(w) + tid;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (tid + i * GS < n) {
+      const float4 q = p[i * GS];
+      v[i] = make_float4(v[i].x * r * q.x, v[i].y * r * q.y, v[i].z * r * q.z, v[i].w * r * q.w);
+    }
 }
 
 template <int GS, int V, bool SLOTS>
-__global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormRows a) {
-  __shared__ float red[2][kThreads / 32];
-  const int tid = threadIdx.x % GS;
-  const int64_t t = (int64_t)blockIdx.x * (kThreads / GS) + threadIdx.x / GS;
+__global__ void __launch_bounds__(GS == 32 ? 256 : GS)
+norm_rows_kernel(const NormRows a) {
+  constexpr int kGroups = GS == 32 ? 8 : 1;
+  __shared__ alignas(16) float red[2][GS == 32 ? 4 : GS / 32];
+  const int tid = threadIdx.x % GS, n = (int)(a.H / 4);
+  const int64_t t = (int64_t)blockIdx.x * kGroups + threadIdx.x / GS;
   pdl_wait();
   pdl_launch();
-  if (t >= a.T) return;  // GS < kThreads only: whole warps
-  const int64_t H = a.H;
-  // the row and its residual are asked for together: the sum of squares must not stand between them
+  if (t >= a.T) return;  // whole warps of GS = 32
+  // a row and its residual are asked for together: the sum of squares must not stand between them
   float4 v[V], x[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int64_t h = 4 * (int64_t)(tid + i * GS);
-    v[i] = x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!SLOTS && h < H) v[i] = load4(a.y, a.y_dtype, t * H + h);
-    if (a.residual != nullptr && h < H) x[i] = load4(a.residual, a.out_dtype, t * H + h);
-  }
+  if (!SLOTS) load_row<GS, V>(v, a.y, a.y_dtype, t * n, tid, n);
+  if (a.residual != nullptr) load_row<GS, V>(x, a.residual, a.out_dtype, t * n, tid, n);
   if (SLOTS) {
     // rows in order, the loads of several at a time
     constexpr int kAhead = V <= 2 ? 4 : V <= 4 ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int j0 = 0; j0 < a.k; j0 += kAhead) {
       float4 u[kAhead][V];
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
         const int64_t s = (int64_t)(j0 + q) * a.T + t;
-        int64_t row = 0;
-        if (j0 + q < a.k) row = (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * H;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int64_t h = 4 * (int64_t)(tid + i * GS);
-          u[q][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (h < H && j0 + q < a.k) u[q][i] = load4(a.d, a.d_dtype, row + h);
-        }
+        if (j0 + q < a.k)
+          load_row<GS, V>(u[q], a.d, a.d_dtype, (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * n, tid, n);
       }
 #pragma unroll
       for (int q = 0; q < kAhead; ++q)
@@ -118,54 +141,98 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormRows a) {
         }
     }
   }
-  float r = 1.f;
-  if (a.post_w != nullptr) r = inv_rms<GS, V>(v, H, a.eps, red[0]);
-  const float* gate = a.gate == nullptr ? nullptr : a.gate + t / a.rows_per_gate * H;
+  if (a.post_w != nullptr) scale_row<GS, V>(v, inv_rms<GS, V>(v, n, a.eps, red[0]), a.post_w, tid, n);
+  if (a.gate != nullptr)
+    scale_row<GS, V>(v, 1.f, a.gate + (int64_t)((uint32_t)t / (uint32_t)a.rows_per_gate) * a.H, tid, n);
+  if (a.residual != nullptr) {
+    const float s = a.residual_scale;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int64_t h = 4 * (int64_t)(tid + i * GS);
-    if (h < H) {
-      if (a.post_w != nullptr) {
-        const float4 w = *reinterpret_cast<const float4*>(a.post_w + h);
-        v[i] = make_float4(v[i].x * r * w.x, v[i].y * r * w.y, v[i].z * r * w.z, v[i].w * r * w.w);
-      }
-      if (gate != nullptr) {
-        const float4 g = *reinterpret_cast<const float4*>(gate + h);
-        v[i] = make_float4(v[i].x * g.x, v[i].y * g.y, v[i].z * g.z, v[i].w * g.w);
-      }
-      if (a.residual != nullptr) {
-        const float s = a.residual_scale;
-        v[i] = make_float4(fmaf(s, x[i].x, v[i].x), fmaf(s, x[i].y, v[i].y), fmaf(s, x[i].z, v[i].z),
-                           fmaf(s, x[i].w, v[i].w));
-      }
-      if (a.out != nullptr) {
-        if (a.out_dtype == FRANK_BF16) v[i] = round_bf16(v[i]);
-        store4(a.out, a.out_dtype, t * H + h, v[i]);
-      }
-    }
+    for (int i = 0; i < V; ++i)
+      v[i] = make_float4(fmaf(s, x[i].x, v[i].x), fmaf(s, x[i].y, v[i].y), fmaf(s, x[i].z, v[i].z),
+                         fmaf(s, x[i].w, v[i].w));
   }
+  if (a.out != nullptr) store_row<GS, V, true>(v, a.out, a.out_dtype, t * n, tid, n);
   if (a.next_w == nullptr) return;
-  r = inv_rms<GS, V>(v, H, a.eps, red[1]);
+  scale_row<GS, V>(v, inv_rms<GS, V>(v, n, a.eps, red[1]), a.next_w, tid, n);
+  if (a.q == nullptr) {
+    store_row<GS, V, false>(v, a.next, a.next_dtype, t * n, tid, n);
+    return;
+  }
+  if (a.next != nullptr) store_row<GS, V, false>(v, a.next, a.next_dtype, t * n, tid, n);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int64_t h = 4 * (int64_t)(tid + i * GS);
-    if (h < H) {
-      const float4 w = *reinterpret_cast<const float4*>(a.next_w + h);
-      v[i] = make_float4(v[i].x * r * w.x, v[i].y * r * w.y, v[i].z * r * w.z, v[i].w * r * w.w);
-      if (a.next != nullptr) store4(a.next, a.next_dtype, t * H + h, v[i]);
-    }
-    if (a.q != nullptr) {  // lanes past H hold zeros
-      v[i] = round_bf16(v[i]);
-      uint32_t m = max(max(abs_bits(v[i].x), abs_bits(v[i].y)), max(abs_bits(v[i].z), abs_bits(v[i].w)));
-      m = __reduce_max_sync(0xffffffffu, m);
-      const BlockScale s = block_scale(m);
-      if (h < H) {
-        *reinterpret_cast<uint32_t*>(a.q + t * H + h) =
-            e4m3x4(v[i].x * s.inv, v[i].y * s.inv, v[i].z * s.inv, v[i].w * s.inv);
-        if (h % kQB == 0) a.q_scale[h / kQB * a.T + t] = s.scale;
-      }
+  for (int i = 0; i < V; ++i) {  // lanes past the row hold zeros
+    const int h = tid + i * GS;
+    const float4 w = unpack4(make_uint2(pack_bf16x2(v[i].x, v[i].y), pack_bf16x2(v[i].z, v[i].w)));
+    const BlockScale s = block_scale(
+        __reduce_max_sync(0xffffffffu, max(max(abs_bits(w.x), abs_bits(w.y)), max(abs_bits(w.z), abs_bits(w.w)))));
+    if (h < n) {
+      *reinterpret_cast<uint32_t*>(a.q + t * a.H + 4 * h) =
+          e4m3x4(w.x * s.inv, w.y * s.inv, w.z * s.inv, w.w * s.inv);
+      if (h % (kQB / 4) == 0) a.q_scale[(int64_t)(h / (kQB / 4)) * a.T + t] = s.scale;
     }
   }
+}
+
+// y[t] = sum_j d[slot_pos[j]] alone: eight columns a thread, eight rows at a time.
+template <class TD, class TY>
+__global__ void __launch_bounds__(128) combine_slots_kernel(const NormRows a) {
+  pdl_wait();
+  pdl_launch();
+  const int64_t t = blockIdx.x;
+  const int h = (blockIdx.y * 128 + threadIdx.x) * 8;
+  if (h >= a.H) return;
+  const TD* d = static_cast<const TD*>(a.d);
+  float v[8] = {};
+  for (int j0 = 0; j0 < a.k; j0 += 8) {
+    float4 u[8][2];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if (j0 + q < a.k) {
+        const int64_t s = (int64_t)(j0 + q) * a.T + t;
+        const TD* row = d + (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * a.H + h;
+        if constexpr (sizeof(TD) == 4) {
+          u[q][0] = *reinterpret_cast<const float4*>(row);
+          u[q][1] = *reinterpret_cast<const float4*>(row + 4);
+        } else {
+          const uint4 p = *reinterpret_cast<const uint4*>(row);
+          u[q][0] = make_float4(__uint_as_float(p.x << 16), __uint_as_float(p.x & 0xffff0000u),
+                                __uint_as_float(p.y << 16), __uint_as_float(p.y & 0xffff0000u));
+          u[q][1] = make_float4(__uint_as_float(p.z << 16), __uint_as_float(p.z & 0xffff0000u),
+                                __uint_as_float(p.w << 16), __uint_as_float(p.w & 0xffff0000u));
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (j0 + q < a.k) {
+        v[0] += u[q][0].x, v[1] += u[q][0].y, v[2] += u[q][0].z, v[3] += u[q][0].w;
+        v[4] += u[q][1].x, v[5] += u[q][1].y, v[6] += u[q][1].z, v[7] += u[q][1].w;
+      }
+  }
+  TY* y = static_cast<TY*>(a.out) + t * a.H + h;
+  if constexpr (sizeof(TY) == 4) {
+    *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(y + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4*>(y) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                              pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  }
+}
+
+template <int GS, int V>
+cudaError_t launch_rows(const NormRows& a, cudaStream_t st) {
+  constexpr int kGroups = GS == 32 ? 8 : 1;
+  const dim3 grid((unsigned)((a.T + kGroups - 1) / kGroups)), block(GS == 32 ? 256 : GS);
+  return a.d != nullptr ? launch_chained(norm_rows_kernel<GS, V, true>, grid, block, 0, st, 1, a)
+                        : launch_chained(norm_rows_kernel<GS, V, false>, grid, block, 0, st, 1, a);
+}
+
+template <class TD>
+cudaError_t launch_combine_slots(const NormRows& a, cudaStream_t st) {
+  const dim3 grid((unsigned)a.T, (unsigned)((a.H + 1023) / 1024));
+  if (a.out_dtype == FRANK_F32)
+    return launch_chained(combine_slots_kernel<TD, float>, grid, dim3(128), 0, st, 1, a);
+  return launch_chained(combine_slots_kernel<TD, __nv_bfloat16>, grid, dim3(128), 0, st, 1, a);
 }
 
 }  // namespace
@@ -174,26 +241,19 @@ namespace frank {
 
 int launch_norm_rows(const NormRows& a, cudaStream_t st) {
   if (a.T == 0) return FRANK_OK;
-  const bool warp_rows = a.H <= 1024;
-  const int64_t vec = (a.H / 4 + (warp_rows ? 32 : kThreads) - 1) / (warp_rows ? 32 : kThreads);
-  const int64_t per = warp_rows ? kThreads / 32 : 1;
-  const dim3 grid((unsigned)((a.T + per - 1) / per)), block(kThreads);
+  const int64_t H4 = a.H / 4;
   cudaError_t e;
-#define FRANK_NORM(GS, V)                                                                      \
-  e = a.d != nullptr ? launch_chained(norm_rows_kernel<GS, V, true>, grid, block, 0, st, 1, a) \
-                     : launch_chained(norm_rows_kernel<GS, V, false>, grid, block, 0, st, 1, a)
-  if (warp_rows) {
-    if (vec <= 1) FRANK_NORM(32, 1);
-    else if (vec <= 2) FRANK_NORM(32, 2);
-    else if (vec <= 4) FRANK_NORM(32, 4);
-    else FRANK_NORM(32, 8);
-  } else {
-    if (vec <= 2) FRANK_NORM(256, 2);
-    else if (vec <= 4) FRANK_NORM(256, 4);
-    else if (vec <= 8) FRANK_NORM(256, 8);
-    else FRANK_NORM(256, 16);
-  }
-#undef FRANK_NORM
+  if (a.d != nullptr && a.post_w == nullptr && a.gate == nullptr && a.residual == nullptr && a.next_w == nullptr &&
+      a.H % 8 == 0)
+    e = a.d_dtype == FRANK_F32 ? launch_combine_slots<float>(a, st) : launch_combine_slots<__nv_bfloat16>(a, st);
+  else if (H4 <= 32) e = launch_rows<32, 1>(a, st);
+  else if (H4 <= 64) e = launch_rows<32, 2>(a, st);
+  else if (H4 <= 128) e = launch_rows<32, 4>(a, st);
+  else if (H4 <= 256) e = launch_rows<32, 8>(a, st);
+  else if (H4 <= 512) e = launch_rows<128, 4>(a, st);
+  else if (H4 <= 1024) e = launch_rows<256, 4>(a, st);
+  else if (H4 <= 2048) e = launch_rows<512, 4>(a, st);
+  else e = launch_rows<1024, 4>(a, st);
   FRANK_CUDA_TRY(e);
   FRANK_LAUNCH_CHECK();
   return FRANK_OK;

@@ -196,7 +196,8 @@ def test_matmul_large_offsets():
 
 
 # ------------------------------------------------------------------- norms --
-@pytest.mark.parametrize("T,H", [(1, 16), (3, 272), (9, 1024), (5, 1040), (2, 2048), (1000, 4096), (2, 16384)])
+@pytest.mark.parametrize("T,H", [(1, 16), (3, 272), (9, 1024), (5, 1040), (2, 2048), (1000, 4096), (2, 16384),
+                                 (19001, 48), (2501, 1040), (1301, 2064)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_rms_norm_fp8(T, H, dtype):
     g = gen(T + H)
@@ -210,7 +211,9 @@ def test_rms_norm_fp8(T, H, dtype):
 
 
 @pytest.mark.parametrize("T,H,gates,nxt", [(1, 4, 1, True), (1, 2048, 0, True), (7, 100, 7, False), (6, 1028, 3, True),
-                                           (12, 4096, 1, True), (3, 16384, 1, True), (1021, 2040, 1021, False)])
+                                           (12, 4096, 1, True), (3, 16384, 1, True), (1021, 2040, 1021, False),
+                                           (19002, 36, 2, True), (2502, 1500, 1, False), (1302, 4100, 3, True),
+                                           (1201, 16384, 0, True)])
 @pytest.mark.parametrize("y_dtype,res_dtype", [(F32, BF16), (BF16, F32), (F32, F32), (BF16, BF16)])
 def test_post_norm_residual(T, H, gates, nxt, y_dtype, res_dtype):
     g = gen(T + H)
