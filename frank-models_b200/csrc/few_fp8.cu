@@ -3,7 +3,7 @@
 // norm.cu), without a permutation or a gather, each weight read once.
 //
 //   few_route   [norm,] quantisation, router, softmax and top-k: clusters of 8
-//               CTAs take 8 tokens, each CTA an eighth of H.  The sums of squares and
+//               CTAs take 4 tokens, each CTA an eighth of H.  The sums of squares and
 //               the partial logits are exchanged through distributed shared memory
 //               and added in CTA order.
 //   few_product<UP>    h = gate * silu(up), quantised: tiles of 128 columns of F (one
@@ -60,12 +60,12 @@ __device__ __forceinline__ float4 load4(const void* p, int dtype, int64_t i) {
 }
 
 // -------------------------------------------------------------- route --
-constexpr int kRouteCtas = 8, kRouteTok = 8, kRouteThreads = 512;
+constexpr int kRouteCtas = 8, kRouteTok = 4, kRouteThreads = 1024;
 
 // PER: experts a lane of the top-k, E <= 32 PER
 template <int PER>
 __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute a) {
-  extern __shared__ float xs[];  // [8 tokens][slice]
+  extern __shared__ float xs[];  // [tokens][slice]
   __shared__ float part[kRouteCtas][kFewMaxE];  // of this CTA's token, from every slice
   __shared__ float ssq_block[kRouteTok][16], ssq[kRouteCtas][kRouteTok];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -151,8 +151,9 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
   }
   if (a.wr == nullptr) return;  // the routing is given
   __syncthreads();
-  // partial logits of this slice: four experts a warp, 8 tokens each; the sums go to the token's CTA
-  float acc[32] = {};
+  // partial logits of this slice: four experts a warp, four tokens each; the sums go to the token's CTA
+  constexpr int kSums = 4 * kRouteTok;
+  float acc[kSums] = {};
   auto step = [&](int q, const float4 (&w)[4]) {
     if (q >= steps) return;
     const int b = q % sb;
@@ -162,14 +163,15 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
         const float4 v = *reinterpret_cast<const float4*>(xs + t * slice + b * kQB + lane * 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          acc[j * 8 + t] =
-              fmaf(v.w, w[j].w, fmaf(v.z, w[j].z, fmaf(v.y, w[j].y, fmaf(v.x, w[j].x, acc[j * 8 + t]))));
+          acc[j * kRouteTok + t] =
+              fmaf(v.w, w[j].w, fmaf(v.z, w[j].z, fmaf(v.y, w[j].y, fmaf(v.x, w[j].x, acc[j * kRouteTok + t]))));
       }
     }
     if (b < sb - 1) return;
-    // 32 sums over 32 lanes: each step halves the values a lane still carries; lane l ends with sum l
+    // kSums sums over the lanes: each step halves the values a lane still carries; lane l ends
+    // with sum l % kSums of half a warp, and the last step adds the halves
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
+    for (int o = kSums / 2; o; o >>= 1) {
       const bool up = lane & o;
 #pragma unroll
       for (int i = 0; i < o; ++i) {
@@ -178,11 +180,13 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
         acc[i] = (up ? acc[i + o] : acc[i]) + got;
       }
     }
-    const int e = (q / sb * kWarps + warp) * 4 + (lane >> 3), t = lane & 7;
-    if (e < a.E && t < nt) st_peer(peer_addr(&part[rank][e], (uint32_t)t), __float_as_uint(acc[0]));
+    const float sum = acc[0] + __shfl_xor_sync(0xffffffffu, acc[0], 16);
+    const int e = (q / sb * kWarps + warp) * 4 + (lane & (kSums - 1)) / kRouteTok, t = lane & (kRouteTok - 1);
+    if (lane < kSums && e < a.E && t < nt) st_peer(peer_addr(&part[rank][e], (uint32_t)t), __float_as_uint(sum));
 #pragma unroll
-    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+    for (int i = 0; i < kSums; ++i) acc[i] = 0.f;
   };
+  static_assert(kSums == 16, "half a warp holds the sums");
 #pragma unroll 1
   for (int q = 0; q < steps; q += 2) {
     step(q, w0);
