@@ -32,9 +32,14 @@ struct Fp8Weights {
   const float *s_up, *s_gate, *s_down;
 };
 
-// A few tokens: the weights bound the call, and few_fp8.cu reads them once.
-static bool few_tokens(int64_t T, int64_t k, int64_t H, int64_t F) {
-  return T <= kFewMaxT && k * T <= kFewMaxSlots && q_blocks(H) <= kFewMaxBlocksH && q_blocks(F) <= kFewMaxBlocksF;
+// A few tokens: the weights bound the call, and few_fp8.cu reads them once.  It takes 32
+// tokens of an expert at once, so the experts must not have many more on average:
+// 64 tokens, 2 of 8 experts of 4096 x 14336: 268 us there and 274 us by the
+// sorted rows; 2 of 4 experts of 4096 x 4096: 101 and 71 us; 8 of 128 experts of
+// 2048 x 768: 132 and 165 us; one token, 8 of 128: 31 and 61 us.
+static bool few_tokens(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
+  return T <= kFewMaxT && k * T <= kFewMaxSlots && k * T <= 24 * E && q_blocks(H) <= kFewMaxBlocksH &&
+         q_blocks(F) <= kFewMaxBlocksF;
 }
 
 // Workspace of one call; the same for a block, its experts and its sub-layer
@@ -71,7 +76,7 @@ static size_t fp8_moe_layout(int64_t T, int64_t H, int64_t F, int64_t E, int64_t
   l.slot_pos = c.take<int32_t>(n);
   l.wsorted = c.take<float>(n);
   l.xn = c.take<__nv_bfloat16>(T * H);
-  const bool few = few_tokens(T, k, H, F);
+  const bool few = few_tokens(T, E, k, H, F);
   const int64_t h_rows = few ? few_h_rows(T, E, k) : n;
   l.xq = c.take<uint8_t>(n * H);
   l.xs = c.take<float>((few ? kFewMaxT : n) * q_blocks(H));
@@ -162,17 +167,17 @@ static FewRoute few_route(int x_dtype, const void* x, const float* norm_w, float
 // The products of a prompt's slots leave in the type of the result: for a bf16 result each
 // slot is rounded once more (half a step of bf16 of its own share of the sum) and
 // the 2 k bytes a value written and read are halved, which end the tiles of a short
-// K: 271 -> 205 us for the down product of 65536 slots, 2048 from 768.  A few
+// K: 271 -> 214 us for the down product of 65536 slots, 2048 from 768.  A few
 // tokens' slots and fp32 results stay in fp32.
-static int d_dtype(int y_dtype, int64_t T, int64_t k, int64_t H, int64_t F) {
-  return few_tokens(T, k, H, F) ? FRANK_F32 : y_dtype;
+static int d_dtype(int y_dtype, int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
+  return few_tokens(T, E, k, H, F) ? FRANK_F32 : y_dtype;
 }
 
 // Routed rows through the experts: L.d[r] = w * down(q(h)) for the expert-sorted rows r.
 static int run_experts(int y_dtype, const void* x, const float* w, const int32_t* ids, const Fp8Weights& W, int64_t T, int64_t E,
                        int64_t k, int64_t H, int64_t F, int32_t* err, const Fp8MoeWs& L, cudaStream_t st) {
   const int64_t n = k * T;
-  if (few_tokens(T, k, H, F)) {
+  if (few_tokens(T, E, k, H, F)) {
     FRANK_TRY(launch_few_route(few_route(FRANK_BF16, x, nullptr, 0.f, FRANK_F32, nullptr, T, E, k, H, F, 0, nullptr,
                                          nullptr, L), st));
     return launch_few_experts(few_args(W, T, E, k, H, F, w, ids, L), err, st);
@@ -216,9 +221,9 @@ static int run_experts(int y_dtype, const void* x, const float* w, const int32_t
 static NormRows combine_of(const Fp8MoeWs& L, int64_t T, int64_t E, int64_t k, int64_t H, int64_t F, int out_dtype,
                            void* out) {
   NormRows a;
-  a.d_dtype = d_dtype(out_dtype, T, k, H, F);
+  a.d_dtype = d_dtype(out_dtype, T, E, k, H, F);
   a.d = L.d;
-  a.slot_pos = few_tokens(T, k, H, F) ? nullptr : L.slot_pos;
+  a.slot_pos = few_tokens(T, E, k, H, F) ? nullptr : L.slot_pos;
   a.k = (int)k;
   a.T = T;
   a.H = H;
@@ -238,7 +243,7 @@ static int route_and_run(int y_dtype, int x_dtype, const void* x, const float* n
   }
   FRANK_TRY(check_float_dtype(wr_dtype, "fp8_moe router"));
   FRANK_CHECK_ARG(wr != nullptr, "fp8_moe router: null pointer");
-  if (few_tokens(T, k, H, F)) {
+  if (few_tokens(T, E, k, H, F)) {
     FRANK_TRY(launch_few_route(
         few_route(x_dtype, x, norm_w, eps, wr_dtype, wr, T, E, k, H, F, normalize, w, ids, L), st));
     return launch_few_experts(few_args(W, T, E, k, H, F, w, ids, L), nullptr, st);

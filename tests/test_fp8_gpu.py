@@ -251,17 +251,22 @@ def block(g, T, H, F, E, k, normalize=True, out_dtype=BF16):
     return fb.Fp8MoEFFNBlock(wr, up, gate, down, E, k, normalize, out_dtype=out_dtype)
 
 
+def prompt(T, b):
+    """Whether T tokens run as a prompt: sorted rows, not the few tokens' kernels."""
+    return T > 64 or b.k * T > 512 or b.k * T > 24 * b.E
+
+
 def want_moe(b, x, rw, rid):
-    """The block in float64 and its bound.  With more than 64 tokens and a bf16 result every slot's product is
-    rounded to bf16 before the fp32 sum: at most half a step of each term, |w d| with its own bound."""
+    """The block in float64 and its bound.  For a prompt and a bf16 result every slot's product is rounded to bf16
+    before the fp32 sum: at most half a step of each term, |w d| with its own bound."""
     args = x.double(), rw.double(), rid, dense(b.w_gate), dense(b.w_up), dense(b.w_down)
     y, bound, terms = Q.moe_experts(*args)
-    if b.out_dtype == BF16 and x.shape[0] > 64:
+    if b.out_dtype == BF16 and prompt(x.shape[0], b):
         bound = bound + Q.half_step(BF16) * (terms + bound)
     return y, bound
 
 
-EXPERTS = [(1, 128, 128, 1, 1), (1, 256, 144, 8, 2), (3, 272, 400, 16, 4), (40, 256, 256, 5, 3), (200, 144, 272, 12, 2),
+EXPERTS = [(64, 256, 272, 2, 2), (33, 128, 256, 1, 1), (24, 128, 256, 1, 1), (1, 128, 128, 1, 1), (1, 256, 144, 8, 2), (3, 272, 400, 16, 4), (40, 256, 256, 5, 3), (200, 144, 272, 12, 2),
            (700, 512, 384, 4, 2), (65, 1040, 96, 130, 6), (2, 16, 16, 3, 3)]
 
 
@@ -367,13 +372,13 @@ def test_sublayer_is_its_parts(T, H, F, E, k, res_dtype, post, gates):
     y, rw2, rid2 = b(xn, return_routing=True)
     assert torch.equal(rid, rid2) and torch.equal(rw, rw2)
     err = None
-    if T > 64 and res_dtype == BF16:  # the slots' products are rounded to bf16 there, half a step each
+    if prompt(T, b) and res_dtype == BF16:  # the slots' products are rounded to bf16 there, half a step each
         _, e, terms = Q.moe_experts(xn.double(), rw.double(), rid, dense(b.w_gate), dense(b.w_up), dense(b.w_down))
         err = Q.half_step(BF16) * (terms + e)
     want, bound = Q.post_norm_residual(y.double(), res.double(), pw.double() if post else None, 1e-5,
                                        None if gate is None else gate.double(), 0.5, err)
     within(out, want, bound)
-    if post and (T <= 64 or res_dtype == F32):
+    if post and (not prompt(T, b) or res_dtype == F32):
         assert torch.equal(out, fb.post_norm_residual(y, res, pw, 1e-5, gate=gate, residual_scale=0.5))
     again = res.clone()
     assert torch.equal(b.sublayer(again, nw, 1e-5, post_norm_w=pw if post else None, gate=gate, residual_scale=0.5,
