@@ -586,6 +586,7 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
           if (!UP) rows(r.s, box, kb, row);
         }
       }
+      if (!ok) outlast_copies();
     }
   } else if (warp == 1) {
     if (lane == 0) {

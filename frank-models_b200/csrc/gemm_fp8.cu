@@ -350,6 +350,7 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
           }
         }
       }
+      if (!ok) outlast_copies();
     } else if (warp == 1 && lane == 0) {
       // ----------------------------------------------- MMA issuer --
       uint32_t it = 0;

@@ -82,6 +82,14 @@ __device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, 
   }
 }
 
+// After a wait gave up: gives this CTA's own copies the time to land (at most a
+// millisecond) before its shared memory goes to another one.
+__device__ __forceinline__ void outlast_copies() {
+  const uint64_t t0 = global_ns();
+  while (global_ns() - t0 < 1000000ull) {
+  }
+}
+
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)

@@ -61,9 +61,12 @@ def _arg(t, name: str, shape=None, dtypes=FLOATS, device=None) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _out(out, name: str, shape, dtype, device) -> torch.Tensor:
-    """The output: new, or the caller's (exact shape and dtype, contiguous, aligned)."""
+def _out(out, name: str, shape, dtype, device, like: torch.Tensor | None = None) -> torch.Tensor:
+    """The output: new, or the caller's (exact shape and dtype, contiguous, aligned).
+    like: a contiguous tensor of the shape (empty_like costs the host half of empty)."""
     if out is None:
+        if like is not None and like.dtype == dtype:
+            return torch.empty_like(like)
         return torch.empty(shape, dtype=dtype, device=device)
     if (not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(shape) or out.dtype != dtype
             or out.device != device or not out.is_contiguous() or out.data_ptr() % 16 != 0):
@@ -193,14 +196,15 @@ def fp8_matmul(x, weights: Fp8Experts, offsets: torch.Tensor | None = None,
 
 
 def _gate_arg(gate, name, T, H, device):
+    """(gate, its rows): [H], or [G, H] with G dividing T."""
     if gate is None:
         return None, 1
     gate = _arg(gate, f"{name}: gate", None, F32_ONLY, device)
-    if gate.dim() == 1:
-        gate = gate[None]
-    if gate.dim() != 2 or gate.shape[1] != H or gate.shape[0] < 1 or T % gate.shape[0] != 0:
-        raise ValueError(f"{name}: gate must be [{H}] or [G, {H}] with G dividing {T}, got {tuple(gate.shape)}")
-    return gate, gate.shape[0]
+    shape = gate.shape
+    rows = shape[0] if len(shape) == 2 else 1
+    if not 1 <= len(shape) <= 2 or shape[-1] != H or rows < 1 or T % rows != 0:
+        raise ValueError(f"{name}: gate must be [{H}] or [G, {H}] with G dividing {T}, got {tuple(shape)}")
+    return gate, rows
 
 
 class Fp8MoEFFNBlock(ops.MoEFFNBlock):
@@ -251,7 +255,7 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
         x = _arg(x, "fp8_moe_block: x", (None, self.H), BF16_ONLY, self.device)
         T = x.shape[0]
         with _on(self.device):
-            y = _out(out, "fp8_moe_block", (T, self.H), self.out_dtype, self.device)
+            y = _out(out, "fp8_moe_block", (T, self.H), self.out_dtype, self.device, x)
             rw, rid = self._routing(T, return_routing)
             ws = self._workspace(T, self.device)
             _lib.check(_lib.load().frank_fp8_moe_block(
@@ -272,7 +276,7 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
         route_w = _arg(route_w, "fp8_moe_experts: route_w", (self.k, T), F32_ONLY, self.device)
         route_ids = _arg(route_ids, "fp8_moe_experts: route_ids", (self.k, T), I32_ONLY, self.device)
         with _on(self.device):
-            y = _out(out, "fp8_moe_experts", (T, self.H), self.out_dtype, self.device)
+            y = _out(out, "fp8_moe_experts", (T, self.H), self.out_dtype, self.device, x)
             err = torch.zeros(1, dtype=torch.int32, device=self.device) if check_ids else None
             ws = self._workspace(T, self.device)
             _lib.check(_lib.load().frank_fp8_moe_experts(
@@ -298,7 +302,7 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
             post_norm_w = _arg(post_norm_w, "fp8_moe_sublayer: post_norm_w", (self.H,), F32_ONLY, self.device)
         gate, gate_rows = _gate_arg(gate, "fp8_moe_sublayer", T, self.H, self.device)
         with _on(self.device):
-            y = _out(out, "fp8_moe_sublayer", (T, self.H), res.dtype, self.device)
+            y = _out(out, "fp8_moe_sublayer", (T, self.H), res.dtype, self.device, res)
             rw, rid = self._routing(T, return_routing)
             ws = self._workspace(T, self.device)
             _lib.check(_lib.load().frank_fp8_moe_sublayer(
@@ -331,8 +335,8 @@ def post_norm_residual(y: torch.Tensor, residual: torch.Tensor, weight: torch.Te
     if next_weight is not None:
         next_weight = _arg(next_weight, "post_norm_residual: next_weight", (H,), F32_ONLY, dev)
     with _on(dev):
-        o = _out(out, "post_norm_residual", (T, H), res.dtype, dev)
-        nxt = torch.empty((T, H), dtype=next_dtype, device=dev) if next_weight is not None else None
+        o = _out(out, "post_norm_residual", (T, H), res.dtype, dev, res)
+        nxt = _out(None, "", (T, H), next_dtype, dev, res) if next_weight is not None else None
         _lib.check(_lib.load().frank_post_norm_residual(
             _DT[y.dtype], _ptr(y), _DT[res.dtype], _ptr(res), _ptr(weight), float(eps), _ptr(gate), gate_rows,
             float(residual_scale), _ptr(o), _ptr(next_weight), _DT[next_dtype], _ptr(nxt), T, H, _stream()))

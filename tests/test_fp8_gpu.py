@@ -483,3 +483,45 @@ def test_experts_the_same_id_twice():
         rid = torch.randint(0, 2, (k, T), generator=g, device=DEV, dtype=torch.int32)
         rw = torch.rand((k, T), generator=g, device=DEV)
         within(b.experts(x, rw, rid), *want_moe(b, x, rw, rid))
+
+
+def test_gate_refusals():
+    y, w = torch.zeros(6, 64, device=DEV), torch.ones(64, device=DEV)
+    for gate in (torch.ones(4, 64, device=DEV), torch.ones(63, device=DEV), torch.ones(6, 1, 64, device=DEV),
+                 torch.ones(0, 64, device=DEV), torch.tensor(1.0, device=DEV)):
+        with pytest.raises(ValueError, match="gate"):
+            fb.post_norm_residual(y, y, w, 1e-5, gate=gate)
+    with pytest.raises(TypeError, match="gate"):
+        fb.post_norm_residual(y, y, w, 1e-5, gate=w.bfloat16())
+
+
+def test_output_refusals():
+    """A wrong out is refused, a right one is written and returned."""
+    g = gen(17)
+    b = block(g, 4, 128, 128, 4, 2, out_dtype=F32)
+    x = randn(g, 4, 128, dtype=BF16)
+    for bad in (torch.empty(4, 128, device=DEV, dtype=BF16), torch.empty(5, 128, device=DEV), torch.empty(4, 128),
+                torch.empty(128, 4, device=DEV).t(), torch.empty(4 * 128 + 1, device=DEV)[1:].view(4, 128)):
+        with pytest.raises(ValueError, match="out must be"):
+            b(x, out=bad)
+    out = torch.empty(4, 128, device=DEV)
+    assert b(x, out=out) is out and torch.equal(out, b(x))
+
+
+def test_calls_on_another_stream_and_device_context():
+    """Calls follow the current stream of their tensors' device."""
+    g = gen(18)
+    b = block(g, 4, 256, 128, 8, 2, out_dtype=F32)
+    x = randn(g, 4, 256, dtype=BF16)
+    want = b(x)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        late = torch.zeros_like(x)
+        torch.cuda._sleep(20_000_000)  # the input arrives late on this stream
+        late.copy_(x)
+        y = b(late)
+        s = b.sublayer(late, torch.ones(256, device=DEV), 1e-5)
+    st.synchronize()
+    assert torch.equal(y, want)
+    assert torch.equal(s, b.sublayer(x, torch.ones(256, device=DEV), 1e-5))
