@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
   constexpr int kWarps = kRouteThreads / 32;
   const uint32_t rank = cta_rank();
   const int t0 = blockIdx.x / kRouteCtas * kRouteTok, nt = min(kRouteTok, a.T - t0);
-  if (a.wr != nullptr) {  // the router's slice does not wait for the stream's last kernel
+  if (a.wr != nullptr) {  // the router's slice comes to L2 while the stream's last kernel ends
     const int64_t esz = a.wr_dtype == FRANK_F32 ? 4 : 2;
     const int h0 = (int)rank * ((a.H + kQB * kRouteCtas - 1) / (kQB * kRouteCtas)) * kQB;
     const int h1 = min(h0 + (a.H + kQB * kRouteCtas - 1) / (kQB * kRouteCtas) * kQB, a.H);
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
   const int nb = (a.H + kQB - 1) / kQB, sb = (nb + kRouteCtas - 1) / kRouteCtas;  // blocks of a row, of a slice
   const int slice = sb * kQB, h0 = (int)rank * slice;
   // A warp's router weights: four experts, one block of columns a step, loaded two steps
-  // ahead; the first two before the stream's last kernel is done.
+  // ahead.
   const int steps = ((a.E + 4 * kWarps - 1) / (4 * kWarps)) * sb;
   auto router = [&](int q, float4 (&w)[4]) {
     const int e0 = (q / sb * kWarps + warp) * 4, c = h0 + q % sb * kQB + lane * 4;
@@ -95,9 +95,9 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
     }
   };
   float4 w0[4], w1[4];
-  if (a.wr != nullptr) router(0, w0), router(1, w1);
-  pdl_wait();
+  pdl_wait();  // the stream's last kernel may have written the router too
   pdl_launch();
+  if (a.wr != nullptr) router(0, w0), router(1, w1);
   cluster_arrive();  // every CTA has started before its memory is written
   for (int i = blockIdx.x * kRouteThreads + threadIdx.x; i < a.n_count; i += gridDim.x * kRouteThreads) a.count[i] = 0;
   // one (token, block) a warp: a vector of 4 for each lane
@@ -373,11 +373,6 @@ __device__ __forceinline__ void load_weights(uint32_t dst, const CUtensorMap* ma
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
       : "memory");
 }
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // K-major operand, 128-byte swizzle: rows of 128 bytes, groups of 8 rows 1024 bytes apart.
@@ -586,7 +581,6 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
           if (!UP) rows(r.s, box, kb, row);
         }
       }
-      if (!ok) outlast_copies();
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -635,7 +629,7 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
             break;
           }
           mbar_expect_tx(sfull_bar(i), bytes);
-          bulk_copy(smem_u32(scales[i]), src + (int64_t)kb * a.h_rows, bytes, sfull_bar(i));
+          bulk_load(smem_u32(scales[i]), src + (int64_t)kb * a.h_rows, bytes, sfull_bar(i));
         }
       }
     }
@@ -874,6 +868,7 @@ few_product_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__
   fence_before();
   __syncthreads();
   if (warp == 1) {
+    if (*abort_flag) outlast_copies();
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
