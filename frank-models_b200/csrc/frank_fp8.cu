@@ -21,6 +21,12 @@ static int check_float_dtype(int d, const char* what) {
   return FRANK_OK;
 }
 
+// Rows are counted in 31 bits.
+static int check_rows(int64_t T, const char* what) {
+  FRANK_CHECK_ARG(T >= 0 && T <= 0x7fffffffLL, "%s: T=%lld out of range", what, (long long)T);
+  return FRANK_OK;
+}
+
 static bool aligned16(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if ((uintptr_t)p % 16 != 0) return false;
@@ -280,8 +286,9 @@ extern "C" {
 
 int frank_quantize_fp8(int x_dtype, const void* x, int64_t T, int64_t K, void* q, float* scale, void* stream) {
   FRANK_TRY(check_float_dtype(x_dtype, "quantize_fp8"));
-  FRANK_CHECK_ARG(T >= 0 && K >= 16 && K % 16 == 0 && K <= 0x7fffffLL,
-                  "quantize_fp8: T=%lld, K=%lld: K must be a positive multiple of 16", (long long)T, (long long)K);
+  FRANK_TRY(check_rows(T, "quantize_fp8"));
+  FRANK_CHECK_ARG(K >= 16 && K % 16 == 0 && K <= 0x7fffffLL, "quantize_fp8: K=%lld must be a positive multiple of 16",
+                  (long long)K);
   if (T == 0) return FRANK_OK;
   FRANK_CHECK_ARG(x && q && scale, "quantize_fp8: null pointer");
   FRANK_CHECK_ARG(aligned16({x, q}), "quantize_fp8: x and q must be 16-byte aligned");
@@ -291,9 +298,9 @@ int frank_quantize_fp8(int x_dtype, const void* x, int64_t T, int64_t K, void* q
 int frank_rms_norm_fp8(int x_dtype, const void* x, const float* weight, int64_t T, int64_t H, float eps, void* xn,
                        void* q, float* scale, void* stream) {
   FRANK_TRY(check_float_dtype(x_dtype, "rms_norm_fp8"));
-  FRANK_CHECK_ARG(T >= 0 && H >= 16 && H % 16 == 0 && H <= kNormMaxH,
-                  "rms_norm_fp8: T=%lld, H=%lld: H must be a multiple of 16 in [16, %lld]", (long long)T, (long long)H,
-                  (long long)kNormMaxH);
+  FRANK_TRY(check_rows(T, "rms_norm_fp8"));
+  FRANK_CHECK_ARG(H >= 16 && H % 16 == 0 && H <= kNormMaxH, "rms_norm_fp8: H=%lld must be a multiple of 16 in [16, %lld]",
+                  (long long)H, (long long)kNormMaxH);
   if (T == 0) return FRANK_OK;
   FRANK_CHECK_ARG(x && weight && q && scale, "rms_norm_fp8: null pointer");
   FRANK_CHECK_ARG(aligned16({x, weight, xn, q}), "rms_norm_fp8: buffers must be 16-byte aligned");
@@ -440,9 +447,9 @@ int frank_post_norm_residual(int y_dtype, const void* y, int res_dtype, const vo
   FRANK_TRY(check_float_dtype(y_dtype, "post_norm_residual"));
   FRANK_TRY(check_float_dtype(res_dtype, "post_norm_residual"));
   if (next != nullptr) FRANK_TRY(check_float_dtype(next_dtype, "post_norm_residual"));
-  FRANK_CHECK_ARG(T >= 0 && H >= 4 && H % 4 == 0 && H <= kNormMaxH,
-                  "post_norm_residual: T=%lld, H=%lld: H must be a multiple of 4 in [4, %lld]", (long long)T,
-                  (long long)H, (long long)kNormMaxH);
+  FRANK_TRY(check_rows(T, "post_norm_residual"));
+  FRANK_CHECK_ARG(H >= 4 && H % 4 == 0 && H <= kNormMaxH,
+                  "post_norm_residual: H=%lld must be a multiple of 4 in [4, %lld]", (long long)H, (long long)kNormMaxH);
   if (T == 0) return FRANK_OK;
   FRANK_CHECK_ARG(y && residual && weight && out && (next == nullptr || next_weight),
                   "post_norm_residual: null pointer");

@@ -55,6 +55,11 @@ def test_library_refusals(lib):
     _refused(lib, lib.frank_quantize_fp8(0, None, 1, 128, P, P, None), "null")
     _refused(lib, lib.frank_quantize_fp8(0, P + 4, 1, 128, P, P, None), "aligned")
     _refused(lib, lib.frank_rms_norm_fp8(0, P, P, 1, 16400, 1e-5, None, P, P, None), "16384")
+    _refused(lib, lib.frank_quantize_fp8(0, P, -1, 128, P, P, None), "out of range")
+    _refused(lib, lib.frank_quantize_fp8(0, P, 1 << 31, 128, P, P, None), "out of range")
+    _refused(lib, lib.frank_rms_norm_fp8(0, P, P, 1 << 32, 128, 1e-5, None, P, P, None), "out of range")
+    _refused(lib, lib.frank_post_norm_residual(1, P, 1, P, P, 1e-5, P, 1, 1.0, P, None, 0, None, 1 << 32, 4, None),
+             "out of range")
     _refused(lib, lib.frank_rms_norm_fp8(0, P, None, 1, 128, 1e-5, None, P, P, None), "null")
     _refused(lib, lib.frank_prepack_experts_fp8(0, P, 16, 16, 257, P, P, None), "extents")
     _refused(lib, lib.frank_fp8_matmul(P, P, P, P, None, 2, 4, 128, 128, 0, P, None), "offsets")
