@@ -233,9 +233,11 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
         self.w_up, self.w_gate, self.w_down = up, gate, down
         self.device = up.q.device
         self.wr = _arg(gate_inp_w, "gate_inp_w", (E, H), device=self.device)
-        self._weights = [_ptr(t) for w in (up, gate, down) for t in (w.q, w.scale)]  # kept alive by w_up, w_gate, w_down
         with _on(self.device):
             self.wr_pack = ops.router_pack(self.wr)
+
+    def _weights(self):
+        return [_ptr(t) for w in (self.w_up, self.w_gate, self.w_down) for t in (w.q, w.scale)]
 
     def workspace_bytes(self, T: int) -> int:
         return _lib.load().frank_fp8_moe_workspace_size(T, self.H, self.F, self.E, self.k)
@@ -259,7 +261,7 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
             rw, rid = self._routing(T, return_routing)
             ws = self._workspace(T, self.device)
             _lib.check(_lib.load().frank_fp8_moe_block(
-                _ptr(x), _lib.ROUTER_PACKED, _ptr(self.wr_pack), *self._weights, T, self.E, self.k, self.H, self.F,
+                _ptr(x), _lib.ROUTER_PACKED, _ptr(self.wr_pack), *self._weights(), T, self.E, self.k, self.H, self.F,
                 int(self.normalize), _DT[self.out_dtype], _ptr(y), _ptr(rw), _ptr(rid), _ptr(ws), ws.numel(),
                 _stream()))
         return (y, rw, rid) if return_routing else y
@@ -280,7 +282,7 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
             err = torch.zeros(1, dtype=torch.int32, device=self.device) if check_ids else None
             ws = self._workspace(T, self.device)
             _lib.check(_lib.load().frank_fp8_moe_experts(
-                _ptr(x), _ptr(route_w), _ptr(route_ids), *self._weights, T, self.E, self.k, self.H, self.F,
+                _ptr(x), _ptr(route_w), _ptr(route_ids), *self._weights(), T, self.E, self.k, self.H, self.F,
                 _DT[self.out_dtype], _ptr(y), _ptr(err), _ptr(ws), ws.numel(), _stream()))
             if check_ids and int(err.item()) != 0:
                 raise _lib.FrankError(_lib.EIDS, f"fp8_moe_experts: an expert id is outside [0, {self.E})")
@@ -307,7 +309,7 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
             ws = self._workspace(T, self.device)
             _lib.check(_lib.load().frank_fp8_moe_sublayer(
                 _DT[res.dtype], _ptr(res), _ptr(ffn_norm_w), float(rms_eps), _lib.ROUTER_PACKED, _ptr(self.wr_pack),
-                *self._weights, T, self.E, self.k, self.H, self.F, int(self.normalize), _ptr(post_norm_w),
+                *self._weights(), T, self.E, self.k, self.H, self.F, int(self.normalize), _ptr(post_norm_w),
                 _ptr(gate), gate_rows, float(residual_scale), _ptr(y), _ptr(rw), _ptr(rid), _ptr(ws), ws.numel(),
                 _stream()))
         return (y, rw, rid) if return_routing else y

@@ -525,3 +525,26 @@ def test_calls_on_another_stream_and_device_context():
     st.synchronize()
     assert torch.equal(y, want)
     assert torch.equal(s, b.sublayer(x, torch.ones(256, device=DEV), 1e-5))
+
+
+@pytest.mark.parametrize("T", [3, 100])
+@pytest.mark.parametrize("std", [1e-3, 30.0, 1e4])
+def test_experts_small_and_large_activations(T, std):
+    """silu over its whole range: near zero, where it is u / 2, and where the exponential under- or overflows."""
+    g = gen(T)
+    b = block(g, T, 256, 272, 4, 2, out_dtype=F32)
+    x = randn(g, T, 256, std=std, dtype=BF16)
+    rw = torch.rand((2, T), generator=g, device=DEV)
+    rid = torch.stack([torch.randperm(4, generator=g, device=DEV)[:2] for _ in range(T)], 1).to(torch.int32)
+    within(b.experts(x, rw, rid), *want_moe(b, x, rw, rid))
+
+
+def test_weights_replaced():
+    """A block reads the weights it has when it is called."""
+    g = gen(23)
+    b, c = (block(g, 5, 256, 256, 4, 2) for _ in range(2))
+    x = randn(g, 5, 256, dtype=BF16)
+    b(x)
+    c.wr, c.wr_pack = b.wr, b.wr_pack
+    b.w_up, b.w_gate, b.w_down = c.w_up, c.w_gate, c.w_down
+    assert torch.equal(b(x), c(x))
