@@ -2,7 +2,6 @@
 // the 8-bit kernels (declared in include/frank_fp8.h).
 #pragma once
 
-#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include <atomic>
@@ -100,8 +99,17 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t amax) {
   return s;
 }
 
-// silu with CUDA's approximate division (2 ulp): 64 of them end a tile of a product.
-__device__ __forceinline__ float silu(float u) { return __fdividef(u, 1.0f + expf(-u)); }
+// silu(u) = u / (1 + 2^(-u log2 e)) by CUDA's approximate exponential and division (2 ulp
+// each); 64 of them end a tile of a product.  The exponent's rounding error is put
+// back as a factor 1 + ln 2 * error.  The clamp keeps 2^t finite; below it the result is 0.
+// An infinite u gives NaN, which its block of 128 becomes in any case.
+__device__ __forceinline__ float silu(float u) {
+  const float t = fminf(u * -1.44269502f, 126.f);
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  const float lost = fmaf(u, -1.92596299e-8f, fmaf(u, -1.44269502f, -t));
+  return __fdividef(u, 1.f + fmaf(e * 0.693147182f, lost, e));
+}
 
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
@@ -109,14 +117,12 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return e4m3x2(a, b) | (e4m3x2(c, d) << 16);
 }
-// two e4m3 values (low 16 bits) as fp16, exact
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t v) {
-  __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)v, __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
-}
-__device__ __forceinline__ float e4m3_to_f32(uint8_t v) {
-  __half_raw h = __nv_cvt_fp8_to_halfraw(v, __NV_E4M3);
-  return __half2float(__half(h));
+
+// 32 bytes of one thread: a whole sector.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 // Programmatic dependent launch: blocks may start while the stream's previous

@@ -18,13 +18,16 @@
 //               128 accumulators a thread, so they take registers from the first four warps
 // Tiles are (expert, m, n) with m fastest inside a band of rows that stays in L2.
 //
-// Measured, 8192 x 14336 x 4096: 482 us, 2.0 PFLOP/s; without the epilogue's loads
-// and FMAs the same pipeline takes 396 us, and 364 us without the loads of A as
-// well: the copies from L2 (48 KB a K block, 11 TB/s over all SMs) and the hand-over of
-// the two TMEM buffers bound it together.  Slower: pairs of CTAs (cta_group::2, 256 x
-// 256 tiles, a third less from L2, but a longer hand-over: 501 us), sixteen
-// epilogue warps (724 us), halves of 128 columns with barriers of their own (581 us),
-// TMEM loads one chunk ahead of the FMAs (533 us).
+// Measured, 8192 x 14336 x 4096: 478 to 490 us, 2.0 PFLOP/s, 1060 cycles a K block where
+// the MMAs alone are 512.  Without the epilogue's loads and FMAs it takes 858 (an MMA reads
+// 96 bytes a cycle from shared memory and the copies write as many, of 128), without
+// MMAs and copies the epilogue takes 965; what bounds it is the way of a TMEM
+// buffer from the last MMA through the loads to the next MMA, with only two buffers.
+// No faster: pairs of CTAs (cta_group::2, 256 x 256 tiles: 465 us, but 65536 sorted rows
+// of 128 experts 719 against 671 us for the expert FFN), sixteen epilogue warps (724 us),
+// halves of 128 columns with barriers of their own (581 us), the next K block's TMEM
+// loads before the last FMAs (523 us), the scales by warps 2 and 3 through shared
+// memory (483 us).
 // Every wait is bounded (about 2 s); on expiry the CTA records FRANK_ETIMEOUT in
 // the device error word and unwinds, freeing its TMEM.
 #include <cuda.h>
@@ -43,14 +46,13 @@ constexpr int kThreads = 384, kEpiWarps = 8;
 constexpr int kRegsLaunch = 168, kRegsFew = 40, kRegsEpilogue = 224;
 static_assert(128 * kRegsFew + 32 * kEpiWarps * kRegsEpilogue <= kThreads * kRegsLaunch, "setmaxnreg would wait");
 constexpr uint32_t kTileBytes = 128 * BK;  // 16 KiB: 128 rows of A or of B
-constexpr uint32_t kEpiBytes = kEpiWarps * 2048;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kStages = 4;
 constexpr uint32_t kStageBytes = 3 * kTileBytes;
 // kind::f8f6f4: D fp32 [4,6)=1, A and B e4m3 [7,10)=[10,13)=0, N>>3 at [17,23), M>>4 at [24,29)
 constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 size_t smem_bytes(int64_t E) {
-  return 1024 + kStages * kStageBytes + kEpiBytes + 2048 + 8 * (2 * kStages + 8) + 16 + 4 * (E + 1) + 64;
+  return 1024 + kStages * kStageBytes + 2048 + 8 * (2 * kStages + 8) + 16 + 8 * (E + 1) + 64;
 }
 
 struct Maps {
@@ -67,6 +69,7 @@ struct Params {
   int band;  // row tiles whose rows of A stay in L2 while the CTAs sweep the columns
   const float* wrow;
   int out_dtype;
+  int wide;  // rows of out are 32-byte aligned
   void* out;
   float* h_scale;
   int32_t* err;
@@ -153,13 +156,14 @@ __device__ __forceinline__ int group_at(const Params& p, int e) {
   return p.offsets != nullptr ? min(max(p.offsets[e], 0), p.rows) : (e == 0 ? 0 : p.rows);
 }
 
-__device__ __forceinline__ Tile tile_at(int t, const int* prefix, const Params& p) {
+// prefix: tiles of the groups before each; begin: their first rows.
+__device__ __forceinline__ Tile tile_at(int t, const int* prefix, const int* begin, const Params& p) {
   int lo = 0, hi = p.E;  // prefix[lo] <= t < prefix[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (prefix[mid] <= t) lo = mid; else hi = mid;
   }
-  const int r0 = group_at(p, lo), r1 = group_at(p, lo + 1);
+  const int r0 = begin[lo], r1 = begin[lo + 1];
   const int mt = (r1 - r0 + BM - 1) / BM;
   const int local = t - prefix[lo];
   const int band = local / (p.band * p.n_tiles);
@@ -168,29 +172,22 @@ __device__ __forceinline__ Tile tile_at(int t, const int* prefix, const Params& 
   return Tile{lo, r0 + (band * p.band + in % gm) * BM, r1, in / gm};
 }
 
-// Rows of a warp's tile to global memory through 2 KB of shared memory: 32
-// rows of 64 bytes, chunk c of row r at c ^ (r / 2 % 4), so that the row-wise
-// writes and the reads of 8 rows x 64 bytes are both free of bank conflicts.
-__device__ __forceinline__ void put_rows(uint4* stage, const uint4 (&v)[4], char* out, int64_t ld_bytes, int row0,
-                                         int row_end, int col_bytes, int end_bytes) {
-  const int lane = threadIdx.x & 31;
-  __syncwarp();
-#pragma unroll
-  for (int c = 0; c < 4; ++c) stage[lane * 4 + (c ^ ((lane >> 1) & 3))] = v[c];
-  __syncwarp();
-  const int c = lane & 3, at = col_bytes + c * 16;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2);
-    const uint4 u = stage[r * 4 + (c ^ ((r >> 1) & 3))];
-    if (row0 + r < row_end && at < end_bytes) *reinterpret_cast<uint4*>(out + (row0 + r) * ld_bytes + at) = u;
+// 32 bytes of this thread's row: one sector.  Every thread writes its own row; through
+// shared memory, eight rows of 64 bytes an instruction, 65536 x 2048 x 768 takes
+// 171 us instead of 163.
+__device__ __forceinline__ void put(char* at, bool wide, const uint32_t (&v)[8]) {
+  if (wide) {
+    store32(at, v);
+  } else {  // rows of 16-byte alignment
+    reinterpret_cast<uint4*>(at)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<uint4*>(at)[1] = make_uint4(v[4], v[5], v[6], v[7]);
   }
 }
 
 // --------------------------------------------------------------- kernel --
 template <int MODE>
 __device__ __forceinline__ bool tile_out(const Params& p, const Tile& tl, int row0, int half, float* acc,
-                                         uint4* stage, uint32_t* amax, int quad, uint32_t parity, uint32_t row_bar,
+                                         uint32_t* amax, int quad, uint32_t parity, uint32_t row_bar,
                                          volatile int* abort_flag) {
   const int lane = threadIdx.x & 31, row = row0 + lane;
   if constexpr (MODE == FP8_SWIGLU) {
@@ -209,46 +206,44 @@ __device__ __forceinline__ bool tile_out(const Params& p, const Tile& tl, int ro
     if (!mbar_wait_inline(row_bar, parity, abort_flag, p.err)) return false;
     m = max(m, mine[(half ^ 1) * 128]);
     const BlockScale s = block_scale(m);
-    uint4 v[4];
+    if (row < tl.m_end) {
+      const int col = tl.n * 128 + half * 64;
+      char* out = static_cast<char*>(p.out) + (int64_t)row * p.N + col;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t w[4];
+      for (int c = 0; c < 2; ++c) {
+        uint32_t w[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float* a = acc + c * 16 + j * 4;
-        w[j] = e4m3x4(a[0] * s.inv, a[1] * s.inv, a[2] * s.inv, a[3] * s.inv);
+        for (int j = 0; j < 8; ++j) {
+          const float* a = acc + c * 32 + j * 4;
+          w[j] = e4m3x4(a[0] * s.inv, a[1] * s.inv, a[2] * s.inv, a[3] * s.inv);
+        }
+        if (col + c * 32 + 32 <= p.N)
+          put(out + c * 32, p.wide, w);
+        else if (col + c * 32 < p.N)  // N ends after 16 of them
+          *reinterpret_cast<uint4*>(out + c * 32) = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      v[c] = make_uint4(w[0], w[1], w[2], w[3]);
+      if (half == 0) p.h_scale[(int64_t)tl.n * p.rows + row] = s.scale;
     }
-    put_rows(stage, v, static_cast<char*>(p.out), p.N, row0, tl.m_end, tl.n * 128 + half * 64, p.N);
-    if (half == 0 && row < tl.m_end) p.h_scale[(int64_t)tl.n * p.rows + row] = s.scale;
-  } else {
-    float s = 1.f;
-    if (MODE == FP8_SCALE && row < tl.m_end) s = p.wrow[row];
+  } else if (row < tl.m_end) {
+    const float s = MODE == FP8_SCALE ? p.wrow[row] : 1.f;
     const int col = tl.n * BN + half * 128;
     if (p.out_dtype == FRANK_F32) {
+      float* out = static_cast<float*>(p.out) + (int64_t)row * p.N + col;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint4 v[4];
+      for (int c = 0; c < 16; ++c) {
+        uint32_t v[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float* a = acc + c * 16 + j * 4;
-          v[j] = make_uint4(__float_as_uint(a[0] * s), __float_as_uint(a[1] * s), __float_as_uint(a[2] * s),
-                            __float_as_uint(a[3] * s));
-        }
-        put_rows(stage, v, static_cast<char*>(p.out), (int64_t)p.N * 4, row0, tl.m_end, (col + c * 16) * 4, p.N * 4);
+        for (int j = 0; j < 8; ++j) v[j] = __float_as_uint(acc[c * 8 + j] * s);
+        if (col + c * 8 < p.N) put(reinterpret_cast<char*>(out + c * 8), p.wide, v);
       }
     } else {
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + (int64_t)row * p.N + col;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint4 v[4];
+      for (int c = 0; c < 8; ++c) {
+        uint32_t v[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float* a = acc + c * 32 + j * 8;
-          v[j] = make_uint4(pack_bf16x2(a[0] * s, a[1] * s), pack_bf16x2(a[2] * s, a[3] * s),
-                            pack_bf16x2(a[4] * s, a[5] * s), pack_bf16x2(a[6] * s, a[7] * s));
-        }
-        put_rows(stage, v, static_cast<char*>(p.out), (int64_t)p.N * 2, row0, tl.m_end, (col + c * 32) * 2, p.N * 2);
+        for (int j = 0; j < 8; ++j) v[j] = pack_bf16x2(acc[c * 16 + 2 * j] * s, acc[c * 16 + 2 * j + 1] * s);
+        if (col + c * 16 < p.N) put(reinterpret_cast<char*>(out + c * 16), p.wide, v);
       }
     }
   }
@@ -260,12 +255,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* epi = smem + kStages * kStageBytes;
-  uint32_t* amax = reinterpret_cast<uint32_t*>(epi + kEpiBytes);  // [2 parities][2 halves][128 rows]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(epi + kEpiBytes + 2048);
+  uint32_t* amax = reinterpret_cast<uint32_t*>(smem + kStages * kStageBytes);  // [2 parities][2 halves][128 rows]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes + 2048);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* prefix = reinterpret_cast<int*>(tmem_slot + 4);  // [E + 1]
+  int* begin = prefix + p.E + 1;                         // [E + 1]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t bar0 = smem_u32(bars);
@@ -297,12 +292,14 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
   }
   pdl_wait();
   pdl_launch();
+  for (int e = threadIdx.x; e <= p.E; e += kThreads) begin[e] = group_at(p, e);
+  __syncthreads();
   if (warp == 0) {  // prefix[e] = tiles of the experts before e
     int carry = 0;
     for (int base = 0; base < p.E; base += 32) {
       const int e = base + lane;
       const int v =
-          e < p.E ? (max(group_at(p, e + 1) - group_at(p, e), 0) + BM - 1) / BM * p.n_tiles : 0;
+          e < p.E ? (max(begin[e + 1] - begin[e], 0) + BM - 1) / BM * p.n_tiles : 0;
       int incl = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -327,7 +324,7 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
       uint32_t it = 0;
       bool ok = true;
       for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        const Tile tl = tile_at(t, prefix, p);
+        const Tile tl = tile_at(t, prefix, begin, p);
         // a small group needs few rows of A: boxes of 128, 64, 32 or 16 rows
         int box = 0;
         while (box < 3 && tl.m_end - tl.m0 <= (64 >> box)) ++box;
@@ -350,7 +347,6 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
           }
         }
       }
-      if (!ok) outlast_copies();
     } else if (warp == 1 && lane == 0) {
       // ----------------------------------------------- MMA issuer --
       uint32_t it = 0;
@@ -379,7 +375,6 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
     // -------------------------------------------------- epilogue --
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
     const int quad = warp & 3, half = (warp - 4) >> 2;
-    uint4* stage = reinterpret_cast<uint4*>(epi + (warp - 4) * 2048);
     // columns of this warp: SWIGLU 64 of gate and the same 64 of up, else 128 in a row
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
     const uint32_t col0 = MODE == FP8_SWIGLU ? half * 64 : half * 128;
@@ -387,7 +382,7 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
     uint32_t it = 0, tiles = 0;  // K blocks; tiles with rows of this warp
     bool ok = true;
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      const Tile tl = tile_at(t, prefix, p);
+      const Tile tl = tile_at(t, prefix, begin, p);
       const int row0 = tl.m0 + quad * 32;
       const bool work = row0 < tl.m_end;
       // where the next scales are: blocks of 128 bytes in 180 GB fit 32 bits
@@ -439,13 +434,14 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
         }
       }
       if (ok && work)
-        ok = tile_out<MODE>(p, tl, row0, half, acc, stage, amax, quad, tiles++ & 1u, row_bar(quad), abort_flag);
+        ok = tile_out<MODE>(p, tl, row0, half, acc, amax, quad, tiles++ & 1u, row_bar(quad), abort_flag);
     }
   }
 
   fence_before();
   __syncthreads();
   if (warp == 1) {
+    if (*abort_flag) outlast_copies();
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
@@ -517,6 +513,8 @@ int launch_fp8_gemm(const Fp8Gemm& g, cudaStream_t st) {
   p.out_dtype = g.out_dtype;
   p.out = g.out;
   p.h_scale = g.h_scale;
+  const int64_t row_bytes = g.N * (g.mode == FP8_SWIGLU ? 1 : g.out_dtype == FRANK_F32 ? 4 : 2);
+  p.wide = (uintptr_t)g.out % 32 == 0 && row_bytes % 32 == 0;
   p.err = device_error_word();
   // rows of A that the CTAs share through L2 while they sweep the columns: 64 MB
   const int64_t band = (64ll << 20) / g.K / BM;
