@@ -967,13 +967,13 @@ int launch_few_experts(const FewArgs& args, int32_t* err, cudaStream_t st) {
     FRANK_CUDA_TRY(launch_chained(few_check_ids_kernel, dim3(1), dim3(256), 0, st, 1, a.ids, a.k * a.T, a.E, err));
     FRANK_LAUNCH_CHECK();
   }
-  FewMaps up, down;
+  FewMaps up{}, down{};
   FRANK_TRY(few_map(&up.w, a.w_gate, a.E, a.F, a.H, 128, true));
   FRANK_TRY(few_map(&up.w2, a.w_up, a.E, a.F, a.H, 128, true));
   FRANK_TRY(few_map(&down.w, a.w_down, a.E, a.H, a.F, 128, true));
   down.w2 = down.w;
-  for (int i = 0; i < 2; ++i) FRANK_TRY(few_map(&down.x[i], a.hq, 1, a.h_rows, a.F, 16u << i, false));
-  up.x[0] = up.x[1] = down.x[0];  // not read
+  for (int i = 0; i < tile_tokens(a.T) / 16; ++i)
+    FRANK_TRY(few_map(&down.x[i], a.hq, 1, a.h_rows, a.F, 16u << i, false));
   FRANK_TRY(launch_few_product<true>(up, a, st));
   return launch_few_product<false>(down, a, st);
 }

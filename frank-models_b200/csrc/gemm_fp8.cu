@@ -55,6 +55,13 @@ size_t smem_bytes(int64_t E) {
   return 1024 + kStages * kStageBytes + 2048 + 8 * (2 * kStages + 8) + 16 + 8 * (E + 1) + 64;
 }
 
+// A small group needs few rows of A: boxes of 128, 64, 32 or 16 rows.
+__host__ __device__ __forceinline__ int box_of(int64_t rows) {
+  int box = 0;
+  while (box < 3 && rows <= (64 >> box)) ++box;
+  return box;
+}
+
 struct Maps {
   CUtensorMap a[4];  // boxes of 128, 64, 32 and 16 rows
   CUtensorMap w, w2;
@@ -325,9 +332,7 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
       bool ok = true;
       for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
         const Tile tl = tile_at(t, prefix, begin, p);
-        // a small group needs few rows of A: boxes of 128, 64, 32 or 16 rows
-        int box = 0;
-        while (box < 3 && tl.m_end - tl.m0 <= (64 >> box)) ++box;
+        const int box = box_of(tl.m_end - tl.m0);
         const uint32_t a_bytes = kTileBytes >> box;
         for (int kb = 0; kb < p.nk; ++kb, ++it) {
           const int s = it % kStages;
@@ -493,8 +498,12 @@ namespace frank {
 
 int launch_fp8_gemm(const Fp8Gemm& g, cudaStream_t st) {
   if (g.rows == 0) return FRANK_OK;
-  Maps maps;
-  for (int i = 0; i < 4; ++i) FRANK_TRY(make_map(&maps.a[i], g.a, 1, g.rows, g.K, 128u >> i, false));
+  Maps maps{};
+  // one group of all rows has whole tiles and one rest at most (a map costs the host 0.4 us)
+  const int tail = box_of(g.rows % BM != 0 ? g.rows % BM : BM);
+  for (int i = 0; i < 4; ++i)
+    if (g.offsets != nullptr || i == tail || (i == 0 && g.rows > BM))
+      FRANK_TRY(make_map(&maps.a[i], g.a, 1, g.rows, g.K, 128u >> i, false));
   FRANK_TRY(make_map(&maps.w, g.w, g.E, g.N, g.K, 128, true));
   maps.w2 = maps.w;
   if (g.mode == FP8_SWIGLU) FRANK_TRY(make_map(&maps.w2, g.w2, g.E, g.N, g.K, 128, true));

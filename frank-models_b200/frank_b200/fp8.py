@@ -61,13 +61,16 @@ def _arg(t, name: str, shape=None, dtypes=FLOATS, device=None) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _new(rows: int, cols: int, dtype, device) -> torch.Tensor:
+    """[rows, cols]; empty_strided costs the host two thirds of empty."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
 def _out(out, name: str, shape, dtype, device, like: torch.Tensor | None = None) -> torch.Tensor:
     """The output: new, or the caller's (exact shape and dtype, contiguous, aligned).
     like: a contiguous tensor of the shape (empty_like costs the host half of empty)."""
     if out is None:
-        if like is not None and like.dtype == dtype:
-            return torch.empty_like(like)
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty_like(like) if like is not None and like.dtype == dtype else _new(*shape, dtype, device)
     if (not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(shape) or out.dtype != dtype
             or out.device != device or not out.is_contiguous() or out.data_ptr() % 16 != 0):
         raise ValueError(f"{name}: out must be contiguous, 16-byte aligned {dtype} {list(shape)} on {device}")
@@ -86,8 +89,8 @@ def quantize_fp8(x: torch.Tensor):
     T, K = x.shape
     _multiple(K, "quantize_fp8: K")
     with _on(x.device):
-        q = torch.empty((T, K), dtype=E4M3, device=x.device)
-        scale = torch.empty((_blocks(K), T), dtype=torch.float32, device=x.device)
+        q = _new(T, K, E4M3, x.device)
+        scale = _new(_blocks(K), T, torch.float32, x.device)
         _lib.check(_lib.load().frank_quantize_fp8(_DT[x.dtype], _ptr(x), T, K, _ptr(q), _ptr(scale), _stream()))
     return q, scale
 
@@ -100,9 +103,9 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, return_norm:
     _multiple(H, "rms_norm_fp8: H")
     weight = _arg(weight, "rms_norm_fp8: weight", (H,), F32_ONLY, x.device)
     with _on(x.device):
-        q = torch.empty((T, H), dtype=E4M3, device=x.device)
-        scale = torch.empty((_blocks(H), T), dtype=torch.float32, device=x.device)
-        xn = torch.empty((T, H), dtype=torch.bfloat16, device=x.device) if return_norm else None
+        q = _new(T, H, E4M3, x.device)
+        scale = _new(_blocks(H), T, torch.float32, x.device)
+        xn = _new(T, H, torch.bfloat16, x.device) if return_norm else None
         _lib.check(_lib.load().frank_rms_norm_fp8(_DT[x.dtype], _ptr(x), _ptr(weight), T, H, float(eps), _ptr(xn),
                                                   _ptr(q), _ptr(scale), _stream()))
     return (q, scale, xn) if return_norm else (q, scale)
@@ -188,9 +191,10 @@ def fp8_matmul(x, weights: Fp8Experts, offsets: torch.Tensor | None = None,
             _lib.check(lib.frank_fp8_matmul(_ptr(q), _ptr(scale), _ptr(weights.q), _ptr(weights.scale),
                                             _ptr(offsets), E, R, N, K, _DT[out_dtype], _ptr(y), _stream()))
         else:
-            ws = torch.empty(lib.frank_fp8_linear_workspace_size(R, K), dtype=torch.uint8, device=dev)
+            need = lib.frank_fp8_linear_workspace_size(R, K)
+            ws = weights.q.new_empty(need)
             _lib.check(lib.frank_fp8_linear(_DT[x.dtype], _ptr(x), _ptr(weights.q), _ptr(weights.scale),
-                                            _ptr(offsets), E, R, N, K, _DT[out_dtype], _ptr(y), _ptr(ws), ws.numel(),
+                                            _ptr(offsets), E, R, N, K, _DT[out_dtype], _ptr(y), _ptr(ws), need,
                                             _stream()))
     return y
 
@@ -249,8 +253,7 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
     def _routing(self, T, wanted):
         if not wanted:
             return None, None
-        return (torch.empty((self.k, T), dtype=torch.float32, device=self.device),
-                torch.empty((self.k, T), dtype=torch.int32, device=self.device))
+        return _new(self.k, T, torch.float32, self.device), _new(self.k, T, torch.int32, self.device)
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None, return_routing: bool = False):
         """moe_ffn_block on tokens x [T, H] bfloat16 -> y [T, H] in ``out_dtype``."""
