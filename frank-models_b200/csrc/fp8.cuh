@@ -72,6 +72,7 @@ struct Fp8Gemm {
 };
 int launch_fp8_gemm(const Fp8Gemm& g, cudaStream_t st);
 constexpr int64_t kFp8MaxE = 256;
+constexpr int64_t kFp8MaxRows = 0x7fffff00LL;  // a tile that begins below the last row ends inside 31 bits
 
 }  // namespace frank
 

@@ -103,7 +103,7 @@ static int check_moe(const char* what, int64_t T, int64_t E, int64_t k, int64_t 
   FRANK_CHECK_ARG(E >= 1 && E <= kFp8MaxE, "%s: n_expert=%lld outside [1, %lld]", what, (long long)E,
                   (long long)kFp8MaxE);
   FRANK_CHECK_ARG(k >= 1 && k <= E && k <= 32, "%s: n_expert_used=%lld outside [1, min(E, 32)]", what, (long long)k);
-  FRANK_CHECK_ARG(T >= 0 && k * T <= 0x7fffffffLL, "%s: T=%lld out of range", what, (long long)T);
+  FRANK_CHECK_ARG(T >= 0 && T <= kFp8MaxRows && k * T <= kFp8MaxRows, "%s: T=%lld out of range", what, (long long)T);
   FRANK_CHECK_ARG(H >= 16 && H % 16 == 0 && H <= kNormMaxH, "%s: n_embd=%lld is not a multiple of 16 in [16, %lld]",
                   what, (long long)H, (long long)kNormMaxH);
   FRANK_CHECK_ARG(F >= 16 && F % 16 == 0 && F <= 0x7fffffLL, "%s: n_ff=%lld is not a positive multiple of 16", what,
@@ -333,7 +333,7 @@ int frank_fp8_matmul(const void* q, const float* scale, const void* w, const flo
   FRANK_CHECK_ARG(offsets != nullptr || E == 1, "fp8_matmul: offsets may be omitted only for a single group");
   FRANK_CHECK_ARG(K >= 16 && K % 16 == 0 && K <= 0x7fffffLL && N >= 16 && N % 16 == 0 && N <= 0x7fffffLL,
                   "fp8_matmul: n_in=%lld and n_out=%lld must be positive multiples of 16", (long long)K, (long long)N);
-  FRANK_CHECK_ARG(rows >= 0 && rows <= 0x7fffffffLL, "fp8_matmul: rows=%lld out of range", (long long)rows);
+  FRANK_CHECK_ARG(rows >= 0 && rows <= kFp8MaxRows, "fp8_matmul: rows=%lld out of range", (long long)rows);
   if (rows == 0) return FRANK_OK;
   FRANK_CHECK_ARG(q && scale && w && w_scale && out, "fp8_matmul: null pointer");
   FRANK_CHECK_ARG(aligned16({q, w, out}), "fp8_matmul: q, w and out must be 16-byte aligned");

@@ -68,8 +68,11 @@ def test_library_refusals(lib):
     _refused(lib, lib.frank_fp8_matmul(P, P, P, P, None, 1, 4, 128, 128, 2, P, None), "dtype")
     _refused(lib, lib.frank_fp8_matmul(P + 8, P, P, P, None, 1, 4, 128, 128, 0, P, None), "aligned")
     _refused(lib, lib.frank_fp8_matmul(P, P, P, P, P, 257, 4, 128, 128, 0, P, None), "E=257")
+    _refused(lib, lib.frank_fp8_matmul(P, P, P, P, None, 1, 0x7fffff01, 16, 16, 0, P, None), "out of range")
     w = [P] * 6
     ws = 1 << 30
+    for T in (-1, 0x7fffff00 // 2 + 1, 1 << 62):
+        _refused(lib, lib.frank_fp8_moe_experts(P, P, P, *w, T, 8, 2, 128, 128, 0, P, None, P, ws, None), "out of range")
     _refused(lib, lib.frank_fp8_moe_experts(P, P, P, *w, 4, 8, 9, 128, 128, 0, P, None, P, ws, None), "n_expert_used")
     _refused(lib, lib.frank_fp8_moe_experts(P, P, P, *w, 4, 8, 2, 120, 128, 0, P, None, P, ws, None), "n_embd")
     _refused(lib, lib.frank_fp8_moe_experts(P, P, P, *w, 4, 8, 2, 128, 100, 0, P, None, P, ws, None), "n_ff")
