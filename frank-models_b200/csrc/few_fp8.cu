@@ -52,9 +52,11 @@ __device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
 __device__ __forceinline__ void st_peer(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
+// Of tensors that an earlier kernel may write while this one has started: not by __ldg, whose
+// reads may come from a stale line and need not stay behind pdl_wait.
 __device__ __forceinline__ float4 load4(const void* p, int dtype, int64_t i) {
-  if (dtype == FRANK_F32) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
-  const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + i));
+  if (dtype == FRANK_F32) return __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
+  const uint2 u = __ldcg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + i));
   return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
                      __uint_as_float(u.y & 0xffff0000u));
 }
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(const FewRoute
       float s = 0.f;
       for (int r = 0; r < kRouteCtas; ++r) s += ssq[r][t];
       const float inv = 1.f / sqrtf(s / (float)a.H + a.eps);
-      const float4 w = __ldg(reinterpret_cast<const float4*>(a.norm_w + h));
+      const float4 w = load4(a.norm_w, FRANK_F32, h);
       v = make_float4(v.x * inv * w.x, v.y * inv * w.y, v.z * inv * w.z, v.w * inv * w.w);
       v.x = __bfloat162float(__float2bfloat16_rn(v.x));
       v.y = __bfloat162float(__float2bfloat16_rn(v.y));

@@ -127,7 +127,8 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
 }
 
 // Programmatic dependent launch: blocks may start while the stream's previous
-// kernel finishes and wait here for its results.
+// kernel finishes and wait here for its results.  What that kernel may write is
+// no read-only data then: it is read by plain loads, __ldcg or copies.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" :::); }
 

@@ -396,10 +396,11 @@ fp8_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Param
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.f;
-      // scales of the next two K blocks: they come from L2 while the tensor core works
+      // scales of the next two K blocks: they come from L2 while the tensor core works.  The kernel
+      // before may have written those of the rows after this one started: not for __ldg.
       float a0 = 0.f, a1 = 0.f, w0 = 0.f, w1 = 0.f, u0 = 0.f, u1 = 0.f;
       auto next_scales = [&](float& fa, float& fw, float& fu) {
-        fa = __ldg(p.a_scale + ia), fw = __ldg(p.w_scale + iw);
+        fa = __ldcg(p.a_scale + ia), fw = __ldg(p.w_scale + iw);
         if (MODE == FP8_SWIGLU) fu = __ldg(p.w2_scale + iw);
         ia += (uint32_t)p.rows, ++iw;
       };

@@ -31,10 +31,12 @@ __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, flo
 
 constexpr int kPairs = 4;  // pairs of blocks a warp
 
+// x and slot_pos may be written until pdl_wait returns, so neither is __restrict__ (which would
+// allow reads through the read-only path).
 template <class TX>
 __global__ void __launch_bounds__(256)
-quantize_rows_kernel(const TX* __restrict__ x, int64_t T, int64_t K, int nb, const int32_t* __restrict__ slot_pos,
-                     int k, uint8_t* __restrict__ q, float* __restrict__ q_scale) {
+quantize_rows_kernel(const TX* x, int64_t T, int64_t K, int nb, const int32_t* slot_pos, int k, uint8_t* q,
+                     float* q_scale) {
   pdl_wait();
   pdl_launch();
   const int half = (threadIdx.x >> 4) & 1, l16 = threadIdx.x & 15;
@@ -43,6 +45,9 @@ quantize_rows_kernel(const TX* __restrict__ x, int64_t T, int64_t K, int nb, con
   if (seg * 2 * kPairs >= nb) return;
   const int64_t R = slot_pos != nullptr ? T * k : T;
   const int b0 = (int)seg * 2 * kPairs + half;
+  // lane j: the j-th place of this warp's row (k <= 32), asked for beside the row
+  const int lane = threadIdx.x & 31;
+  const int place = slot_pos != nullptr && lane < k ? slot_pos[lane * T + t] : 0;
   float v[kPairs][8];
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
@@ -66,7 +71,8 @@ quantize_rows_kernel(const TX* __restrict__ x, int64_t T, int64_t K, int nb, con
     u[i].y = e4m3x4(v[i][4] * s.inv, v[i][5] * s.inv, v[i][6] * s.inv, v[i][7] * s.inv);
   }
   for (int j = 0; j < k; ++j) {
-    const int64_t r = slot_pos != nullptr ? (int64_t)slot_pos[j * T + t] : t;
+    const int at = __shfl_sync(0xffffffffu, place, j);
+    const int64_t r = slot_pos != nullptr ? at : t;
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
       const int b = b0 + 2 * i;

@@ -132,3 +132,21 @@ def test_python_refusals():
         fb.Fp8MoEFFNBlock(x, x, x, x, 8, 2, False, out_dtype=torch.float16)
     with pytest.raises(ValueError, match="n_expert_used"):
         fb.Fp8MoEFFNBlock(x, x, x, x, 8, 9, False)
+
+
+def test_chained_kernels_read_what_may_change_coherently():
+    """A kernel that starts before its predecessor has ended may take the read-only path (`__ldg`, or a pointer to const
+    that is `__restrict__`) only for expert weights' scales: all else may be written while it runs."""
+    import re
+    from pathlib import Path
+
+    csrc = Path(__file__).resolve().parent.parent / "frank-models_b200" / "csrc"
+    scales = re.compile(r"p\.w2?_scale \+ |\(UP \? a\.s_gate : a\.s_down\) \+ |a\.s_up \+ ")
+    for name in ("quantize_fp8.cu", "gemm_fp8.cu", "few_fp8.cu", "norm.cu"):
+        code = re.sub(r"//[^\n]*", "", (csrc / name).read_text())
+        for m in re.finditer(r"__ldg\(([^;]{0,60})", code):
+            assert scales.match(m.group(1)), (name, m.group(0))
+        for kernel in re.split(r"__global__", code)[1:]:
+            params, _, body = kernel.partition("{")
+            if "pdl_wait" in body:
+                assert not re.search(r"const [\w:]+\s*\* ?__restrict__", params), (name, params)

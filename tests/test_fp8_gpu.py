@@ -548,3 +548,34 @@ def test_weights_replaced():
     c.wr, c.wr_pack = b.wr, b.wr_pack
     b.w_up, b.w_gate, b.w_down = c.w_up, c.w_gate, c.w_down
     assert torch.equal(b(x), c(x))
+
+
+@pytest.mark.parametrize("T", [3, 100])
+def test_chains_without_a_pause(T):
+    """Calls that each read what the call before has just written, in buffers that are used again with new values
+    every round: the bits of the same calls with a synchronisation after each."""
+    g = gen(24)
+    H = 512
+    b = block(g, T, H, 256, 16, 4)
+    nw, pw = 1 + randn(g, H, std=0.1), 1 + randn(g, H, std=0.1)
+    lin = weights(g, 1, H, H)
+    inputs = [randn(g, T, H, dtype=BF16) for _ in range(40)]
+    buf, mid = torch.empty_like(inputs[0]), torch.empty_like(inputs[0])
+
+    def chain(x, pause):
+        buf.copy_(x)
+        for _ in range(3):
+            b.sublayer(buf, nw, 1e-5, post_norm_w=pw, out=buf)
+            pause()
+            fb.post_norm_residual(buf, buf, pw, 1e-5, out=mid)
+            pause()
+            q, s = fb.quantize_fp8(mid)
+            pause()
+            fb.fp8_matmul((q, s), lin, out=buf)
+            pause()
+        return buf.clone()
+
+    want = [chain(x, torch.cuda.synchronize) for x in inputs]
+    got = [chain(x, lambda: None) for x in inputs]
+    for a, w in zip(got, want):
+        assert torch.equal(a, w)
