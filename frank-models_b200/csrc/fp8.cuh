@@ -20,8 +20,7 @@ struct NormRows {
   // source: y [T, H], or the sum over k slots of d (rows at slot_pos[j*T+t], or j*T+t)
   int y_dtype = FRANK_F32;
   const void* y = nullptr;
-  int d_dtype = FRANK_F32;
-  const void* d = nullptr;
+  const float* d = nullptr;
   const int32_t* slot_pos = nullptr;
   int k = 0;
   // v = residual_scale * residual + gate * (post_w ? rms_norm(v, post_w) : v)
@@ -52,7 +51,7 @@ int launch_prepack_fp8(int in_dtype, const void* src, int64_t O, int64_t I, int6
 
 // Grouped product of 8-bit rows and weights (gemm_fp8.cu).
 //   PLAIN : out [rows, N] in out_dtype
-//   SCALE : out [rows, N] in out_dtype, row r times wrow[r]
+//   SCALE : out fp32 [rows, N], row r times wrow[r]
 //   SWIGLU: w = gate, w2 = up; h = gate * silu(up) quantised -> out e4m3 [rows, N], h_scale [ceil(N/128), rows]
 enum Fp8Mode { FP8_PLAIN = 0, FP8_SCALE = 1, FP8_SWIGLU = 2 };
 struct Fp8Gemm {

@@ -62,7 +62,7 @@ struct Fp8MoeWs {
   float* xs;              // [H/128, n]
   uint8_t* hq;            // [n, F]
   float* hs;              // [F/128, n]
-  void* d;                // [n, H], see d_dtype
+  float* d;               // [n, H]
   float* partial;         // a few tokens: partial sums of divided tiles, and their counters
   int32_t* count;
   float* logits;
@@ -88,7 +88,7 @@ static size_t fp8_moe_layout(int64_t T, int64_t H, int64_t F, int64_t E, int64_t
   l.xs = c.take<float>((few ? kFewMaxT : n) * q_blocks(H));
   l.hq = c.take<uint8_t>(h_rows * F);
   l.hs = c.take<float>(h_rows * q_blocks(F));
-  l.d = c.take<float>(n * H);  // enough for either type
+  l.d = c.take<float>(n * H);
   l.partial = c.take<float>(few ? few_partials(T) : 0);
   l.count = c.take<int32_t>(few ? few_counts(T, E, k, H, F) : 0);
   l.logits = c.take<float>(router_scratch_bytes(FRANK_BF16, T, H, E) / sizeof(float) + 1);
@@ -135,7 +135,7 @@ static FewArgs few_args(const Fp8Weights& W, int64_t T, int64_t E, int64_t k, in
   a.count = L.count;
   a.hq = L.hq;
   a.hs = L.hs;
-  a.d = static_cast<float*>(L.d);
+  a.d = L.d;
   a.w = w;
   a.ids = ids;
   a.T = (int)T;
@@ -170,17 +170,9 @@ static FewRoute few_route(int x_dtype, const void* x, const float* norm_w, float
   return r;
 }
 
-// The products of a prompt's slots leave in the type of the result: for a bf16 result each
-// slot is rounded once more (half a step of bf16 of its own share of the sum) and
-// the 2 k bytes a value written and read are halved, which end the tiles of a short
-// K: 271 -> 214 us for the down product of 65536 slots, 2048 from 768.  A few
-// tokens' slots and fp32 results stay in fp32.
-static int d_dtype(int y_dtype, int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
-  return few_tokens(T, E, k, H, F) ? FRANK_F32 : y_dtype;
-}
-
-// Routed rows through the experts: L.d[r] = w * down(q(h)) for the expert-sorted rows r.
-static int run_experts(int y_dtype, const void* x, const float* w, const int32_t* ids, const Fp8Weights& W, int64_t T, int64_t E,
+// Routed rows through the experts: L.d[r] = w * down(q(h)) for the expert-sorted rows r, in
+// fp32 whatever the result's type: the sum over a token's slots, and the norm after it, round once.
+static int run_experts(const void* x, const float* w, const int32_t* ids, const Fp8Weights& W, int64_t T, int64_t E,
                        int64_t k, int64_t H, int64_t F, int32_t* err, const Fp8MoeWs& L, cudaStream_t st) {
   const int64_t n = k * T;
   if (few_tokens(T, E, k, H, F)) {
@@ -219,7 +211,6 @@ static int run_experts(int y_dtype, const void* x, const float* w, const int32_t
   d.N = H;
   d.K = F;
   d.wrow = L.wsorted;
-  d.out_dtype = y_dtype;
   d.out = L.d;
   return launch_fp8_gemm(d, st);
 }
@@ -227,7 +218,6 @@ static int run_experts(int y_dtype, const void* x, const float* w, const int32_t
 static NormRows combine_of(const Fp8MoeWs& L, int64_t T, int64_t E, int64_t k, int64_t H, int64_t F, int out_dtype,
                            void* out) {
   NormRows a;
-  a.d_dtype = d_dtype(out_dtype, T, E, k, H, F);
   a.d = L.d;
   a.slot_pos = few_tokens(T, E, k, H, F) ? nullptr : L.slot_pos;
   a.k = (int)k;
@@ -239,7 +229,7 @@ static NormRows combine_of(const Fp8MoeWs& L, int64_t T, int64_t E, int64_t k, i
 }
 
 // The block up to L.d: x [T, H] bf16, or with norm_w the residual it is normalised from.
-static int route_and_run(int y_dtype, int x_dtype, const void* x, const float* norm_w, float eps, int wr_dtype, const void* wr,
+static int route_and_run(int x_dtype, const void* x, const float* norm_w, float eps, int wr_dtype, const void* wr,
                          const Fp8Weights& W, int64_t T, int64_t E, int64_t k, int64_t H, int64_t F, int normalize,
                          float* w, int32_t* ids, const Fp8MoeWs& L, cudaStream_t st) {
   const __nv_bfloat16* wr3 = nullptr;
@@ -267,7 +257,7 @@ static int route_and_run(int y_dtype, int x_dtype, const void* x, const float* n
     x = L.xn;
   }
   FRANK_TRY(launch_router_topk(FRANK_BF16, x, wr_dtype, wr, T, H, E, k, normalize, w, ids, L.logits, st, wr3));
-  return run_experts(y_dtype, x, w, ids, W, T, E, k, H, F, nullptr, L, st);
+  return run_experts(x, w, ids, W, T, E, k, H, F, nullptr, L, st);
 }
 
 static int check_gate(const char* what, const float* gate, int64_t gate_rows, int64_t T) {
@@ -387,7 +377,7 @@ int frank_fp8_moe_experts(const void* x, const float* route_w, const int32_t* ro
   cudaStream_t st = as_stream(stream);
   Fp8MoeWs L;
   fp8_moe_layout(T, H, F, E, k, workspace, ws_bytes, &L);
-  FRANK_TRY(run_experts(y_dtype, x, route_w, route_ids, W, T, E, k, H, F, err_flag, L, st));
+  FRANK_TRY(run_experts(x, route_w, route_ids, W, T, E, k, H, F, err_flag, L, st));
   return launch_norm_rows(combine_of(L, T, E, k, H, F, y_dtype, y), st);
 }
 
@@ -406,7 +396,7 @@ int frank_fp8_moe_block(const void* x, int wr_dtype, const void* wr, const void*
   fp8_moe_layout(T, H, F, E, k, workspace, ws_bytes, &L);
   float* w = route_w ? route_w : L.w;
   int32_t* ids = route_ids ? route_ids : L.ids;
-  FRANK_TRY(route_and_run(y_dtype, FRANK_BF16, x, nullptr, 0.f, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
+  FRANK_TRY(route_and_run(FRANK_BF16, x, nullptr, 0.f, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
   return launch_norm_rows(combine_of(L, T, E, k, H, F, y_dtype, y), st);
 }
 
@@ -429,7 +419,7 @@ int frank_fp8_moe_sublayer(int res_dtype, const void* residual, const float* nor
   float* w = route_w ? route_w : L.w;
   int32_t* ids = route_ids ? route_ids : L.ids;
   FRANK_TRY(
-      route_and_run(res_dtype, res_dtype, residual, norm_w, eps, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
+      route_and_run(res_dtype, residual, norm_w, eps, wr_dtype, wr, W, T, E, k, H, F, normalize, w, ids, L, st));
   NormRows a = combine_of(L, T, E, k, H, F, res_dtype, out);
   a.post_w = post_w;
   a.eps = eps;

@@ -234,7 +234,7 @@ __device__ __forceinline__ bool tile_out(const Params& p, const Tile& tl, int ro
   } else if (row < tl.m_end) {
     const float s = MODE == FP8_SCALE ? p.wrow[row] : 1.f;
     const int col = tl.n * BN + half * 128;
-    if (p.out_dtype == FRANK_F32) {
+    if (MODE == FP8_SCALE || p.out_dtype == FRANK_F32) {
       float* out = static_cast<float*>(p.out) + (int64_t)row * p.N + col;
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
@@ -249,7 +249,7 @@ __device__ __forceinline__ bool tile_out(const Params& p, const Tile& tl, int ro
       for (int c = 0; c < 8; ++c) {
         uint32_t v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = pack_bf16x2(acc[c * 16 + 2 * j] * s, acc[c * 16 + 2 * j + 1] * s);
+        for (int j = 0; j < 8; ++j) v[j] = pack_bf16x2(acc[c * 16 + 2 * j], acc[c * 16 + 2 * j + 1]);
         if (col + c * 16 < p.N) put(reinterpret_cast<char*>(out + c * 16), p.wide, v);
       }
     }

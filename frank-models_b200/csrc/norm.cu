@@ -126,7 +126,7 @@ norm_rows_kernel(const NormRows a) {
       for (int q = 0; q < kAhead; ++q) {
         const int64_t s = (int64_t)(j0 + q) * a.T + t;
         if (j0 + q < a.k)
-          load_row<GS, V>(u[q], a.d, a.d_dtype, (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * n, tid, n);
+          load_row<GS, V>(u[q], a.d, FRANK_F32, (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * n, tid, n);
       }
 #pragma unroll
       for (int q = 0; q < kAhead; ++q)
@@ -174,14 +174,13 @@ norm_rows_kernel(const NormRows a) {
 }
 
 // y[t] = sum_j d[slot_pos[j]] alone: eight columns a thread, eight rows at a time.
-template <class TD, class TY>
+template <class TY>
 __global__ void __launch_bounds__(128) combine_slots_kernel(const NormRows a) {
   pdl_wait();
   pdl_launch();
   const int64_t t = blockIdx.x;
   const int h = (blockIdx.y * 128 + threadIdx.x) * 8;
   if (h >= a.H) return;
-  const TD* d = static_cast<const TD*>(a.d);
   float v[8] = {};
   for (int j0 = 0; j0 < a.k; j0 += 8) {
     float4 u[8][2];
@@ -189,17 +188,9 @@ __global__ void __launch_bounds__(128) combine_slots_kernel(const NormRows a) {
     for (int q = 0; q < 8; ++q) {
       if (j0 + q < a.k) {
         const int64_t s = (int64_t)(j0 + q) * a.T + t;
-        const TD* row = d + (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * a.H + h;
-        if constexpr (sizeof(TD) == 4) {
-          u[q][0] = *reinterpret_cast<const float4*>(row);
-          u[q][1] = *reinterpret_cast<const float4*>(row + 4);
-        } else {
-          const uint4 p = *reinterpret_cast<const uint4*>(row);
-          u[q][0] = make_float4(__uint_as_float(p.x << 16), __uint_as_float(p.x & 0xffff0000u),
-                                __uint_as_float(p.y << 16), __uint_as_float(p.y & 0xffff0000u));
-          u[q][1] = make_float4(__uint_as_float(p.z << 16), __uint_as_float(p.z & 0xffff0000u),
-                                __uint_as_float(p.w << 16), __uint_as_float(p.w & 0xffff0000u));
-        }
+        const float* row = a.d + (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * a.H + h;
+        u[q][0] = *reinterpret_cast<const float4*>(row);
+        u[q][1] = *reinterpret_cast<const float4*>(row + 4);
       }
     }
 #pragma unroll
@@ -227,12 +218,11 @@ cudaError_t launch_rows(const NormRows& a, cudaStream_t st) {
                         : launch_chained(norm_rows_kernel<GS, V, false>, grid, block, 0, st, 1, a);
 }
 
-template <class TD>
 cudaError_t launch_combine_slots(const NormRows& a, cudaStream_t st) {
   const dim3 grid((unsigned)a.T, (unsigned)((a.H + 1023) / 1024));
   if (a.out_dtype == FRANK_F32)
-    return launch_chained(combine_slots_kernel<TD, float>, grid, dim3(128), 0, st, 1, a);
-  return launch_chained(combine_slots_kernel<TD, __nv_bfloat16>, grid, dim3(128), 0, st, 1, a);
+    return launch_chained(combine_slots_kernel<float>, grid, dim3(128), 0, st, 1, a);
+  return launch_chained(combine_slots_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, 1, a);
 }
 
 }  // namespace
@@ -245,7 +235,7 @@ int launch_norm_rows(const NormRows& a, cudaStream_t st) {
   cudaError_t e;
   if (a.d != nullptr && a.post_w == nullptr && a.gate == nullptr && a.residual == nullptr && a.next_w == nullptr &&
       a.H % 8 == 0)
-    e = a.d_dtype == FRANK_F32 ? launch_combine_slots<float>(a, st) : launch_combine_slots<__nv_bfloat16>(a, st);
+    e = launch_combine_slots(a, st);
   else if (H4 <= 32) e = launch_rows<32, 1>(a, st);
   else if (H4 <= 64) e = launch_rows<32, 2>(a, st);
   else if (H4 <= 128) e = launch_rows<32, 4>(a, st);

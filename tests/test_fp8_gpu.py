@@ -579,3 +579,24 @@ def test_chains_without_a_pause(T):
     got = [chain(x, lambda: None) for x in inputs]
     for a, w in zip(got, want):
         assert torch.equal(a, w)
+
+
+@pytest.mark.parametrize("T,H,F,E,k", [(64, 256, 272, 2, 2), (200, 144, 272, 12, 2), (700, 512, 384, 4, 2),
+                                       (65, 1040, 96, 130, 6), (90, 256, 128, 32, 32)])
+def test_prompt_slots_stay_in_fp32(T, H, F, E, k):
+    """A prompt's products are summed over the slots in fp32 and a bf16 result is rounded once: the bound of the fp32
+    result and half a step; a sub-layer's post-norm sees the fp32 sums."""
+    g = gen(T + 25)
+    b = block(g, T, H, F, E, k)
+    assert prompt(T, b)
+    x = randn(g, T, H, dtype=BF16)
+    rid = torch.rand((T, E), generator=g, device=DEV).topk(k, 1)[1].t().to(torch.int32).contiguous()
+    rw = torch.rand((k, T), generator=g, device=DEV)
+    want, bound, _ = Q.moe_experts(x.double(), rw.double(), rid, dense(b.w_gate), dense(b.w_up), dense(b.w_down))
+    y = b.experts(x, rw, rid)
+    within(y, want, bound)
+    f = fb.Fp8MoEFFNBlock(b.wr, b.w_up, b.w_gate, b.w_down, E, k, True, out_dtype=F32)
+    assert torch.equal(y, f.experts(x, rw, rid).to(BF16))
+    nw, pw = 1 + randn(g, H, std=0.1), 1 + randn(g, H, std=0.1)
+    xn = fb.rms_norm_fp8(x, nw, 1e-5, return_norm=True)[2]
+    assert torch.equal(b.sublayer(x, nw, 1e-5, post_norm_w=pw), fb.post_norm_residual(f(xn), x, pw, 1e-5))
