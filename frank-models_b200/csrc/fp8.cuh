@@ -101,13 +101,16 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t amax) {
 
 // silu(u) = u / (1 + 2^(-u log2 e)) by CUDA's approximate exponential and division (2 ulp
 // each); 64 of them end a tile of a product.  The exponent's rounding error is put
-// back as a factor 1 + ln 2 * error.  The clamp keeps 2^t finite; below it the result is 0.
-// An infinite u gives NaN, which its block of 128 becomes in any case.
+// back as a factor 1 + ln 2 * error.  u is clamped to +-88 in the exponent, where 2^t and
+// the error stay finite: above, the divisor is 1 and the result u, also for the largest
+// finite u; below, the divisor is over 2^126, for which the approximate division gives 0.
+// An infinite or NaN u gives infinity or NaN, and its block of 128 the scale NaN.
 __device__ __forceinline__ float silu(float u) {
-  const float t = fminf(u * -1.44269502f, 126.f);
+  const float c = fminf(fmaxf(u, -88.f), 88.f);
+  const float t = c * -1.44269502f;
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  const float lost = fmaf(u, -1.92596299e-8f, fmaf(u, -1.44269502f, -t));
+  const float lost = fmaf(c, -1.92596299e-8f, fmaf(c, -1.44269502f, -t));
   return __fdividef(u, 1.f + fmaf(e * 0.693147182f, lost, e));
 }
 

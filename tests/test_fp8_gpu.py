@@ -600,3 +600,24 @@ def test_prompt_slots_stay_in_fp32(T, H, F, E, k):
     nw, pw = 1 + randn(g, H, std=0.1), 1 + randn(g, H, std=0.1)
     xn = fb.rms_norm_fp8(x, nw, 1e-5, return_norm=True)[2]
     assert torch.equal(b.sublayer(x, nw, 1e-5, post_norm_w=pw), fb.post_norm_residual(f(xn), x, pw, 1e-5))
+
+
+@pytest.mark.parametrize("T", [3, 100])
+def test_silu_up_to_the_largest_number(T):
+    """Finite up-products to 3e38, past where their exponent overflows: silu(u) is u (or 0), not NaN."""
+    g = gen(26)
+    H, F, E = 144, 272, 2
+    up, gate, down = weights(g, E, F, H), weights(g, E, F, H), weights(g, E, H, F)
+    up.q[:, :, 0] = (torch.randn((E, F), generator=g, device=DEV) * 300).clamp_(-448, 448).to(E4M3)
+    up.q[:, :4, 0] = torch.tensor([448.0, -448.0, 352.0, -352.0], device=DEV).to(E4M3)
+    up.scale.fill_(3.2e38 / 448)
+    gate.scale.fill_(1e-32)
+    b = fb.Fp8MoEFFNBlock(randn(g, E, H), up, gate, down, E, 1, False, out_dtype=F32)
+    x = torch.zeros((T, H), dtype=BF16, device=DEV)
+    x[:, 0] = 1.0
+    x[T - 1, 0] = -1.0
+    rw = torch.ones((1, T), device=DEV)
+    rid = torch.randint(0, E, (1, T), generator=g, device=DEV, dtype=torch.int32)
+    y = b.experts(x, rw, rid)
+    assert torch.isfinite(y).all() and (y != 0).any()
+    within(y, *want_moe(b, x, rw, rid))
