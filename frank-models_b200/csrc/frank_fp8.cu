@@ -260,6 +260,21 @@ static int route_and_run(int x_dtype, const void* x, const float* norm_w, float 
   return run_experts(x, w, ids, W, T, E, k, H, F, nullptr, L, st);
 }
 
+// The arguments of a product of rows x, quantised or to be quantised.
+static int check_matmul(const char* what, const void* x, const void* w, const float* w_scale, const int32_t* offsets,
+                        int64_t E, int64_t rows, int64_t N, int64_t K, int out_dtype, const void* out) {
+  FRANK_TRY(check_float_dtype(out_dtype, what));
+  FRANK_CHECK_ARG(E >= 1 && E <= kFp8MaxE, "%s: E=%lld outside [1, %lld]", what, (long long)E, (long long)kFp8MaxE);
+  FRANK_CHECK_ARG(offsets != nullptr || E == 1, "%s: offsets may be omitted only for a single group", what);
+  FRANK_CHECK_ARG(K >= 16 && K % 16 == 0 && K <= 0x7fffffLL && N >= 16 && N % 16 == 0 && N <= 0x7fffffLL,
+                  "%s: n_in=%lld and n_out=%lld must be positive multiples of 16", what, (long long)K, (long long)N);
+  FRANK_CHECK_ARG(rows >= 0 && rows <= kFp8MaxRows, "%s: rows=%lld out of range", what, (long long)rows);
+  if (rows == 0) return FRANK_OK;
+  FRANK_CHECK_ARG(x && w && w_scale && out, "%s: null pointer", what);
+  FRANK_CHECK_ARG(aligned16({x, w, out}), "%s: rows, w and out must be 16-byte aligned", what);
+  return FRANK_OK;
+}
+
 static int check_gate(const char* what, const float* gate, int64_t gate_rows, int64_t T) {
   if (gate == nullptr) return FRANK_OK;
   FRANK_CHECK_ARG(gate_rows >= 1 && T % gate_rows == 0, "%s: gate_rows=%lld does not divide T=%lld", what,
@@ -318,15 +333,9 @@ int frank_prepack_experts_fp8(int in_dtype, const void* w_oie, int64_t O, int64_
 
 int frank_fp8_matmul(const void* q, const float* scale, const void* w, const float* w_scale, const int32_t* offsets,
                      int64_t E, int64_t rows, int64_t N, int64_t K, int out_dtype, void* out, void* stream) {
-  FRANK_TRY(check_float_dtype(out_dtype, "fp8_matmul"));
-  FRANK_CHECK_ARG(E >= 1 && E <= kFp8MaxE, "fp8_matmul: E=%lld outside [1, %lld]", (long long)E, (long long)kFp8MaxE);
-  FRANK_CHECK_ARG(offsets != nullptr || E == 1, "fp8_matmul: offsets may be omitted only for a single group");
-  FRANK_CHECK_ARG(K >= 16 && K % 16 == 0 && K <= 0x7fffffLL && N >= 16 && N % 16 == 0 && N <= 0x7fffffLL,
-                  "fp8_matmul: n_in=%lld and n_out=%lld must be positive multiples of 16", (long long)K, (long long)N);
-  FRANK_CHECK_ARG(rows >= 0 && rows <= kFp8MaxRows, "fp8_matmul: rows=%lld out of range", (long long)rows);
+  FRANK_TRY(check_matmul("fp8_matmul", q, w, w_scale, offsets, E, rows, N, K, out_dtype, out));
   if (rows == 0) return FRANK_OK;
-  FRANK_CHECK_ARG(q && scale && w && w_scale && out, "fp8_matmul: null pointer");
-  FRANK_CHECK_ARG(aligned16({q, w, out}), "fp8_matmul: q, w and out must be 16-byte aligned");
+  FRANK_CHECK_ARG(scale != nullptr, "fp8_matmul: null pointer");
   Fp8Gemm g;
   g.a = q;
   g.a_scale = scale;
@@ -349,12 +358,16 @@ size_t frank_fp8_linear_workspace_size(int64_t rows, int64_t K) {
 int frank_fp8_linear(int x_dtype, const void* x, const void* w, const float* w_scale, const int32_t* offsets,
                      int64_t E, int64_t rows, int64_t N, int64_t K, int out_dtype, void* out, void* workspace,
                      size_t ws_bytes, void* stream) {
-  if (rows == 0) return frank_fp8_matmul(nullptr, nullptr, w, w_scale, offsets, E, 0, N, K, out_dtype, out, stream);
-  if (rows > 0 && K > 0 && (workspace == nullptr || ws_bytes < frank_fp8_linear_workspace_size(rows, K))) {
-    set_error("fp8_linear: workspace %zu < %zu bytes", workspace ? ws_bytes : (size_t)0,
-              frank_fp8_linear_workspace_size(rows, K));
+  // everything is checked before the rows are quantised: a refused call launches nothing
+  FRANK_TRY(check_float_dtype(x_dtype, "fp8_linear"));
+  FRANK_TRY(check_matmul("fp8_linear", x, w, w_scale, offsets, E, rows, N, K, out_dtype, out));
+  if (rows == 0) return FRANK_OK;
+  const size_t need = frank_fp8_linear_workspace_size(rows, K);
+  if (workspace == nullptr || ws_bytes < need) {
+    set_error("fp8_linear: workspace %zu < %zu bytes", workspace ? ws_bytes : (size_t)0, need);
     return FRANK_ENOSPC;
   }
+  FRANK_CHECK_ARG(aligned16({workspace}), "fp8_linear: workspace must be 16-byte aligned");
   float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up((size_t)rows * K, 256));
   FRANK_TRY(frank_quantize_fp8(x_dtype, x, rows, K, workspace, scale, stream));
   return frank_fp8_matmul(workspace, scale, w, w_scale, offsets, E, rows, N, K, out_dtype, out, stream);

@@ -150,3 +150,31 @@ def test_chained_kernels_read_what_may_change_coherently():
             params, _, body = kernel.partition("{")
             if "pdl_wait" in body:
                 assert not re.search(r"const [\w:]+\s*\* ?__restrict__", params), (name, params)
+
+
+def test_linear_refuses_before_it_launches(lib):
+    """What the product would refuse, frank_fp8_linear refuses before the rows are quantised: no launch is tried."""
+    from frank_b200 import _lib
+
+    ws = 1 << 20
+    linear = lambda off, E, rows, N, K, out_dtype=0, x=P, x_dtype=0, w=P, sw=P, out=P, ptr=P: lib.frank_fp8_linear(  # noqa: E731
+        x_dtype, x, w, sw, off, E, rows, N, K, out_dtype, out, ptr, ws, None)
+    _refused(lib, linear(None, 1, 4, 120, 128), "multiples of 16")
+    _refused(lib, linear(None, 1, 4, 128, 136), "multiple")
+    _refused(lib, linear(None, 2, 4, 128, 128), "offsets")
+    _refused(lib, linear(P, 257, 4, 128, 128), "E=257")
+    _refused(lib, linear(None, 1, 4, 128, 128, out_dtype=2), "dtype")
+    _refused(lib, linear(None, 1, 4, 128, 128, x_dtype=2), "dtype")
+    _refused(lib, linear(None, 1, 4, 128, 128, x=None), "null")
+    _refused(lib, linear(None, 1, 4, 128, 128, w=None), "null")
+    _refused(lib, linear(None, 1, 4, 128, 128, sw=None), "null")
+    _refused(lib, linear(None, 1, 4, 128, 128, out=None), "null")
+    _refused(lib, linear(None, 1, 4, 128, 128, x=P + 4), "aligned")
+    _refused(lib, linear(None, 1, 4, 128, 128, w=P + 8), "aligned")
+    _refused(lib, linear(None, 1, 4, 128, 128, out=P + 8), "aligned")
+    _refused(lib, linear(None, 1, 4, 128, 128, ptr=P + 8), "aligned")
+    _refused(lib, linear(None, 1, -1, 128, 128), "out of range")
+    _refused(lib, linear(None, 1, 0x7fffff01, 16, 16), "out of range")
+    _refused(lib, linear(None, 1, 4, 128, -16), "multiple")
+    assert linear(None, 1, 4, 128, 128, ptr=None) == _lib.ENOSPC
+    assert linear(None, 1, 1 << 20, 128, 128) == _lib.ENOSPC
