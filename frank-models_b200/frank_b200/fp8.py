@@ -215,7 +215,9 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
     """:class:`MoEFFNBlock` with 8-bit expert weights: tokens in bfloat16, rows
     and the hidden values quantised in blocks of 128 on the way, sums in fp32.
     The expert weights are :class:`Fp8Experts` or the reference layouts (up/gate
-    [F, H, E], down [H, F, E]), which are quantised once here."""
+    [F, H, E], down [H, F, E]), which are quantised once here.  A call reads the
+    expert weights that ``w_up``, ``w_gate`` and ``w_down`` are then, in-place changes
+    included, and the router that ``wr`` was when it was last assigned."""
 
     def __init__(self, gate_inp_w, up_exps_w, gate_exps_w, down_exps_w, n_expert: int, n_expert_used: int,
                  normalize_weights: bool, out_dtype: torch.dtype = torch.float32):
@@ -236,9 +238,26 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
         self.H, self.F = H, F
         self.w_up, self.w_gate, self.w_down = up, gate, down
         self.device = up.q.device
-        self.wr = _arg(gate_inp_w, "gate_inp_w", (E, H), device=self.device)
+        self.wr_pack = None
+        self.wr = gate_inp_w
+
+    @property
+    def wr(self) -> torch.Tensor:
+        """The router [E, H].  Calls read its packed form ``wr_pack``, which assigning ``wr`` rewrites in place on the
+        current stream, so captured graphs take the new router up too.  After a change of ``wr`` in place, assign it
+        again (``block.wr = block.wr``)."""
+        return self._wr
+
+    @wr.setter
+    def wr(self, gate_inp_w: torch.Tensor) -> None:
+        wr = _arg(gate_inp_w, "gate_inp_w", (self.E, self.H), device=self.device)
         with _on(self.device):
-            self.wr_pack = ops.router_pack(self.wr)
+            pack = ops.router_pack(wr)
+            if self.wr_pack is None:
+                self.wr_pack = pack
+            else:
+                self.wr_pack.copy_(pack)
+        self._wr = wr
 
     def _weights(self):
         return [_ptr(t) for w in (self.w_up, self.w_gate, self.w_down) for t in (w.q, w.scale)]

@@ -621,3 +621,27 @@ def test_silu_up_to_the_largest_number(T):
     y = b.experts(x, rw, rid)
     assert torch.isfinite(y).all() and (y != 0).any()
     within(y, *want_moe(b, x, rw, rid))
+
+
+@pytest.mark.parametrize("T", [3, 200])
+def test_router_replaced(T):
+    """A block routes by the router it has when it is called; one changed in place is taken up by assigning it again."""
+    g = gen(27)
+    b = block(g, T, 256, 256, 8, 2, out_dtype=F32)
+    x = randn(g, T, 256, dtype=BF16)
+    b(x)
+    fresh = lambda wr: fb.Fp8MoEFFNBlock(wr, b.w_up, b.w_gate, b.w_down, 8, 2, True, out_dtype=F32)  # noqa: E731
+    step = ops.GraphedMoEFFN(b, T)
+    for wr in (randn(g, 8, 256), randn(g, 8, 256, dtype=BF16), randn(g, 256, 8).t()):
+        b.wr = wr
+        want = fresh(wr)(x, return_routing=True)
+        assert all(torch.equal(a, w) for a, w in zip(b(x, return_routing=True), want))
+        assert torch.equal(step(x), want[0]), "a graph of the block takes the new router up"
+    b.wr.copy_(randn(g, 8, 256))
+    b.wr = b.wr
+    assert torch.equal(b(x), fresh(b.wr)(x))
+    for bad in (randn(g, 9, 256), randn(g, 8, 128), randn(g, 8, 256).half(), randn(g, 8, 256).cpu(), None):
+        kept = b.wr
+        with pytest.raises((TypeError, ValueError), match="gate_inp_w"):
+            b.wr = bad
+        assert b.wr is kept
