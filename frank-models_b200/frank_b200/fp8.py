@@ -114,15 +114,34 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, return_norm:
 class Fp8Experts:
     """Expert weights in 8 bits: ``q`` float8_e4m3fn [E, N, K] and ``scale``
     float32 [E, ceil(N/128), ceil(K/128)], one for each 128 x 128 block; any
-    finite scales (a quantised checkpoint's are used as they are)."""
+    finite scales (a quantised checkpoint's are used as they are).  The tensors
+    are held, not copied, unless they are not contiguous or not 16-byte aligned;
+    others of the same shape may be assigned."""
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
         q = _arg(q, "Fp8Experts: q", (None, None, None), E4M3_ONLY)
         E, N, K = q.shape
         _multiple(N, "Fp8Experts: n_out")
         _multiple(K, "Fp8Experts: n_in")
-        self.q = q
-        self.scale = _arg(scale, "Fp8Experts: scale", (E, _blocks(N), _blocks(K)), F32_ONLY, q.device)
+        self._q = q
+        self.scale = scale
+
+    @property
+    def q(self) -> torch.Tensor:
+        return self._q
+
+    @q.setter
+    def q(self, q: torch.Tensor) -> None:
+        self._q = _arg(q, "Fp8Experts: q", self._q.shape, E4M3_ONLY, self._q.device)
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return self._scale
+
+    @scale.setter
+    def scale(self, scale: torch.Tensor) -> None:
+        E, N, K = self._q.shape
+        self._scale = _arg(scale, "Fp8Experts: scale", (E, _blocks(N), _blocks(K)), F32_ONLY, self._q.device)
 
     @classmethod
     def from_reference(cls, w_oie: torch.Tensor) -> "Fp8Experts":
@@ -166,8 +185,9 @@ def fp8_matmul(x, weights: Fp8Experts, offsets: torch.Tensor | None = None,
     left as they were."""
     if not isinstance(weights, Fp8Experts):
         raise TypeError(f"fp8_matmul: weights must be Fp8Experts, got {type(weights).__name__}")
-    E, N, K = weights.q.shape
-    dev = weights.q.device
+    wq = weights.q
+    E, N, K = wq.shape
+    dev = wq.device
     if out_dtype not in FLOATS:
         raise TypeError(f"fp8_matmul: unsupported output dtype {out_dtype}")
     quantised = isinstance(x, (tuple, list))
@@ -188,12 +208,12 @@ def fp8_matmul(x, weights: Fp8Experts, offsets: torch.Tensor | None = None,
     with _on(dev):
         y = _out(out, "fp8_matmul", (R, N), out_dtype, dev)
         if quantised:
-            _lib.check(lib.frank_fp8_matmul(_ptr(q), _ptr(scale), _ptr(weights.q), _ptr(weights.scale),
+            _lib.check(lib.frank_fp8_matmul(_ptr(q), _ptr(scale), _ptr(wq), _ptr(weights.scale),
                                             _ptr(offsets), E, R, N, K, _DT[out_dtype], _ptr(y), _stream()))
         else:
             need = lib.frank_fp8_linear_workspace_size(R, K)
-            ws = weights.q.new_empty(need)
-            _lib.check(lib.frank_fp8_linear(_DT[x.dtype], _ptr(x), _ptr(weights.q), _ptr(weights.scale),
+            ws = wq.new_empty(need)
+            _lib.check(lib.frank_fp8_linear(_DT[x.dtype], _ptr(x), _ptr(wq), _ptr(weights.scale),
                                             _ptr(offsets), E, R, N, K, _DT[out_dtype], _ptr(y), _ptr(ws), need,
                                             _stream()))
     return y
@@ -230,14 +250,9 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
             raise ValueError(f"Fp8MoEFFNBlock: n_expert_used={self.k} outside [1, min({self.E}, 32)]")
         up, gate, down = (w if isinstance(w, Fp8Experts) else Fp8Experts.from_reference(w)
                           for w in (up_exps_w, gate_exps_w, down_exps_w))
-        E, F, H = up.q.shape
-        if E != self.E or tuple(gate.q.shape) != (E, F, H) or tuple(down.q.shape) != (E, H, F):
-            raise ValueError("Fp8MoEFFNBlock: expert weight shapes disagree")
-        if not up.q.device == gate.q.device == down.q.device:
-            raise ValueError("Fp8MoEFFNBlock: expert weights are on different devices")
-        self.H, self.F = H, F
-        self.w_up, self.w_gate, self.w_down = up, gate, down
+        _, self.F, self.H = up.q.shape
         self.device = up.q.device
+        self.w_up, self.w_gate, self.w_down = up, gate, down
         self.wr_pack = None
         self.wr = gate_inp_w
 
@@ -259,8 +274,26 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
                 self.wr_pack.copy_(pack)
         self._wr = wr
 
+    def _fit(self, weights: Fp8Experts, name: str, n_out: int, n_in: int) -> Fp8Experts:
+        """Weights for this block: the kernels read them by the block's sizes."""
+        if not isinstance(weights, Fp8Experts):
+            raise TypeError(f"Fp8MoEFFNBlock: {name} must be Fp8Experts, got {type(weights).__name__}")
+        q = weights.q
+        if tuple(q.shape) != (self.E, n_out, n_in):
+            raise ValueError(f"Fp8MoEFFNBlock: {name} has shape {tuple(q.shape)}, expected "
+                             f"[{self.E}, {n_out}, {n_in}]")
+        if q.device != self.device:
+            raise ValueError(f"Fp8MoEFFNBlock: {name} is on device {q.device}, expected {self.device}")
+        return weights
+
+    w_up = property(lambda self: self._up, lambda self, w: setattr(self, "_up", self._fit(w, "w_up", self.F, self.H)))
+    w_gate = property(lambda self: self._gate,
+                      lambda self, w: setattr(self, "_gate", self._fit(w, "w_gate", self.F, self.H)))
+    w_down = property(lambda self: self._down,
+                      lambda self, w: setattr(self, "_down", self._fit(w, "w_down", self.H, self.F)))
+
     def _weights(self):
-        return [_ptr(t) for w in (self.w_up, self.w_gate, self.w_down) for t in (w.q, w.scale)]
+        return [_ptr(t) for w in (self._up, self._gate, self._down) for t in (w._q, w._scale)]
 
     def workspace_bytes(self, T: int) -> int:
         return _lib.load().frank_fp8_moe_workspace_size(T, self.H, self.F, self.E, self.k)

@@ -178,3 +178,48 @@ def test_linear_refuses_before_it_launches(lib):
     _refused(lib, linear(None, 1, 4, 128, -16), "multiple")
     assert linear(None, 1, 4, 128, 128, ptr=None) == _lib.ENOSPC
     assert linear(None, 1, 1 << 20, 128, 128) == _lib.ENOSPC
+
+
+def _experts_stand_in(E, N, K):
+    """An Fp8Experts without a device: the checks of assignments read shapes and devices only."""
+    import frank_b200 as fb
+
+    w = fb.Fp8Experts.__new__(fb.Fp8Experts)
+    w._q = torch.zeros((E, N, K), dtype=torch.uint8).view(torch.float8_e4m3fn)
+    w._scale = torch.ones((E, -(-N // 128), -(-K // 128)))
+    return w
+
+
+def test_assigned_weights_are_checked():
+    """Weights given to a block after its construction have to fit it: the kernels read them by the block's sizes."""
+    import frank_b200 as fb
+
+    b = fb.Fp8MoEFFNBlock.__new__(fb.Fp8MoEFFNBlock)
+    b.E, b.H, b.F, b.device = 4, 256, 128, torch.device("cpu")
+    good = {"w_up": _experts_stand_in(4, 128, 256), "w_gate": _experts_stand_in(4, 128, 256),
+            "w_down": _experts_stand_in(4, 256, 128)}
+    for name, w in good.items():
+        setattr(b, name, w)
+        assert getattr(b, name) is w
+        for bad in ((3, 128, 256), (4, 256, 256), (4, 128, 128), (4, 112, 256)):
+            with pytest.raises(ValueError, match="shape"):
+                setattr(b, name, _experts_stand_in(*bad))
+        with pytest.raises(TypeError, match="Fp8Experts"):
+            setattr(b, name, w._q)
+        assert getattr(b, name) is w
+    b.device = torch.device("cuda", 0)
+    with pytest.raises(ValueError, match="device"):
+        b.w_up = good["w_up"]
+
+
+def test_assigned_tensors_of_weights_are_checked():
+    """An Fp8Experts keeps its sizes: another q or scale has to fit them."""
+    w = _experts_stand_in(2, 144, 256)
+    for bad in (torch.zeros(2, 144, 128), torch.zeros(2, 144, 256)):
+        with pytest.raises((TypeError, ValueError)):
+            w.q = bad.to(torch.float8_e4m3fn if bad.shape[2] == 128 else torch.float32)
+    with pytest.raises(ValueError, match="shape"):
+        w.scale = torch.ones(2, 1, 2)
+    with pytest.raises(TypeError, match="dtype"):
+        w.scale = torch.ones(2, 2, 2, dtype=torch.float64)
+    assert tuple(w.q.shape) == (2, 144, 256) and tuple(w.scale.shape) == (2, 2, 2)

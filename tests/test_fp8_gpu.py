@@ -645,3 +645,21 @@ def test_router_replaced(T):
         with pytest.raises((TypeError, ValueError), match="gate_inp_w"):
             b.wr = bad
         assert b.wr is kept
+
+
+def test_assigned_weights_fit_the_block():
+    """Weights of other sizes are refused; tensors exchanged inside Fp8Experts are read by the next call."""
+    g = gen(28)
+    b, c = (block(g, 5, 256, 128, 4, 2) for _ in range(2))
+    x = randn(g, 5, 256, dtype=BF16)
+    with pytest.raises(ValueError, match="shape"):
+        fb.Fp8MoEFFNBlock(b.wr, b.w_up, b.w_down, b.w_down, 4, 2, True)
+    for bad in (weights(g, 3, 128, 256), weights(g, 4, 112, 256), b.w_down):
+        with pytest.raises(ValueError, match="shape"):
+            b.w_up = bad
+    with pytest.raises(ValueError, match="shape"):
+        b.w_up.q = b.w_down.q
+    c.wr = b.wr
+    for mine, other in ((b.w_up, c.w_up), (b.w_gate, c.w_gate), (b.w_down, c.w_down)):
+        mine.q, mine.scale = other.q, other.scale
+    assert torch.equal(b(x), c(x))
