@@ -82,7 +82,9 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 // scale = 2^p and 1/scale for the largest |v| of a block, given as bits
 // (integer maxima keep NaN above infinity above every number).  448 = 1.75 * 2^8:
 // amax = 1.m * 2^e <= 448 * 2^p  <=>  p >= e - 8 + (1.m > 1.75).
-// p >= -110 keeps 1/scale and the products of two scales inside fp32's range.
+// p is in [-110, 120], so scale and 1/scale are normal numbers.  A product's two scales are
+// multiplied first (one FMA a value then): frank_fp8.h has the range that this leaves the
+// weights' scales.
 struct BlockScale {
   float scale, inv;
 };

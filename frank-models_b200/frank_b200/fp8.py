@@ -113,9 +113,9 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, return_norm:
 
 class Fp8Experts:
     """Expert weights in 8 bits: ``q`` float8_e4m3fn [E, N, K] and ``scale``
-    float32 [E, ceil(N/128), ceil(K/128)], one for each 128 x 128 block; any
-    finite scales (a quantised checkpoint's are used as they are).  The tensors
-    are held, not copied, unless they are not contiguous or not 16-byte aligned;
+    float32 [E, ceil(N/128), ceil(K/128)], one for each 128 x 128 block (a quantised
+    checkpoint's are used as they are; magnitudes below 2^8 serve every row).  The
+    tensors are held, not copied, unless they are not contiguous or not 16-byte aligned;
     others of the same shape may be assigned."""
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):

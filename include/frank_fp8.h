@@ -16,8 +16,12 @@
  * so that v / 2^p is exact and the value is rounded once.  A block that holds
  * a NaN or an infinity gets the scale NaN: every product with it is NaN.
  *
- * 8-bit weights.  e4m3 q [E, N, K] and one fp32 scale (any finite value) for each
- * 128 x 128 block: scale [E, ceil(N/128), ceil(K/128)].
+ * 8-bit weights.  e4m3 q [E, N, K] and one fp32 scale for each 128 x 128 block:
+ * scale [E, ceil(N/128), ceil(K/128)].  Products form (row's scale) * (weights'
+ * scale) in fp32.  A row's scale is in [2^-110, 2^120], so weights' scales of
+ * magnitude below 2^8 never overflow there; a larger one gives infinities or NaN
+ * with those rows whose scale takes the product to 2^128.  A product of
+ * scales below 2^-126 keeps fewer bits: an error of up to 2^-125 for each block of K.
  *
  * K, N, H and F are multiples of 16; the last block may be short.
  */

@@ -663,3 +663,27 @@ def test_assigned_weights_fit_the_block():
     for mine, other in ((b.w_up, c.w_up), (b.w_gate, c.w_gate), (b.w_down, c.w_down)):
         mine.q, mine.scale = other.q, other.scale
     assert torch.equal(b(x), c(x))
+
+
+@pytest.mark.parametrize("R", [3, 300])
+def test_scales_at_the_ends_of_their_range(R):
+    """Rows of the largest scale with weights' scales just below 2^8: partial sums of 0 stay 0.  Rows and weights whose
+    scales multiply to less than 2^-126: an absolute error of 2^-125 a block of K, and half a step of fp32's least number
+    for each of its additions."""
+    g = gen(29)
+    K, N = 400, 272
+    w = weights(g, 1, N, K)
+    w.scale.fill_(255.0)
+    w.q[:, :, :128] = torch.zeros((1, N, 128), device=DEV).to(E4M3)
+    x = randn(g, R, K, std=1e-3)
+    x[:, 3] = 3.3e38
+    q, s = fb.quantize_fp8(x)
+    assert s.max() == 2.0 ** 120
+    within(fb.fp8_matmul((q, s), w, out_dtype=F32), *Q.product(values(q, s), dense(w)[0]))
+    w = weights(g, 1, N, K)
+    for scale in (1e-5, 1e-10, 1e-20, 1e-38):
+        w.scale.fill_(scale)
+        q, s = fb.quantize_fp8(randn(g, R, K, std=1e-33))
+        assert s.min() == 2.0 ** -110
+        want, bound = Q.product(values(q, s), dense(w)[0])
+        within(fb.fp8_matmul((q, s), w, out_dtype=F32), want, bound + 4 * (2.0 ** -125 + 2.0 ** -150))
