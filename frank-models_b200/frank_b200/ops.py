@@ -352,8 +352,13 @@ def moe_ffn_host(block, x_host: torch.Tensor, y_host: torch.Tensor, chunks: int 
     (pinned host tensors).  The tokens are split into ``chunks`` pieces that
     flow through three streams -- host-to-device copy, the block on the
     current stream, device-to-host copy -- so the PCIe transfers of one chunk
-    overlap the compute of its neighbours.  Tokens are independent in the
-    block, so the result equals one call on all T tokens bit for bit.
+    overlap the compute of its neighbours.  The result is that of one block
+    call for each chunk, bit for bit.  Tokens are independent in the block, so
+    it is also that of one call on all T tokens as far as the block sums alike
+    for any number of tokens.  Blocks choose kernels by the number of tokens
+    of a call: :class:`Fp8MoEFFNBlock` has other orders of sums for few tokens
+    than for many, and values next to a rounding border or near-tied experts
+    may then fall on the other side.
     x_dev / y_dev: optional device staging buffers of the full size
     (allocated when absent).  No host synchronisation.  Returns a CUDA event
     that completes when y_host is written; with ``order_copy_out`` (default)

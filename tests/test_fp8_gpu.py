@@ -687,3 +687,22 @@ def test_scales_at_the_ends_of_their_range(R):
         assert s.min() == 2.0 ** -110
         want, bound = Q.product(values(q, s), dense(w)[0])
         within(fb.fp8_matmul((q, s), w, out_dtype=F32), want, bound + 4 * (2.0 ** -125 + 2.0 ** -150))
+
+
+@pytest.mark.parametrize("T,chunks", [(200, 4), (130, 2), (9, 3)])
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+def test_host_chunks_across_the_rule(T, chunks, out_dtype):
+    """Tokens from the host in chunks that take the few tokens' kernels, where one call for all takes a prompt's: the
+    bits of a call for each chunk, and every chunk within the bounds of the definition for the routing that it took,
+    which is the strict one but for near ties."""
+    g = gen(T)
+    b = block(g, T, 256, 128, 16, 4, out_dtype=out_dtype)
+    x = randn(g, T, 256, dtype=BF16)
+    xh, yh = x.cpu().pin_memory(), torch.zeros((T, 256), dtype=out_dtype).pin_memory()
+    ops.moe_ffn_host(b, xh, yh, chunks=chunks).synchronize()
+    bounds = [T * i // chunks for i in range(chunks + 1)]
+    for lo, hi in zip(bounds, bounds[1:]):
+        y, rw, rid = b(x[lo:hi], return_routing=True)
+        assert torch.equal(yh[lo:hi], y.cpu())
+        strict_route(x[lo:hi].double().cpu().numpy(), b.wr.cpu().numpy(), rw.cpu().numpy(), rid.cpu().numpy(), 4, True)
+        within(y, *want_moe(b, x[lo:hi], rw, rid))
