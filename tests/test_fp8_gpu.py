@@ -706,3 +706,54 @@ def test_host_chunks_across_the_rule(T, chunks, out_dtype):
         assert torch.equal(yh[lo:hi], y.cpu())
         strict_route(x[lo:hi].double().cpu().numpy(), b.wr.cpu().numpy(), rw.cpu().numpy(), rid.cpu().numpy(), 4, True)
         within(y, *want_moe(b, x[lo:hi], rw, rid))
+
+
+@pytest.mark.parametrize("T,H,F,E,k", [(3, 16384, 128, 8, 2), (5, 7168, 128, 256, 8), (2, 12304, 144, 16, 4),
+                                       (64, 8208, 128, 24, 3), (70, 16384, 144, 8, 2), (90, 7168, 128, 256, 8)])
+def test_long_rows_and_many_experts(T, H, F, E, k):
+    """Rows up to 16384 and 256 experts: the router's slices of several blocks, the widest sums of squares and top-k."""
+    g = gen(T + H)
+    b = block(g, T, H, F, E, k, out_dtype=F32)
+    b.wr = randn(g, E, H, std=0.02)
+    # rows of +-1 have the mean square 1 exactly, so with eps = 0 and weights in bf16 every kernel's norm is res * nw
+    res = torch.where(randn(g, T, H) > 0, 1.0, -1.0)
+    nw, pw = (1 + randn(g, H, std=0.1)).to(BF16).float(), 1 + randn(g, H, std=0.1)
+    x = (res * nw).to(BF16)
+    assert torch.equal(fb.rms_norm_fp8(res, nw, 0.0, return_norm=True)[2], x)
+    y, rw, rid = b(x, return_routing=True)
+    _, _, near, differ = strict_route(x.double().cpu().numpy(), b.wr.cpu().numpy(), rw.cpu().numpy(),
+                                      rid.cpu().numpy(), k, True)
+    print(f"near-tied {near}, routed differently {differ} of {T}")
+    within(y, *want_moe(b, x, rw, rid))
+    out, rw2, rid2 = b.sublayer(res, nw, 0.0, post_norm_w=pw, return_routing=True)
+    assert torch.equal(rw2, rw) and torch.equal(rid2, rid)
+    assert torch.equal(out, fb.post_norm_residual(y, res, pw, 0.0))
+    assert ops.read_device_error() == 0
+
+
+@pytest.mark.parametrize("T", [3, 40, 100, 200])
+@pytest.mark.parametrize("wr_dtype", [F32, BF16])
+def test_router_weights_as_they_are(T, wr_dtype):
+    """The C entries take the router in fp32 or bf16 without a pack: the bits of the packed call."""
+    from frank_b200 import _lib
+
+    g = gen(T + 30)
+    H, F, E, k = 272, 144, 32, 4
+    b = block(g, T, H, F, E, k)
+    wr = randn(g, E, H, std=0.05, dtype=wr_dtype)
+    b.wr = wr
+    x = randn(g, T, H, dtype=BF16)
+    nw = 1 + randn(g, H, std=0.1)
+    lib, p = _lib.load(), lambda t: t.data_ptr()
+    w = [p(t) for e in (b.w_up, b.w_gate, b.w_down) for t in (e.q, e.scale)]
+    ws = torch.empty(b.workspace_bytes(T), dtype=torch.uint8, device=DEV)
+    dt = {F32: _lib.F32, BF16: _lib.BF16}[wr_dtype]
+    st = torch.cuda.current_stream().cuda_stream
+    y, rw, rid = torch.empty_like(x), torch.empty(k, T, device=DEV), torch.empty(k, T, dtype=torch.int32, device=DEV)
+    _lib.check(lib.frank_fp8_moe_block(p(x), dt, p(wr), *w, T, E, k, H, F, 1, _lib.BF16, p(y), p(rw), p(rid), p(ws),
+                                       ws.numel(), st))
+    want = b(x, return_routing=True)
+    assert torch.equal(y, want[0]) and torch.equal(rw, want[1]) and torch.equal(rid, want[2])
+    _lib.check(lib.frank_fp8_moe_sublayer(_lib.BF16, p(x), p(nw), 1e-5, dt, p(wr), *w, T, E, k, H, F, 1, None, None, 1,
+                                          1.0, p(y), None, None, p(ws), ws.numel(), st))
+    assert torch.equal(y, b.sublayer(x, nw, 1e-5))
