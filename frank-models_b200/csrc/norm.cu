@@ -173,41 +173,34 @@ norm_rows_kernel(const NormRows a) {
   }
 }
 
-// y[t] = sum_j d[slot_pos[j]] alone: eight columns a thread, eight rows at a time.
+// y[t] = sum_j d[slot_pos[j]] alone: four columns a thread, eight rows at a time.
 template <class TY>
 __global__ void __launch_bounds__(128) combine_slots_kernel(const NormRows a) {
   pdl_wait();
   pdl_launch();
   const int64_t t = blockIdx.x;
-  const int h = (blockIdx.y * 128 + threadIdx.x) * 8;
+  const int h = (blockIdx.y * 128 + threadIdx.x) * 4;
   if (h >= a.H) return;
-  float v[8] = {};
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int j0 = 0; j0 < a.k; j0 += 8) {
-    float4 u[8][2];
+    float4 u[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       if (j0 + q < a.k) {
         const int64_t s = (int64_t)(j0 + q) * a.T + t;
-        const float* row = a.d + (a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s) * a.H + h;
-        u[q][0] = *reinterpret_cast<const float4*>(row);
-        u[q][1] = *reinterpret_cast<const float4*>(row + 4);
+        const int64_t row = a.slot_pos != nullptr ? (int64_t)a.slot_pos[s] : s;
+        u[q] = *reinterpret_cast<const float4*>(a.d + row * a.H + h);
       }
     }
 #pragma unroll
     for (int q = 0; q < 8; ++q)
-      if (j0 + q < a.k) {
-        v[0] += u[q][0].x, v[1] += u[q][0].y, v[2] += u[q][0].z, v[3] += u[q][0].w;
-        v[4] += u[q][1].x, v[5] += u[q][1].y, v[6] += u[q][1].z, v[7] += u[q][1].w;
-      }
+      if (j0 + q < a.k) v.x += u[q].x, v.y += u[q].y, v.z += u[q].z, v.w += u[q].w;
   }
   TY* y = static_cast<TY*>(a.out) + t * a.H + h;
-  if constexpr (sizeof(TY) == 4) {
-    *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(y + 4) = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    *reinterpret_cast<uint4*>(y) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                              pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-  }
+  if constexpr (sizeof(TY) == 4)
+    *reinterpret_cast<float4*>(y) = v;
+  else
+    *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
 }
 
 template <int GS, int V>
@@ -219,7 +212,7 @@ cudaError_t launch_rows(const NormRows& a, cudaStream_t st) {
 }
 
 cudaError_t launch_combine_slots(const NormRows& a, cudaStream_t st) {
-  const dim3 grid((unsigned)a.T, (unsigned)((a.H + 1023) / 1024));
+  const dim3 grid((unsigned)a.T, (unsigned)((a.H + 511) / 512));
   if (a.out_dtype == FRANK_F32)
     return launch_chained(combine_slots_kernel<float>, grid, dim3(128), 0, st, 1, a);
   return launch_chained(combine_slots_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, 1, a);
@@ -233,8 +226,7 @@ int launch_norm_rows(const NormRows& a, cudaStream_t st) {
   if (a.T == 0) return FRANK_OK;
   const int64_t H4 = a.H / 4;
   cudaError_t e;
-  if (a.d != nullptr && a.post_w == nullptr && a.gate == nullptr && a.residual == nullptr && a.next_w == nullptr &&
-      a.H % 8 == 0)
+  if (a.d != nullptr && a.post_w == nullptr && a.gate == nullptr && a.residual == nullptr && a.next_w == nullptr)
     e = launch_combine_slots(a, st);
   else if (H4 <= 32) e = launch_rows<32, 1>(a, st);
   else if (H4 <= 64) e = launch_rows<32, 2>(a, st);
