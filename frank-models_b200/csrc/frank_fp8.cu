@@ -38,11 +38,13 @@ struct Fp8Weights {
   const float *s_up, *s_gate, *s_down;
 };
 
-// A few tokens: the weights bound the call, and few_fp8.cu reads them once.  It takes 32
-// tokens of an expert at once, so the experts must not have many more on average:
-// 64 tokens, 2 of 8 experts of 4096 x 14336: 268 us there and 274 us by the
-// sorted rows; 2 of 4 experts of 4096 x 4096: 101 and 71 us; 8 of 128 experts of
-// 2048 x 768: 132 and 165 us; one token, 8 of 128: 31 and 61 us.
+// A few tokens: the weights bound the call, and few_fp8.cu reads them once for each 32 slots
+// of an expert, so the experts must not have many more on average.  Graph of experts() from a
+// cold L2, us there / by the sorted rows, at 8, 16, 20, 24, 26, 28 and 32 slots an expert:
+//   2 of 4 of 4096 x 4096    59/72  61/72  63/72  64/72  64/72  78/72  90/74
+//   8 of 16 of 2048 x 2048   61/74  63/74  66/74  66/74  66/74  82/74  88/74
+//   4 of 8 of 4096 x 14336   272/287  266/274  268/272  274/274  279/279  279/274  375/276
+// 8 of 128 of 2048 x 768, 64 tokens (4 an expert): 131 / 158.
 static bool few_tokens(int64_t T, int64_t E, int64_t k, int64_t H, int64_t F) {
   return T <= kFewMaxT && k * T <= kFewMaxSlots && k * T <= 24 * E && q_blocks(H) <= kFewMaxBlocksH &&
          q_blocks(F) <= kFewMaxBlocksF;

@@ -23,11 +23,16 @@
 // 96 bytes a cycle from shared memory and the copies write as many, of 128), without
 // MMAs and copies the epilogue takes 965; what bounds it is the way of a TMEM
 // buffer from the last MMA through the loads to the next MMA, with only two buffers.
-// No faster: pairs of CTAs (cta_group::2, 256 x 256 tiles: 465 us, but 65536 sorted rows
-// of 128 experts 719 against 671 us for the expert FFN), sixteen epilogue warps (724 us),
-// halves of 128 columns with barriers of their own (581 us), the next K block's TMEM
-// loads before the last FMAs (523 us), the scales by warps 2 and 3 through shared
-// memory (483 us).
+// These are times at 1965 MHz; in a row for longer than about 0.1 s the power cap takes the
+// clock to 1.6 GHz and the time to 550 us, called from Python or from a graph alike.
+// Pairs of CTAs (cta_group::2, 256 x 256 tiles) take 465 us here, but 719 against 671 us
+// for an expert FFN of 65536 sorted rows of 128 experts, so tiles are single.  No faster:
+// sixteen epilogue warps (724 us), halves of 128 columns with barriers of their own (581
+// us), the next K block's TMEM loads before the last FMAs (523 us), the scales by
+// warps 2 and 3 through shared memory (483 us).
+// Weights' scales may be any fp32 numbers here.  Where all are powers of two, as this
+// library's own quantiser makes them, the MMA could apply them itself and sum all
+// of K in TMEM; there is no such form.
 // Every wait is bounded (about 2 s); on expiry the CTA records FRANK_ETIMEOUT in
 // the device error word and unwinds, freeing its TMEM.
 #include <cuda.h>

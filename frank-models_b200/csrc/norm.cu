@@ -14,6 +14,8 @@
 // 16384 rows of 4096, fp32 y, bf16 residual and next: 106 us,
 // 6.36 TB/s.  Slower: two vectors a thread (128 us), a run of rows
 // a block with the weights in shared memory and the next row on its way (217 us).
+// With the 8-bit form instead, 8192 rows of 4096: bf16 in 37 us (15.5 for the bytes), fp32 in
+// 38 us (25.6): two passes of reductions a row, which is short work for a block of 256 threads.
 #include "fp8.cuh"
 
 namespace {

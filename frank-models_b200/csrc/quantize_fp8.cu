@@ -6,6 +6,9 @@
 // row under way, neighbouring warps have neighbouring rows, whose scales are
 // neighbours.  With slot_pos a row is read once and written to each of its k
 // expert-sorted places: the gather of the bf16 path costs no pass of its own.
+// 8192 x 4096: bf16 24 us (15.5 for the bytes), fp32 28 us (25.6); 8192 rows of 2048 to
+// 8 places each 34 us (25.6).  What is over the bytes is the start of each warp: one row
+// segment, then its end.
 #include "fp8.cuh"
 
 namespace {
@@ -87,7 +90,8 @@ quantize_rows_kernel(const TX* x, int64_t T, int64_t K, int nb, const int32_t* s
 
 // [O, I, E] -> [E, O, I]: one block for each 128 x 128 block of (o, i) and all
 // experts.  The first pass finds each expert's maximum (values of one o are
-// contiguous over (i, e)), the second writes runs along i.  Done once.
+// contiguous over (i, e)) with an atomic on shared memory a value, the second writes
+// runs along i.  Done once: 768 x 2048 x 128 in 6.4 ms, 4096 x 4096 x 8 in 0.7 ms.
 template <class TX>
 __global__ void __launch_bounds__(256)
 prepack_fp8_kernel(const TX* __restrict__ src, int64_t O, int64_t I, int64_t E, uint8_t* __restrict__ q,

@@ -324,7 +324,7 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
     def experts(self, x: torch.Tensor, route_w: torch.Tensor, route_ids: torch.Tensor,
                 out: torch.Tensor | None = None, check_ids: bool = False) -> torch.Tensor:
         """The expert FFN with the routing given: x [T, H] bfloat16, route_w
-        float32 [k, T], route_ids int32 [k, T] (distinct for each token) -> y
+        float32 [k, T], route_ids int32 [k, T] (one named twice counts twice) -> y
         [T, H] = sum_j route_w[j] * down(gate(x) * silu(up(x))).  With check_ids,
         ids outside [0, E) raise FrankError(EIDS) (this synchronises the stream);
         without, they are clamped."""

@@ -89,8 +89,8 @@ int frank_fp8_linear(int x_dtype, const void* x, const void* w,
  * The expert FFN with the routing given: x [T, H] bf16 is quantised,
  *   h = gate(x) * silu(up(x))   (fp32, then quantised in blocks of 128 of F)
  *   y[t] = sum_j route_w[j, t] * down(h[j, t])     (fp32, j in order; rounded once)
- * route_w [k, T] fp32, route_ids [k, T] int32 in [0, E), the ids of one token
- * distinct; y [T, H] in y_dtype.  An id outside [0, E) is clamped and recorded
+ * route_w [k, T] fp32, route_ids [k, T] int32 in [0, E) (an id that a token names
+ * twice counts twice); y [T, H] in y_dtype.  An id outside [0, E) is clamped and recorded
  * in *err_flag (device int32, zeroed by the caller; may be NULL).
  * Workspace: frank_fp8_moe_workspace_size(T, H, F, E, k) bytes, no header, any
  * contents; calls that share one must not overlap.
