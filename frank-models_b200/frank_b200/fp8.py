@@ -237,7 +237,8 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
     The expert weights are :class:`Fp8Experts` or the reference layouts (up/gate
     [F, H, E], down [H, F, E]), which are quantised once here.  A call reads the
     expert weights that ``w_up``, ``w_gate`` and ``w_down`` are then, in-place changes
-    included, and the router that ``wr`` was when it was last assigned."""
+    included, and the router that ``wr`` was when it was last assigned.  A captured
+    graph goes on reading the expert tensors that it was captured with."""
 
     def __init__(self, gate_inp_w, up_exps_w, gate_exps_w, down_exps_w, n_expert: int, n_expert_used: int,
                  normalize_weights: bool, out_dtype: torch.dtype = torch.float32):
@@ -267,11 +268,11 @@ class Fp8MoEFFNBlock(ops.MoEFFNBlock):
     def wr(self, gate_inp_w: torch.Tensor) -> None:
         wr = _arg(gate_inp_w, "gate_inp_w", (self.E, self.H), device=self.device)
         with _on(self.device):
-            pack = ops.router_pack(wr)
             if self.wr_pack is None:
-                self.wr_pack = pack
+                self.wr_pack = ops.router_pack(wr)
             else:
-                self.wr_pack.copy_(pack)
+                _lib.check(_lib.load().frank_router_pack(_DT[wr.dtype], _ptr(wr), self.E, self.H, _ptr(self.wr_pack),
+                                                         _stream()))
         self._wr = wr
 
     def _fit(self, weights: Fp8Experts, name: str, n_out: int, n_in: int) -> Fp8Experts:

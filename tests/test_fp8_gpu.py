@@ -757,3 +757,32 @@ def test_router_weights_as_they_are(T, wr_dtype):
     _lib.check(lib.frank_fp8_moe_sublayer(_lib.BF16, p(x), p(nw), 1e-5, dt, p(wr), *w, T, E, k, H, F, 1, None, None, 1,
                                           1.0, p(y), None, None, p(ws), ws.numel(), st))
     assert torch.equal(y, b.sublayer(x, nw, 1e-5))
+
+
+def test_block_of_inference_mode():
+    """A block made and called under inference mode; its router and weights are replaced and it is called outside."""
+    g = gen(31)
+    with torch.inference_mode():
+        b = block(g, 3, 256, 128, 8, 2)
+        x = randn(g, 3, 256, dtype=BF16)
+        y = b(x)
+    assert torch.equal(b(x), y)
+    c = block(g, 3, 256, 128, 8, 2)
+    b.wr, b.w_up, b.w_gate, b.w_down = c.wr, c.w_up, c.w_gate, c.w_down
+    want = c(x)
+    assert torch.equal(b(x), want)
+    with torch.inference_mode():
+        assert torch.equal(b(x), want)
+
+
+def test_graphed_host_step_takes_the_block():
+    """A step from pinned host tokens to the pinned host result as one graph: the bits of a call on the device."""
+    g = gen(32)
+    for T in (2, 80):
+        b = block(g, T, 256, 128, 16, 2)
+        step = ops.GraphedHostMoEFFN(b, T)
+        for _ in range(2):
+            x = randn(g, T, 256, dtype=BF16)
+            step.x_host.copy_(x.cpu())
+            step.replay().synchronize()
+            assert torch.equal(step.y_host, b(x).cpu())
